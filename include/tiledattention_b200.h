@@ -60,6 +60,8 @@ extern "C" {
 #define TA_DEVSTAT_TIMEOUT_EPILOG  8u
 #define TA_DEVSTAT_TIMEOUT_DRAIN   16u
 #define TA_DEVSTAT_PEER_TIMEOUT    32u  /* ta_peer_barrier: a peer did not arrive in time */
+#define TA_DEVSTAT_BAD_PAGE        64u  /* cache operators: a page id outside the cache; its tokens were not written, or read as zeros */
+#define TA_DEVSTAT_BAD_LENGTH      128u /* cache operators: a start, count or length outside its range; it was held in range */
 
 /* Largest group ta_peer_barrier / ta_lse_merge_peers serve (one NVLink domain of 8 GPUs). */
 #define TA_MAX_PEERS 8
@@ -178,6 +180,76 @@ int ta_sdpa_fwd_split_noalloc(const void* q, const void* k, const void* v, void*
                               const int64_t* v_strides, const int64_t* o_strides,
                               int dtype, int causal, float scale, int n_split,
                               unsigned int* dev_status, void* stream);
+
+/*
+ * ta_rotary — rotary positions for q and (optionally) k, one launch, asynchronous on
+ * `stream`. No reference counterpart (the reference's user applies positions before sdpa).
+ * Pair i < rotary_dim / 2 of every head at position n turns by theta = n * inv_freq[i]:
+ *   (a, b) -> magnitude * (a cos theta - b sin theta, b cos theta + a sin theta)
+ * with pair i = dims (i, rotary_dim / 2 + i), or (2 i, 2 i + 1) when interleaved; dims from
+ * rotary_dim on are copied. inverse = 1 turns the other way: the gradient of the call with
+ * inverse = 0. Angles are reduced in double, so positions may be large; the rest is fp32 with
+ * one rounding.
+ *
+ *   q, k          device, `dtype` (TA_DTYPE_F16 / BF16), [B,Hq,S,D] and [B,Hk,S,D] with
+ *                 element strides (unit dim stride); k null with Hk = 0 for q alone
+ *   q_out, k_out  outputs of the same shapes; the input itself (same strides) is allowed
+ *   positions     device int32, or int64 with positions_64 = 1, [B,S] with the two element
+ *                 strides position_strides (0 for a shared row)
+ *   inv_freq      device double [rotary_dim / 2], radians per position
+ * Bases and strides that are multiples of 16 bytes, with D a multiple of 8 and rotary_dim of
+ * 16 (interleaved: 8), take 16-byte accesses; everything else runs element by element.
+ */
+int ta_rotary(const void* q, void* q_out, const int64_t* q_strides, const int64_t* q_out_strides,
+              int Hq, const void* k, void* k_out, const int64_t* k_strides,
+              const int64_t* k_out_strides, int Hk, int B, int S, int D, int rotary_dim,
+              const void* positions, int positions_64, const int64_t* position_strides,
+              const double* inv_freq, int interleaved, int inverse, float magnitude, int dtype,
+              void* stream);
+
+/*
+ * The paged 8-bit key/value cache (no reference counterpart): k_pages and v_pages are device
+ * e4m3 codes [num_pages, Hkv, page, D], contiguous and 16-byte aligned, with page 16, 32, 64
+ * or 128 and D a multiple of 16 up to 256; k_scale and v_scale are device float32
+ * [num_pages, Hkv], powers of two 2^e, -50 <= e <= 50: a value is code * scale. Token i of
+ * sequence b is row i % page of page table[b * table_stride + i / page] (device int32, width
+ * table_width). Page ids outside [0, num_pages) set TA_DEVSTAT_BAD_PAGE and are neither read
+ * nor written; starts, counts and lengths outside their range set TA_DEVSTAT_BAD_LENGTH and
+ * are held in range.
+ *
+ * ta_kv8_append — writes tokens starts[b] .. starts[b] + counts[b] - 1 of every sequence from
+ * k, v [B,Hkv,T,D] (counts null: all T; rows from counts[b] on are not read). A page whose first
+ * row is among them begins anew with the least scale 2^e that holds its new tokens' largest
+ * finite value (amax <= 448 * 2^e); one that already holds tokens keeps the larger of its
+ * scale and the needed one, and where that grows its old codes are rounded again. Codes are
+ * x / scale, rounded to nearest even, saturating at +-448; NaN stays NaN. Rows behind the last
+ * new token stay as they are. A page that two sequences write in one call has no defined
+ * content.
+ */
+int ta_kv8_append(const void* k, const void* v, const int64_t* k_strides, const int64_t* v_strides,
+                  void* k_pages, void* v_pages, float* k_scale, float* v_scale, int num_pages,
+                  int page, const int* table, int64_t table_stride, int table_width,
+                  const int* starts, const int* counts, int B, int Hkv, int T, int D, int dtype,
+                  unsigned int* dev_status, void* stream);
+
+/*
+ * ta_sdpa_kv8 — o = softmax(scale q K^T + mask) V of T query rows per sequence over the cached
+ * tokens [0, lengths[b]) of sequence b, for Hq = G * Hkv query heads (head h reads cache head
+ * h / G). counts[b] (null: T) of the T rows are real; they are the sequence's last tokens, so
+ * with causal = 1 row t sees keys [0, lengths[b] - counts[b] + t]; with causal = 0 all
+ * lengths[b]. Rows without a key, and rows from counts[b] on, give o = 0 and lse = -inf.
+ *   q, o        device, `dtype`, [B,Hq,T,D] with element strides (multiples of 16 bytes)
+ *   lse         optional device float32 [B,Hq,T], natural log
+ *   workspace   device memory of ta_sdpa_kv8_workspace(...) bytes, 16-byte aligned, for this
+ *               call alone until it has run; nothing in it needs clearing
+ */
+int64_t ta_sdpa_kv8_workspace(int B, int Hq, int Hkv, int T, int D);
+int ta_sdpa_kv8(const void* q, const int64_t* q_strides, void* o, const int64_t* o_strides,
+                float* lse, const void* k_pages, const void* v_pages, const float* k_scale,
+                const float* v_scale, int num_pages, int page, const int* table,
+                int64_t table_stride, int table_width, const int* lengths, const int* counts,
+                int B, int Hq, int Hkv, int T, int D, int dtype, int causal, float scale,
+                void* workspace, int64_t workspace_bytes, unsigned int* dev_status, void* stream);
 
 /*
  * ta_device_supported — 1 if `device` is a compute-capability 10.0 GPU this build runs

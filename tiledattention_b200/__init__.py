@@ -19,7 +19,9 @@ from ._errors import (
     UnsupportedPlatformError,
 )
 from ._version import __version__
+from .kv_cache import KVCache8, kv_cache_alloc, kv_cache_append, sdpa_kv_cache
 from .launch import check_device_status
+from .rotary import rotary, rotary_frequencies
 from .sdpa import sdpa, sdpa_partial, sdpa_split_kv, sdpa_with_lse
 
 __all__ = [
@@ -28,6 +30,12 @@ __all__ = [
     "sdpa_with_lse",
     "sdpa_split_kv",
     "sdpa_partial",
+    "rotary",
+    "rotary_frequencies",
+    "KVCache8",
+    "kv_cache_alloc",
+    "kv_cache_append",
+    "sdpa_kv_cache",
     "check_device_status",
     "TiledAttentionError",
     "UnsupportedPlatformError",

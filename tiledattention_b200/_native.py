@@ -38,6 +38,8 @@ DEVSTAT_BITS = {
     8: "epilogue wait timed out",
     16: "drain of in-flight copies/MMAs timed out",
     32: "peer barrier timed out (a peer GPU did not arrive)",
+    64: "a page id outside the cache (its tokens were not written, or read as zeros)",
+    128: "a start, count or length outside its range (it was held in range)",
 }
 
 # Every symbol include/tiledattention_b200.h declares, with its ctypes signature.
@@ -93,6 +95,40 @@ SIGNATURES = {
             _I64P, _I64P, _I64P, _I64P,
             ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int,
             ctypes.c_void_p, ctypes.c_void_p,
+        ],
+    ),
+    "ta_rotary": (
+        ctypes.c_int,
+        [
+            ctypes.c_void_p, ctypes.c_void_p, _I64P, _I64P, ctypes.c_int,
+            ctypes.c_void_p, ctypes.c_void_p, _I64P, _I64P, ctypes.c_int,
+            ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+            ctypes.c_void_p, ctypes.c_int, _I64P, ctypes.c_void_p,
+            ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_int, ctypes.c_void_p,
+        ],
+    ),
+    "ta_kv8_append": (
+        ctypes.c_int,
+        [
+            ctypes.c_void_p, ctypes.c_void_p, _I64P, _I64P,
+            ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+            ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
+            ctypes.c_void_p, ctypes.c_void_p,
+            ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+            ctypes.c_void_p, ctypes.c_void_p,
+        ],
+    ),
+    "ta_sdpa_kv8_workspace": (ctypes.c_int64, [ctypes.c_int] * 5),
+    "ta_sdpa_kv8": (
+        ctypes.c_int,
+        [
+            ctypes.c_void_p, _I64P, ctypes.c_void_p, _I64P, ctypes.c_void_p,
+            ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+            ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
+            ctypes.c_void_p, ctypes.c_void_p,
+            ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+            ctypes.c_int, ctypes.c_int, ctypes.c_float,
+            ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
         ],
     ),
     "ta_device_supported": (ctypes.c_int, [ctypes.c_int]),
@@ -205,6 +241,8 @@ def load_fast_launch(lib):
         addr = lambda fn: ctypes.cast(fn, ctypes.c_void_p).value  # noqa: E731
         mod.set_entry(addr(lib.ta_sdpa_fwd))
         mod.bind_ops(addr(lib.ta_sdpa_fwd_partial), addr(lib.ta_last_error))
+        mod.bind_serving(addr(lib.ta_rotary), addr(lib.ta_kv8_append),
+                         addr(lib.ta_sdpa_kv8_workspace), addr(lib.ta_sdpa_kv8))
         _fast = mod
         return mod
 

@@ -22,8 +22,10 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 OUT_DIR = os.path.join(PKG_DIR, "_lib")
 OUT = os.path.join(OUT_DIR, "libtiledattention_b200.so")
-SOURCES = ["capi.cu", "sdpa_fwd_sm100.cu", "sdpa_fwd_sm100_shared_kv.cu", "lse_combine.cu", "noalloc_split.cu", "peer_merge.cu"]
-HEADERS = ["sm100_ptx.cuh", "sdpa_common.cuh", "sdpa_fwd_sm100.h", "lse_combine.h", "capi_internal.h"]
+SOURCES = ["capi.cu", "sdpa_fwd_sm100.cu", "sdpa_fwd_sm100_shared_kv.cu", "lse_combine.cu", "noalloc_split.cu", "peer_merge.cu",
+           "rotary.cu", "kv8_append.cu", "sdpa_kv8.cu", "capi_serving.cu"]
+HEADERS = ["sm100_ptx.cuh", "sdpa_common.cuh", "sdpa_fwd_sm100.h", "lse_combine.h", "capi_internal.h",
+           "rotary.h", "kv8.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # One-call host launcher (CPython extension over libtorch; no device code): see
 # csrc/fast_launch.cpp.

@@ -116,6 +116,8 @@ int ta_capi_fail(int code, const char* msg) { return fail(code, "%s", msg); }
 
 void ta_capi_clear_error() { g_last_error.clear(); }
 
+int ta_capi_check_device() { return check_device(); }
+
 extern "C" {
 
 #ifdef TA_TRACE

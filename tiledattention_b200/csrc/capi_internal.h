@@ -17,6 +17,9 @@ int run_forward(const void* q, const void* k, const void* v, void* o, bool out_f
 int ta_capi_fail(int code, const char* msg);
 void ta_capi_clear_error();
 
+// TA_OK where the current device is one this build runs on.
+int ta_capi_check_device();
+
 // NVTX range named after the entry point, open for the scope (host-side launch work, seen on
 // the CPU row of nsys and by ncu --nvtx filters). Without a tool attached it costs a check.
 struct TaNvtxRange {

@@ -17,6 +17,9 @@
 // through set_entry(address) with the address of the symbol in the already-loaded native
 // library, so the two share one copy of the library's state.
 //
+// rotary(), kv8_append() and sdpa_kv8() do the same for the operators around a decoder's
+// attention: None (nothing launched) where the Python path has to raise, copy or differentiate.
+//
 // The same module registers the torch operators of the reference's native-op slot
 // (torch-ext/torch_binding.cpp:6-19: TORCH_LIBRARY + ops.impl(..., kCUDA, ...)) in C++:
 //   tiledattention_b200::sdpa_fwd(Tensor q, Tensor k, Tensor v, bool causal, float scale)
@@ -29,6 +32,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/constant_pad_nd.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -52,6 +56,10 @@ using LastErrorFn = decltype(&ta_last_error);
 SdpaFwdFn g_entry = nullptr;
 SdpaPartialFn g_partial = nullptr;
 LastErrorFn g_last_error = nullptr;
+decltype(&ta_rotary) g_rotary = nullptr;
+decltype(&ta_kv8_append) g_kv8_append = nullptr;
+decltype(&ta_sdpa_kv8_workspace) g_kv8_workspace = nullptr;
+decltype(&ta_sdpa_kv8) g_sdpa_kv8 = nullptr;
 constexpr int kMaxDevices = 64;
 unsigned int* g_status[kMaxDevices] = {};
 unsigned long long g_launches = 0;  // launches taken by this module (read by the tests)
@@ -182,6 +190,248 @@ PyObject* launch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
 }
 
+// ---------------------------------------------------------------- rotary and the 8-bit cache
+
+// bind_serving(rotary, kv8_append, sdpa_kv8_workspace, sdpa_kv8): entry points by address.
+PyObject* bind_serving(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 4) {
+    PyErr_SetString(PyExc_TypeError, "bind_serving takes four addresses");
+    return nullptr;
+  }
+  uintptr_t a[4];
+  for (int i = 0; i < 4; ++i) {
+    a[i] = static_cast<uintptr_t>(PyLong_AsUnsignedLongLong(args[i]));
+    if (PyErr_Occurred()) return nullptr;
+  }
+  g_rotary = reinterpret_cast<decltype(g_rotary)>(a[0]);
+  g_kv8_append = reinterpret_cast<decltype(g_kv8_append)>(a[1]);
+  g_kv8_workspace = reinterpret_cast<decltype(g_kv8_workspace)>(a[2]);
+  g_sdpa_kv8 = reinterpret_cast<decltype(g_sdpa_kv8)>(a[3]);
+  Py_RETURN_NONE;
+}
+
+// The tensor of a Python argument, or null.
+const at::Tensor* tensor_arg(PyObject* o) {
+  return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
+}
+
+struct Strides4 {
+  int64_t v[4];
+  explicit Strides4(const at::Tensor& t)
+      : v{t.stride(0), t.stride(1), t.stride(2), t.stride(3)} {}
+};
+
+int dtype_code(const at::Tensor& t) {
+  const auto st = t.scalar_type();
+  return st == at::kHalf ? kDtypeF16 : st == at::kBFloat16 ? kDtypeBf16 : -1;
+}
+
+bool fits_int(int64_t n) { return n > 0 && n <= INT32_MAX; }
+
+// A contiguous int32 vector of n entries on dev (unit stride where n > 1).
+bool int_vector(const at::Tensor* t, int64_t n, c10::Device dev) {
+  return t && t->dim() == 1 && t->size(0) == n && t->scalar_type() == at::kInt &&
+         t->device() == dev && (n <= 1 || t->stride(0) == 1);
+}
+
+PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 7 || g_rotary == nullptr) Py_RETURN_NONE;
+  const at::Tensor* q = tensor_arg(args[0]);
+  const bool has_k = args[1] != Py_None;
+  const at::Tensor* k = has_k ? tensor_arg(args[1]) : nullptr;
+  const at::Tensor* pos = tensor_arg(args[2]);
+  const at::Tensor* freq = tensor_arg(args[3]);
+  if (!q || (has_k && !k) || !pos || !freq) Py_RETURN_NONE;
+  if (!PyBool_Check(args[4]) || !PyFloat_Check(args[5]) || !PyBool_Check(args[6])) Py_RETURN_NONE;
+  const double magnitude = PyFloat_AS_DOUBLE(args[5]);
+  try {
+    if (q->dim() != 4 || !q->is_cuda() || !std::isfinite(magnitude)) Py_RETURN_NONE;
+    if (at::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad())))
+      Py_RETURN_NONE;
+    const int dtype = dtype_code(*q);
+    const c10::Device dev = q->device();
+    const int64_t B = q->size(0), H = q->size(1), S = q->size(2), D = q->size(3);
+    if (dtype < 0 || !fits_int(B) || !fits_int(H) || !fits_int(S) || !fits_int(D) ||
+        q->stride(3) != 1)
+      Py_RETURN_NONE;
+    if (k && (k->dim() != 4 || k->device() != dev || dtype_code(*k) != dtype || k->size(0) != B ||
+              !fits_int(k->size(1)) || k->size(2) != S || k->size(3) != D || k->stride(3) != 1))
+      Py_RETURN_NONE;
+    const auto pt = pos->scalar_type();
+    if (pos->device() != dev || (pt != at::kInt && pt != at::kLong)) Py_RETURN_NONE;
+    const bool row = pos->dim() == 1;
+    if (!(row ? pos->size(0) == S
+              : pos->dim() == 2 && (pos->size(0) == B || pos->size(0) == 1) && pos->size(1) == S))
+      Py_RETURN_NONE;
+    if (freq->device() != dev || freq->scalar_type() != at::kDouble || freq->dim() != 1 ||
+        freq->size(0) < 1 || 2 * freq->size(0) > D || (freq->size(0) > 1 && freq->stride(0) != 1))
+      Py_RETURN_NONE;
+
+    c10::cuda::CUDAGuard guard(dev);
+    at::Tensor qo = at::empty({B, H, S, D}, q->options());
+    at::Tensor ko;
+    if (k) ko = at::empty({B, k->size(1), S, D}, k->options());
+    const Strides4 qs(*q), qos(qo), ks(k ? *k : *q), kos(k ? ko : qo);
+    const int64_t ps[2] = {row || pos->size(0) == 1 ? 0 : pos->stride(0),
+                           pos->stride(row ? 0 : 1)};
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_rotary(q->data_ptr(), qo.data_ptr(), qs.v, qos.v, static_cast<int>(H),
+                  k ? k->data_ptr() : nullptr, k ? ko.data_ptr() : nullptr, k ? ks.v : nullptr,
+                  k ? kos.v : nullptr, k ? static_cast<int>(k->size(1)) : 0, static_cast<int>(B),
+                  static_cast<int>(S), static_cast<int>(D), static_cast<int>(2 * freq->size(0)),
+                  pos->data_ptr(), pt == at::kLong, ps, freq->data_ptr<double>(),
+                  args[4] == Py_True, args[6] == Py_True, static_cast<float>(magnitude), dtype,
+                  stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) Py_RETURN_NONE;
+    ++g_launches;
+    PyObject* out = PyTuple_New(2);
+    if (out == nullptr) return nullptr;
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(qo)));
+    if (k) {
+      PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(ko)));
+    } else {
+      Py_INCREF(Py_None);
+      PyTuple_SET_ITEM(out, 1, Py_None);
+    }
+    return out;
+  } catch (const std::exception&) {
+    Py_RETURN_NONE;
+  }
+}
+
+// The cache's four tensors (args) and the page table, where they are as the kernels take them.
+struct CacheArgs {
+  const at::Tensor* t[4];  // k, v, k_scale, v_scale
+  const at::Tensor* table;
+  int64_t pages, heads, page, dim;
+};
+bool cache_args(PyObject* const* args, PyObject* table, int64_t B, c10::Device dev, CacheArgs& c) {
+  for (int i = 0; i < 4; ++i) {
+    c.t[i] = tensor_arg(args[i]);
+    if (!c.t[i] || c.t[i]->device() != dev || !c.t[i]->is_contiguous() ||
+        c.t[i]->requires_grad() || c.t[i]->dim() != (i < 2 ? 4 : 2) ||
+        c.t[i]->scalar_type() != (i < 2 ? at::kFloat8_e4m3fn : at::kFloat))
+      return false;
+  }
+  c.pages = c.t[0]->size(0);
+  c.heads = c.t[0]->size(1);
+  c.page = c.t[0]->size(2);
+  c.dim = c.t[0]->size(3);
+  if (c.t[1]->sizes() != c.t[0]->sizes() || !fits_int(c.pages) || !fits_int(c.heads) ||
+      !fits_int(c.page) || !fits_int(c.dim))
+    return false;
+  for (int i = 2; i < 4; ++i)
+    if (c.t[i]->size(0) != c.pages || c.t[i]->size(1) != c.heads) return false;
+  c.table = tensor_arg(table);
+  return c.table && c.table->dim() == 2 && c.table->size(0) == B && fits_int(c.table->size(1)) &&
+         c.table->scalar_type() == at::kInt && c.table->device() == dev &&
+         (c.table->size(1) == 1 || c.table->stride(1) == 1);
+}
+
+// kv8_append(k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, table, starts, counts)
+PyObject* kv8_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 9 || g_kv8_append == nullptr) Py_RETURN_NONE;
+  const at::Tensor* k = tensor_arg(args[0]);
+  const at::Tensor* v = tensor_arg(args[1]);
+  const at::Tensor* starts = tensor_arg(args[7]);
+  const at::Tensor* counts = args[8] != Py_None ? tensor_arg(args[8]) : nullptr;
+  if (!k || !v || !starts || (args[8] != Py_None && !counts)) Py_RETURN_NONE;
+  try {
+    if (k->dim() != 4 || v->dim() != 4 || !k->is_cuda()) Py_RETURN_NONE;
+    const int dtype = dtype_code(*k);
+    const c10::Device dev = k->device();
+    const int64_t B = k->size(0), H = k->size(1), T = k->size(2), D = k->size(3);
+    if (dtype < 0 || dtype_code(*v) != dtype || v->device() != dev || v->sizes() != k->sizes() ||
+        !fits_int(B) || !fits_int(H) || !fits_int(T) || !fits_int(D) || !tma_ok(*k) || !tma_ok(*v))
+      Py_RETURN_NONE;
+    CacheArgs c;
+    if (!cache_args(args + 2, args[6], B, dev, c) || c.heads != H || c.dim != D) Py_RETURN_NONE;
+    if (!int_vector(starts, B, dev) || (counts && !int_vector(counts, B, dev))) Py_RETURN_NONE;
+    const int idx = dev.index();
+    if (idx < 0 || idx >= kMaxDevices || g_status[idx] == nullptr) Py_RETURN_NONE;
+    c10::cuda::CUDAGuard guard(dev);
+    const Strides4 ks(*k), vs(*v);
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(idx).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_kv8_append(k->data_ptr(), v->data_ptr(), ks.v, vs.v, c.t[0]->data_ptr(),
+                      c.t[1]->data_ptr(), c.t[2]->data_ptr<float>(), c.t[3]->data_ptr<float>(),
+                      static_cast<int>(c.pages), static_cast<int>(c.page),
+                      c.table->data_ptr<int>(), c.table->stride(0),
+                      static_cast<int>(c.table->size(1)), starts->data_ptr<int>(),
+                      counts ? counts->data_ptr<int>() : nullptr, static_cast<int>(B),
+                      static_cast<int>(H), static_cast<int>(T), static_cast<int>(D), dtype,
+                      g_status[idx], stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) Py_RETURN_NONE;
+    ++g_launches;
+    Py_RETURN_TRUE;
+  } catch (const std::exception&) {
+    Py_RETURN_NONE;
+  }
+}
+
+// sdpa_kv8(q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, lengths, counts, causal,
+//          scale, want_lse); scale -1.0: the default 1/sqrt(D)
+PyObject* sdpa_kv8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 11 || g_sdpa_kv8 == nullptr) Py_RETURN_NONE;
+  const at::Tensor* q = tensor_arg(args[0]);
+  const at::Tensor* lengths = tensor_arg(args[6]);
+  const at::Tensor* counts = args[7] != Py_None ? tensor_arg(args[7]) : nullptr;
+  if (!q || !lengths || (args[7] != Py_None && !counts)) Py_RETURN_NONE;
+  if (!PyBool_Check(args[8]) || !PyFloat_Check(args[9]) || !PyBool_Check(args[10])) Py_RETURN_NONE;
+  double scale = PyFloat_AS_DOUBLE(args[9]);
+  const bool want_lse = args[10] == Py_True;
+  try {
+    if (q->dim() != 4 || !q->is_cuda()) Py_RETURN_NONE;
+    const int dtype = dtype_code(*q);
+    const c10::Device dev = q->device();
+    const int64_t B = q->size(0), H = q->size(1), T = q->size(2), D = q->size(3);
+    if (dtype < 0 || !fits_int(B) || !fits_int(H) || !fits_int(T) || !fits_int(D) || !tma_ok(*q))
+      Py_RETURN_NONE;
+    CacheArgs c;
+    if (!cache_args(args + 1, args[5], B, dev, c) || c.dim != D || H % c.heads != 0) Py_RETURN_NONE;
+    if (!int_vector(lengths, B, dev) || (counts && !int_vector(counts, B, dev))) Py_RETURN_NONE;
+    const int idx = dev.index();
+    if (idx < 0 || idx >= kMaxDevices || g_status[idx] == nullptr) Py_RETURN_NONE;
+    if (scale == -1.0) scale = 1.0 / std::sqrt(static_cast<double>(D));
+    if (!(scale > 0.0) || !std::isfinite(scale)) Py_RETURN_NONE;
+    c10::cuda::CUDAGuard guard(dev);
+    const int b = static_cast<int>(B), h = static_cast<int>(H), t = static_cast<int>(T),
+              d = static_cast<int>(D), hk = static_cast<int>(c.heads);
+    const int64_t bytes = g_kv8_workspace(b, h, hk, t, d);
+    at::Tensor o = at::empty({B, H, T, D}, q->options());
+    at::Tensor lse;
+    if (want_lse) lse = at::empty({B, H, T}, q->options().dtype(at::kFloat));
+    at::Tensor work = at::empty({bytes}, q->options().dtype(at::kByte));
+    const Strides4 qs(*q), os(o);
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(idx).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_sdpa_kv8(q->data_ptr(), qs.v, o.data_ptr(), os.v,
+                    want_lse ? lse.data_ptr<float>() : nullptr, c.t[0]->data_ptr(),
+                    c.t[1]->data_ptr(), c.t[2]->data_ptr<float>(), c.t[3]->data_ptr<float>(),
+                    static_cast<int>(c.pages), static_cast<int>(c.page), c.table->data_ptr<int>(),
+                    c.table->stride(0), static_cast<int>(c.table->size(1)),
+                    lengths->data_ptr<int>(), counts ? counts->data_ptr<int>() : nullptr, b, h, hk,
+                    t, d, dtype, args[8] == Py_True, static_cast<float>(scale), work.data_ptr(),
+                    bytes, g_status[idx], stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) Py_RETURN_NONE;
+    ++g_launches;
+    if (!want_lse) return THPVariable_Wrap(std::move(o));
+    PyObject* out = PyTuple_New(2);
+    if (out == nullptr) return nullptr;
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(o)));
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(lse)));
+    return out;
+  } catch (const std::exception&) {
+    Py_RETURN_NONE;
+  }
+}
 
 // ---------------------------------------------------------------- torch operators
 
@@ -294,6 +544,14 @@ PyMethodDef kMethods[] = {
      "Bind ta_sdpa_fwd by its address in the loaded native library."},
     {"bind_ops", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(bind_ops)),
      METH_FASTCALL, "Bind the entry points the torch operators call."},
+    {"bind_serving", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(bind_serving)),
+     METH_FASTCALL, "Bind the rotary and 8-bit cache entry points."},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(rotary)),
+     METH_FASTCALL, "Checked single-call rotary launch; None when the full path must run."},
+    {"kv8_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(kv8_append)),
+     METH_FASTCALL, "Checked single-call cache append; None when the full path must run."},
+    {"sdpa_kv8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sdpa_kv8)),
+     METH_FASTCALL, "Checked single-call cache attention; None when the full path must run."},
     {"set_status", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(set_status)),
      METH_FASTCALL, "Register the device status word of a device."},
     {"launches", reinterpret_cast<PyCFunction>(launches), METH_NOARGS,

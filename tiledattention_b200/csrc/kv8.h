@@ -1,0 +1,145 @@
+// The paged 8-bit key/value cache: what the kernels that write it (kv8_append.cu) and read it
+// (sdpa_kv8*.cu) share. Host-callable parts are checked on the CPU (tests/native/kv8_check.cu).
+//
+// Pages [P, Hkv, page, D] of e4m3, D a multiple of 16 up to 256, page 16, 32, 64 or 128; one
+// float32 scale 2^e, e in [kScaleExpMin, kScaleExpMax], for each (page, head). Powers of two
+// cost an e4m3 value nothing (its own exponent does the rest) and make every product with a
+// scale exact. The range of e keeps 2^(difference of two exponents) inside float32.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace ta {
+namespace kv8 {
+
+constexpr int kScaleExpMin = -50;
+constexpr int kScaleExpMax = 50;
+
+// Least e with amax <= 448 * 2^e (448 = 1.75 * 2^8 is e4m3's largest value), held in range;
+// amax_bits: the bits of a finite float32 >= 0. Zero (a page of zeros) gives the least e.
+__host__ __device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
+  const int e = static_cast<int>(amax_bits >> 23) - 127;
+  const int up = (amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0;
+  const int need = e - 8 + up;
+  return need < kScaleExpMin ? kScaleExpMin : (need > kScaleExpMax ? kScaleExpMax : need);
+}
+
+// Exponent of a stored scale (a power of two), held in range whatever the bits are.
+__host__ __device__ __forceinline__ int stored_exponent(uint32_t scale_bits) {
+  const int e = static_cast<int>((scale_bits >> 23) & 0xffu) - 127;
+  return e < kScaleExpMin ? kScaleExpMin : (e > kScaleExpMax ? kScaleExpMax : e);
+}
+
+// A page id from the table, or -1 where the slot or the id is outside its range.
+__host__ __device__ __forceinline__ int checked_page(const int32_t* table_row, int64_t slot,
+                                                     int width, int num_pages) {
+  if (slot < 0 || slot >= width) return -1;
+  const int id = table_row[slot];
+  return id >= 0 && id < num_pages ? id : -1;
+}
+
+// Tokens start .. start + count of one sequence that fall into table slot `slot`: rows
+// [row0, row1) of its page are written from token t0 on; row0 rows before them are kept.
+struct SlotSpan {
+  int row0, row1;
+  int64_t t0;
+};
+__host__ __device__ __forceinline__ SlotSpan slot_span(int64_t start, int64_t count, int64_t slot,
+                                                       int page) {
+  const int64_t first = slot * page;
+  const int64_t lo = start > first ? start : first;
+  const int64_t hi = start + count < first + page ? start + count : first + page;
+  if (hi <= lo) return {0, 0, 0};
+  return {static_cast<int>(lo - first), static_cast<int>(hi - first), lo - start};
+}
+
+struct AppendParams {
+  const void* x[2];               // k, v: [B, Hkv, T, D], 16-bit
+  int64_t sb[2], sh[2], ss[2];    // element strides (dim stride 1)
+  uint8_t* pages[2];
+  float* scale[2];
+  const int32_t* table;           // [B, width] int32, row stride table_stride
+  int64_t table_stride;
+  const int32_t* starts;          // [B]
+  const int32_t* counts;          // [B] or null (all T)
+  unsigned int* status;
+  int B, Hkv, T, D, page, width, num_pages, bf16;
+};
+
+cudaError_t launch_append(const AppendParams& p, cudaStream_t stream);
+
+struct AttendParams {
+  const void* q;                  // [B, Hq, T, D], 16-bit
+  int64_t q_sb, q_sh, q_ss;
+  void* o;
+  int64_t o_sb, o_sh, o_ss;
+  float* lse;                     // optional [B, Hq, T] contiguous
+  const uint8_t* pages[2];
+  const float* scale[2];
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lengths;         // [B] tokens in the cache
+  const int32_t* counts;          // [B] or null (all T rows are real)
+  unsigned int* status;
+  float* part_o;                  // partial outputs, maxima and sums (see sdpa_kv8.cu)
+  float* part_ml;
+  int B, Hq, Hkv, T, D, page, page_shift, width, num_pages, bf16, causal;
+  int group;                      // Hq / Hkv
+  int row_blocks;                 // blocks of rows (token, head of the group) per kv head
+  float scale_log2;               // softmax scale * log2(e)
+};
+
+// Keys of a sequence that its row of token t may see: [0, limit).
+__host__ __device__ __forceinline__ int row_limit(int length, int count, int t, int causal) {
+  if (t >= count) return 0;
+  const int lim = causal ? length - count + t + 1 : length;
+  return lim > 0 ? lim : 0;
+}
+
+// Length and count of one sequence with every out-of-range value held in range.
+struct SeqExtent {
+  int length, count;
+  bool bad;
+};
+__host__ __device__ __forceinline__ SeqExtent checked_extent(int length, int count, int T,
+                                                             int64_t capacity) {
+  SeqExtent e{length, count, false};
+  if (e.length < 0) e.length = 0, e.bad = true;
+  if (e.length > capacity) e.length = static_cast<int>(capacity), e.bad = true;
+  if (e.count < 0) e.count = 0, e.bad = true;
+  if (e.count > T) e.count = T, e.bad = true;
+  return e;
+}
+
+// Work of the split kernel is a line of `total` tiles (sequence, then head and row block, then
+// keys), cut into `parts` equal runs: run i is [i * total / parts, (i + 1) * total / parts).
+__host__ __device__ __forceinline__ int64_t run_begin(int64_t i, int64_t total, int64_t parts) {
+  return i * total / parts;
+}
+// The run that holds tile w.
+__host__ __device__ __forceinline__ int64_t run_of(int64_t w, int64_t total, int64_t parts) {
+  return ((w + 1) * parts - 1) / total;
+}
+
+// Byte offset in shared memory of 16-byte chunk c of a row of codes, rows PITCH bytes apart:
+// 8 consecutive rows at one chunk, and 4 consecutive chunks of an even row and the row after
+// it, fall on different banks.
+template <int PITCH>
+__host__ __device__ __forceinline__ uint32_t chunk_at(int row, int c) {
+  if constexpr (PITCH == 64) return row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
+  const int f = ((row & 1) << 2) | (row & 2) | ((row >> 2) & 1);
+  return row * PITCH + ((c ^ f) << 4);
+}
+
+// Key, within its 16, of column n of score tile `half` (see sdpa_kv8.cu).
+__host__ __device__ __forceinline__ int key_of_column(int n, int half) {
+  return 4 * (n >> 1) + 2 * half + (n & 1);
+}
+
+// Workspace floats of the split kernel's partial results for a problem.
+size_t attend_workspace_bytes(int B, int Hq, int Hkv, int T, int D, int sm_count);
+cudaError_t launch_attend(const AttendParams& p, int sm_count, cudaStream_t stream);
+
+}  // namespace kv8
+}  // namespace ta

@@ -1,0 +1,202 @@
+// Writes keys and values into the paged 8-bit cache.
+//
+// For each (sequence, table slot, head) that new tokens fall into, and for K and V apart: the
+// largest finite magnitude of the page's new tokens gives the least power of two s with
+// amax <= 448 s; a page that already holds tokens keeps max(its s, the needed one), and where
+// that grows its old codes are rounded again (exact outside e4m3's subnormals). Codes are
+// x / s rounded to nearest even; what is beyond +-448 s saturates, NaN stays NaN.
+//
+// HBM-bound: 2 bytes read and 1 written a value. One block per (page, head, K or V): the page's
+// tokens are loaded once into registers (kHeld 16-byte vectors a thread: 64 x 128 values fit
+// 128 threads), reduced to their amax, scaled and stored; only what does not fit the
+// registers is read again, from L2.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "kv8.h"
+#include "tiledattention_b200.h"
+
+namespace ta {
+namespace kv8 {
+namespace {
+
+constexpr int kHeld = 8;  // vectors of 8 values a thread keeps
+
+// Largest |x| of 8 packed values as 16-bit integers (magnitudes of floats order as integers).
+__device__ __forceinline__ uint32_t max_magnitude(const uint4& v, uint32_t m) {
+  const uint32_t k = 0x7fff7fffu;
+  m = __vmaxu2(m, v.x & k);
+  m = __vmaxu2(m, v.y & k);
+  m = __vmaxu2(m, v.z & k);
+  return __vmaxu2(m, v.w & k);
+}
+
+// The same over the finite values only.
+template <bool BF16>
+__device__ __forceinline__ uint32_t max_finite(const uint4& v, uint32_t m) {
+  const uint32_t inf = BF16 ? 0x7f80u : 0x7c00u;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = w[i] & 0x7fffu, hi = (w[i] >> 16) & 0x7fffu;
+    if (lo < inf) m = max(m, lo);
+    if (hi < inf) m = max(m, hi);
+  }
+  return m;
+}
+
+// Bits of the float32 value of a non-negative 16-bit float.
+template <bool BF16>
+__device__ __forceinline__ uint32_t f32_bits(uint32_t h) {
+  if constexpr (BF16) return h << 16;
+  float f;
+  asm("cvt.f32.f16 %0, %1;" : "=f"(f) : "h"(static_cast<uint16_t>(h)));
+  return __float_as_uint(f);
+}
+
+// Two values of a packed word, times `mul` (a power of two), as two e4m3 codes.
+template <bool BF16>
+__device__ __forceinline__ uint32_t codes2(uint32_t w, float mul) {
+  float lo, hi;
+  if constexpr (BF16) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+  } else {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
+        : "=f"(lo), "=f"(hi) : "r"(w));
+  }
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi * mul), "f"(lo * mul));
+  return r;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint2 codes8(const uint4& v, float mul) {
+  return make_uint2(codes2<BF16>(v.x, mul) | (codes2<BF16>(v.y, mul) << 16),
+                    codes2<BF16>(v.z, mul) | (codes2<BF16>(v.w, mul) << 16));
+}
+
+// Four e4m3 codes times mul (a power of two <= 1), rounded again.
+__device__ __forceinline__ uint32_t recode4(uint32_t w, float mul) {
+  uint32_t out = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(w >> (16 * i))));
+    out |= codes2<false>(h, mul) << (16 * i);
+  }
+  return out;
+}
+
+__device__ __forceinline__ float pow2f(int e) {
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(128) append_kernel(const AppendParams p, int slots) {
+  const int b = blockIdx.x / slots;
+  const int h = blockIdx.y;
+  const int kind = blockIdx.z;
+  const int64_t start = p.starts[b];
+  int64_t count = p.counts ? p.counts[b] : p.T;
+  const int64_t capacity = static_cast<int64_t>(p.width) * p.page;
+  const bool first_block = blockIdx.x % slots == 0 && h == 0 && kind == 0 && threadIdx.x == 0;
+  if (start < 0 || count < 0 || count > p.T || start + count > capacity) {
+    if (first_block && p.status) atomicOr(p.status, TA_DEVSTAT_BAD_LENGTH);
+    if (start < 0 || count < 0) return;
+    count = min(min(count, static_cast<int64_t>(p.T)), capacity - start);
+  }
+  const int64_t slot = start / p.page + blockIdx.x % slots;
+  const SlotSpan span = slot_span(start, count, slot, p.page);
+  if (span.row1 <= span.row0) return;
+  const int page = checked_page(p.table + b * p.table_stride, slot, p.width, p.num_pages);
+  if (page < 0) {
+    if (h == 0 && kind == 0 && threadIdx.x == 0 && p.status)
+      atomicOr(p.status, TA_DEVSTAT_BAD_PAGE);
+    return;
+  }
+
+  const int vecs = p.D / 8;  // vectors per token
+  const int n = (span.row1 - span.row0) * vecs;
+  const uint16_t* x = static_cast<const uint16_t*>(p.x[kind]) + b * p.sb[kind] + h * p.sh[kind] +
+                      span.t0 * p.ss[kind];
+  const int64_t ss = p.ss[kind];
+  uint8_t* out = p.pages[kind] +
+                 ((static_cast<int64_t>(page) * p.Hkv + h) * p.page) * static_cast<int64_t>(p.D);
+  auto load = [&](int i) {
+    const int row = i / vecs;
+    return *reinterpret_cast<const uint4*>(x + row * ss + (i - row * vecs) * 8);
+  };
+
+  uint4 held[kHeld];
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    const int i = threadIdx.x + k * 128;
+    held[k] = i < n ? load(i) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) m = max_magnitude(held[k], m);
+  for (int i = threadIdx.x + kHeld * 128; i < n; i += 128) m = max_magnitude(load(i), m);
+  constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
+  m = max(m & 0xffffu, m >> 16);
+  __shared__ uint32_t s_max[4];
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (threadIdx.x % 32 == 0) s_max[threadIdx.x / 32] = m;
+  __syncthreads();
+  m = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+  if (m >= kInf) {  // an infinity or NaN among them: once more, over the finite values
+    m = 0;
+    for (int i = threadIdx.x; i < n; i += 128) m = max_finite<BF16>(load(i), m);
+    m = __reduce_max_sync(0xffffffffu, m);
+    __syncthreads();
+    if (threadIdx.x % 32 == 0) s_max[threadIdx.x / 32] = m;
+    __syncthreads();
+    m = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+  }
+
+  int e = scale_exponent(f32_bits<BF16>(m));
+  float* scale = p.scale[kind] + static_cast<int64_t>(page) * p.Hkv + h;
+  if (span.row0 > 0) {
+    const int before = stored_exponent(__float_as_uint(*scale));
+    __syncthreads();  // every thread has read the old scale before thread 0 replaces it
+    if (e > before) {
+      const float mul = pow2f(before - e);
+      uint4* old = reinterpret_cast<uint4*>(out);
+      for (int i = threadIdx.x; i < span.row0 * p.D / 16; i += 128) {
+        uint4 w = old[i];
+        w.x = recode4(w.x, mul);
+        w.y = recode4(w.y, mul);
+        w.z = recode4(w.z, mul);
+        w.w = recode4(w.w, mul);
+        old[i] = w;
+      }
+    } else {
+      e = before;
+    }
+  }
+  if (threadIdx.x == 0) *scale = pow2f(e);
+  const float mul = pow2f(-e);
+  uint2* dst = reinterpret_cast<uint2*>(out + span.row0 * p.D);  // rows are contiguous
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    const int i = threadIdx.x + k * 128;
+    if (i < n) dst[i] = codes8<BF16>(held[k], mul);
+  }
+  for (int i = threadIdx.x + kHeld * 128; i < n; i += 128) dst[i] = codes8<BF16>(load(i), mul);
+}
+
+}  // namespace
+
+cudaError_t launch_append(const AppendParams& p, cudaStream_t stream) {
+  const int slots = (p.T + p.page - 2) / p.page + 1;  // pages that T tokens touch at most
+  const int64_t blocks = static_cast<int64_t>(p.B) * slots;
+  if (blocks > 0x7fffffffll || p.Hkv > 65535) return cudaErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(blocks), p.Hkv, 2);
+  if (p.bf16) append_kernel<true><<<grid, 128, 0, stream>>>(p, slots);
+  else append_kernel<false><<<grid, 128, 0, stream>>>(p, slots);
+  return cudaGetLastError();
+}
+
+}  // namespace kv8
+}  // namespace ta

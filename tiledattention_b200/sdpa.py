@@ -30,6 +30,12 @@ def _prepare(q, k, v, causal, scale):
     return float(scale) if scale is not None else 1.0 / math.sqrt(head_dim)
 
 
+def _async_mode() -> bool:
+    """Whether TILEDATTN_SYNC_MODE is the default, asynchronous mode."""
+    mode = os.environ.get("TILEDATTN_SYNC_MODE")
+    return mode is None or mode.strip().lower() == "async"
+
+
 def _fast_launch(q, k, v, causal, scale, want_lse):
     """The one-call native launcher for the common case, or None (the full path then runs
     and raises the reference's error, copies or pads as needed). Taken only once the runtime
@@ -37,8 +43,7 @@ def _fast_launch(q, k, v, causal, scale, want_lse):
     fast = _native._fast
     if fast is None or not _runtime._runtime_ready:
         return None
-    mode = os.environ.get("TILEDATTN_SYNC_MODE")
-    if mode is not None and mode.strip().lower() != "async":
+    if not _async_mode():
         return None
     if scale is None:
         scale = -1.0  # the launcher's code for 1/sqrt(D)
