@@ -60,7 +60,7 @@ extern "C" {
 #define TA_DEVSTAT_TIMEOUT_EPILOG  8u
 #define TA_DEVSTAT_TIMEOUT_DRAIN   16u
 #define TA_DEVSTAT_PEER_TIMEOUT    32u  /* ta_peer_barrier: a peer did not arrive in time */
-#define TA_DEVSTAT_BAD_PAGE        64u  /* cache operators: a page id outside the cache; its tokens were not written, or read as zeros */
+#define TA_DEVSTAT_BAD_PAGE        64u  /* cache operators: a page id outside the cache; its tokens were not written, or left out */
 #define TA_DEVSTAT_BAD_LENGTH      128u /* cache operators: a start, count or length outside its range; it was held in range */
 
 /* Largest group ta_peer_barrier / ta_lse_merge_peers serve (one NVLink domain of 8 GPUs). */
@@ -213,8 +213,8 @@ int ta_rotary(const void* q, void* q_out, const int64_t* q_strides, const int64_
  * or 128 and D a multiple of 16 up to 256; k_scale and v_scale are device float32
  * [num_pages, Hkv], powers of two 2^e, -50 <= e <= 50: a value is code * scale. Token i of
  * sequence b is row i % page of page table[b * table_stride + i / page] (device int32, width
- * table_width). Page ids outside [0, num_pages) set TA_DEVSTAT_BAD_PAGE and are neither read
- * nor written; starts, counts and lengths outside their range set TA_DEVSTAT_BAD_LENGTH and
+ * table_width). Page ids outside [0, num_pages) set TA_DEVSTAT_BAD_PAGE and are neither written
+ * nor attended to; starts, counts and lengths outside their range set TA_DEVSTAT_BAD_LENGTH and
  * are held in range.
  *
  * ta_kv8_append — writes tokens starts[b] .. starts[b] + counts[b] - 1 of every sequence from

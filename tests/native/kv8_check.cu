@@ -27,28 +27,26 @@ static uint32_t bits(float f) {
   return u;
 }
 
-template <int PITCH>
+template <int COLS, int PLANE>
 static bool offsets_fit(int rows, int chunks) {
   std::set<uint32_t> seen;
   for (int r = 0; r < rows; ++r)
     for (int c = 0; c < chunks; ++c) {
-      const uint32_t at = chunk_at<PITCH>(r, c);
-      if (at % 16 || at + 16 > static_cast<uint32_t>(rows * PITCH) || !seen.insert(at).second)
+      const uint32_t at = chunk_at<COLS, PLANE>(r, c);
+      if (at % 16 || at + 16 > static_cast<uint32_t>(rows * chunks * 16) || !seen.insert(at).second)
         return false;
       ++checks;
     }
-  for (int c = 0; c < chunks; ++c)  // 8 rows of one ldmatrix phase
-    for (int r0 = 0; r0 < rows; r0 += 8) {
-      std::set<uint32_t> banks;
-      for (int r = r0; r < r0 + 8; ++r) banks.insert(chunk_at<PITCH>(r, c) % 128);
-      if (banks.size() != 8) return false;
-    }
-  for (int c0 = 0; c0 < chunks; c0 += 4)  // two rows of a quarter warp's 16-byte loads
-    for (int r = 0; r + 1 < rows; r += 2) {
-      std::set<uint32_t> banks;
-      for (int k = 0; k < 8; ++k) banks.insert(chunk_at<PITCH>(r + k / 4, c0 + k % 4) % 128);
-      if (banks.size() != 8) return false;
-    }
+  for (int c = 0; c < chunks; ++c)  // 8 rows of one ldmatrix phase, in and out of order
+    for (int r0 = 0; r0 < rows; r0 += 16)
+      for (int half = 0; half < 2; ++half) {
+        std::set<uint32_t> banks, keys;
+        for (int r = 0; r < 8; ++r) {
+          banks.insert(chunk_at<COLS, PLANE>(r0 + key_at(8 * half + r), c) % 128);
+          keys.insert(chunk_at<COLS, PLANE>(r0 + key_of_column(r, half), c) % 128);
+        }
+        if (banks.size() != 8 || keys.size() != 8) return false;
+      }
   return true;
 }
 
@@ -121,19 +119,21 @@ int main() {
         CHECK(run_begin(r, total, parts) < run_begin(r + 1, total, parts));
     }
 
-  CHECK((offsets_fit<64>(32, 4)));
-  CHECK((offsets_fit<128>(32, 8)));
-  CHECK((offsets_fit<256>(16, 16)));
+  CHECK((offsets_fit<64, 0>(32, 4)));
+  CHECK((offsets_fit<64, 0>(16, 4)));
+  CHECK((offsets_fit<128, 0>(32, 8)));
+  CHECK((offsets_fit<128, 0>(16, 8)));
+  CHECK((offsets_fit<128, 16 * 128>(16, 16)));
 
-  // score columns: each key of 16 once, pairs of columns are neighbouring keys
+  // score columns: each key of 16 once, columns 2t, 2t+1 of the halves at positions 4t .. 4t+3
   std::set<int> keys;
   for (int half = 0; half < 2; ++half)
     for (int n = 0; n < 8; ++n) keys.insert(key_of_column(n, half));
   CHECK(keys.size() == 16 && *keys.begin() == 0 && *keys.rbegin() == 15);
   for (int t = 0; t < 4; ++t)
     for (int half = 0; half < 2; ++half) {
-      CHECK(key_of_column(2 * t, half) == 4 * t + 2 * half);
-      CHECK(key_of_column(2 * t + 1, half) == 4 * t + 2 * half + 1);
+      CHECK(key_of_column(2 * t, half) == key_at(4 * t + 2 * half));
+      CHECK(key_of_column(2 * t + 1, half) == key_of_column(2 * t, half) + 1);
     }
   std::printf("ok %d\n", checks);
   return 0;

@@ -128,11 +128,11 @@ def attend64(q, k_pages, v_pages, k_scale, v_scale, table, lengths, counts=None,
         # of the sum's size), then the scale, the shift and exp2, in magnitudes up to |s| log2 e.
         ds = dim * 2.0 ** -23 * torch.where(seen, size, torch.zeros_like(size)).amax(-1, keepdim=True)
         ds = ds + (torch.nan_to_num(top.abs(), posinf=0.0) * 1.45 + 110) * 2.0 ** -22
-        # Weights: 2^-12 of rounding each (fp16), or 2^-25 absolutely against a largest weight of
-        # one or more on codes up to 448, of which the largest value v shows at least half; and
-        # fp32 sums over n keys.
+        # Weights: 2^-12 of rounding each (fp16), or 2^-25 absolutely at its lower end against a
+        # largest weight of 2^7 or more, on codes up to 448, of which the largest value v shows at
+        # least half: per key 448 * 2^-25 / 2^7 <= 2 v * 2^-32. And fp32 sums over n keys.
         e = (2.0 ** -12 + 2 * ds + n * 2.0 ** -23)
-        t = e * absr + n * 2.0 ** -24 * torch.nan_to_num(v).abs().amax((1, 2))[:, None, None, None]
+        t = e * absr + n * 2.0 ** -31 * torch.nan_to_num(v).abs().amax((1, 2))[:, None, None, None]
         t = t + half_step(q.dtype) * (r.abs() + t) + torch.finfo(q.dtype).tiny * half_step(q.dtype) * 2
         tol[b, :, :c] = t.reshape(heads, c, dim)
         lse_tol[b, :, :c] = (ds + n * 2.0 ** -23).squeeze(-1).reshape(heads, c)

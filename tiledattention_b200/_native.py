@@ -38,7 +38,7 @@ DEVSTAT_BITS = {
     8: "epilogue wait timed out",
     16: "drain of in-flight copies/MMAs timed out",
     32: "peer barrier timed out (a peer GPU did not arrive)",
-    64: "a page id outside the cache (its tokens were not written, or read as zeros)",
+    64: "a page id outside the cache (its tokens were not written, or left out)",
     128: "a start, count or length outside its range (it was held in range)",
 }
 

@@ -97,7 +97,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return OUT
     os.makedirs(OUT_DIR, exist_ok=True)
     cmd = [
-        nvcc_path(), "-O3", "-std=c++17", *ARCH, "-lineinfo",
+        nvcc_path(), "-O3", "-std=c++17", "--threads=0", *ARCH, "-lineinfo",
         "-Xcompiler", "-fPIC", "-shared",
         "-I", os.path.join(REPO_DIR, "include"),
         "-o", OUT + ".tmp",

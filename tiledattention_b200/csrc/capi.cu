@@ -118,6 +118,8 @@ void ta_capi_clear_error() { g_last_error.clear(); }
 
 int ta_capi_check_device() { return check_device(); }
 
+void* ta_capi_tensor_map_encoder() { return reinterpret_cast<void*>(encode_fn()); }
+
 extern "C" {
 
 #ifdef TA_TRACE

@@ -20,6 +20,9 @@ void ta_capi_clear_error();
 // TA_OK where the current device is one this build runs on.
 int ta_capi_check_device();
 
+// The driver's cuTensorMapEncodeTiled (a PFN_cuTensorMapEncodeTiled_v12000), or null.
+void* ta_capi_tensor_map_encoder();
+
 // NVTX range named after the entry point, open for the scope (host-side launch work, seen on
 // the CPU row of nsys and by ncu --nvtx filters). Without a tool attached it costs a check.
 struct TaNvtxRange {

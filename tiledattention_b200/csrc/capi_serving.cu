@@ -1,9 +1,12 @@
 // C ABI of the operators around a decoder's attention: rotary positions, the write into the
 // paged 8-bit cache and attention over it. Argument checks and launches; see
 // include/tiledattention_b200.h for the contracts.
+#include <cuda.h>
 #include <cuda_runtime.h>
+#include <cudaTypedefs.h>
 
 #include <cmath>
+#include <cstdio>
 
 #include "capi_internal.h"
 #include "kv8.h"
@@ -62,10 +65,30 @@ int check_cache(const void* k_pages, const void* v_pages, const float* k_scale,
     return ta_capi_fail(TA_ERR_INVALID_ARGUMENT, "table_width * page must be below 2^31");
   if (table_stride < table_width && B > 1)
     return ta_capi_fail(TA_ERR_LAYOUT, "page table rows overlap");
+  if (static_cast<int64_t>(num_pages) * Hkv > 0x7fffffffll)
+    return ta_capi_fail(TA_ERR_INVALID_ARGUMENT, "num_pages * Hkv must be below 2^31");
   if (Hkv > 65535) return ta_capi_fail(TA_ERR_INVALID_ARGUMENT, "too many heads");
   if (!aligned(k_pages, 16) || !aligned(v_pages, 16))
     return ta_capi_fail(TA_ERR_LAYOUT, "cache pages must be 16-byte aligned");
   return TA_OK;
+}
+
+// Map of the cache's pages as (D, page, P * Hkv) bytes with boxes of `rows` tokens; columns from
+// D on read as zeros.
+int make_pages_map(CUtensorMap* map, const void* pages, int D, int page, int64_t planes, int rows) {
+  const auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ta_capi_tensor_map_encoder());
+  if (!enc) return ta_capi_fail(TA_ERR_DRIVER, "cuTensorMapEncodeTiled entry point unavailable");
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(page),
+                              static_cast<cuuint64_t>(planes)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(D) * page};
+  const cuuint32_t box[3] = {D <= 64 ? 64u : 128u, static_cast<cuuint32_t>(rows), 1};
+  const cuuint32_t step[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(pages), dims,
+                         strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         D <= 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TA_OK
+                           : ta_capi_fail(TA_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the cache");
 }
 
 }  // namespace
@@ -241,7 +264,13 @@ int ta_sdpa_kv8(const void* q, const int64_t* q_strides, void* o, const int64_t*
   p.causal = causal != 0;
   p.group = Hq / Hkv;
   p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
-  return launched(ta::kv8::launch_attend(p, sms, static_cast<cudaStream_t>(stream)),
+  CUtensorMap map_k, map_v;
+  const int box = page < ta::kv8::kKeysPerStep ? page : ta::kv8::kKeysPerStep;
+  const int64_t planes = static_cast<int64_t>(num_pages) * Hkv;
+  if ((rc = make_pages_map(&map_k, k_pages, D, page, planes, box)) ||
+      (rc = make_pages_map(&map_v, v_pages, D, page, planes, box)))
+    return rc;
+  return launched(ta::kv8::launch_attend(p, map_k, map_v, sms, static_cast<cudaStream_t>(stream)),
                   "cache attention launch failed");
 }
 

@@ -7,6 +7,7 @@
 // scale exact. The range of e keeps 2^(difference of two exponents) inside float32.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -122,24 +123,36 @@ __host__ __device__ __forceinline__ int64_t run_of(int64_t w, int64_t total, int
   return ((w + 1) * parts - 1) / total;
 }
 
-// Byte offset in shared memory of 16-byte chunk c of a row of codes, rows PITCH bytes apart:
-// 8 consecutive rows at one chunk, and 4 consecutive chunks of an even row and the row after
-// it, fall on different banks.
-template <int PITCH>
+// Byte offset in shared memory of 16-byte chunk c of a row of codes, as TMA's 64- and 128-byte
+// swizzles lay out boxes of COLS bytes a row: 8 consecutive rows at one chunk fall on
+// different banks. Chunks beyond COLS bytes are in the next plane, PLANE bytes on.
+template <int COLS, int PLANE>
 __host__ __device__ __forceinline__ uint32_t chunk_at(int row, int c) {
-  if constexpr (PITCH == 64) return row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
-  const int f = ((row & 1) << 2) | (row & 2) | ((row >> 2) & 1);
-  return row * PITCH + ((c ^ f) << 4);
+  if constexpr (COLS == 64) return row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
+  return (c >> 3) * PLANE + row * 128 + (((c & 7) ^ (row & 7)) << 4);
 }
 
-// Key, within its 16, of column n of score tile `half` (see sdpa_kv8.cu).
+// Order of 16 keys in the matrix instructions (see sdpa_kv8.cu): the key at position p of the
+// second product's depth, and the key of column n of score tile `half`, which is position
+// 4 (n / 2) + 2 half + n % 2. Chosen so that the 8 rows of every ldmatrix phase, of K (the columns of
+// one half) and of V (positions 0-7 and 8-15), differ modulo 8: no bank conflicts.
+__host__ __device__ __forceinline__ int key_at(int p) {
+  return 8 * (p >> 3) + 4 * (((p >> 1) & 1) ^ (p >> 3)) + 2 * ((p >> 2) & 1) + (p & 1);
+}
 __host__ __device__ __forceinline__ int key_of_column(int n, int half) {
-  return 4 * (n >> 1) + 2 * half + (n & 1);
+  return key_at(4 * (n >> 1) + 2 * half + (n & 1));
 }
 
-// Workspace floats of the split kernel's partial results for a problem.
+// Keys a warp of the split kernel takes a step, which is also the rows of a copied box where the
+// page has as many.
+constexpr int kKeysPerStep = 32;
+
+// Workspace of the split kernel's partial results for a problem.
 size_t attend_workspace_bytes(int B, int Hq, int Hkv, int T, int D, int sm_count);
-cudaError_t launch_attend(const AttendParams& p, int sm_count, cudaStream_t stream);
+// map_k, map_v: 3-D maps (D, page, P * Hkv) of the pages' bytes, boxes of 64 (D <= 64, 64-byte
+// swizzle) or 128 columns (128-byte swizzle) x min(page, kKeysPerStep) rows.
+cudaError_t launch_attend(const AttendParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v,
+                          int sm_count, cudaStream_t stream);
 
 }  // namespace kv8
 }  // namespace ta

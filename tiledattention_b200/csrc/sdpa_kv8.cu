@@ -8,24 +8,32 @@
 // then measure each key's share of the output in units of its e4m3 codes, so one fp16 weight
 // (11 bits, <= 2^8) is right for pages of any scale. The denominator is summed in fp32.
 //
-// HBM-bound: 2 D bytes a key against 4 D G operations for the G heads that share it. Codes go to
-// fp16 in registers (exact; 160 codes/ns/SM measured against the 44 bytes/ns/SM that HBM
-// delivers) and feed mma.sync m16n8k16: 16 rows at a time is what decoding has, and a
-// tcgen05 tile of 128 rows would be empty for the most part.
+// HBM-bound: 2 D bytes a key against 4 D G operations for the G heads that share it. The codes go
+// to fp16 in registers (exact) and feed mma.sync m16n8k16 with the KEYS on the 16-side and the
+// rows on the 8-side: scores^T = K q^T and o^T += V^T p^T, so 8 heads of a group fill the
+// instruction, where rows on the 16-side would leave half of it and of the output registers
+// empty. A tcgen05 tile of 128 rows would be empty for the most part; mma.sync on e4m3 itself
+// is no faster (it was measured to run as two fp16 ones with the conversions inside).
 //
-// One warp = its own keys: it copies kKeys keys a stage with cp.async into its own shared
-// memory, keeps its own running maximum, sums and output, and waits for nobody; the four warps
-// of a block merge when a (sequence, head) ends. Work is a line of tiles over all sequences
-// and heads, cut into equal runs, one a block, so batches of uneven lengths fill the GPU
-// evenly; a (sequence, head) that lies in one run is written at once, one that is cut leaves
-// partial results for the merge kernel, which starts before this one ends (programmatic
-// launch).
+// One warp = its own keys: it copies 32 keys' K and V in turn by TMA into its own ring in shared
+// memory, keeps its own reference, sums and output, and waits for nobody; the four warps of a
+// block merge when a (sequence, head) ends. Work is a line of tiles over all sequences and
+// heads, cut into equal runs, one a block, so batches of uneven lengths fill the GPU evenly; a
+// (sequence, head) that lies in one run is written at once, one that is cut leaves partial
+// results for the merge kernel, which starts before this one ends (programmatic launch).
 //
-// Operands without shuffles: K codes are read with 16-byte loads, thread (g, t) of a warp
-// taking dims 64 j + 16 t ..+15 of key g, and Q's fragments use the same order of dims. V codes
-// come through ldmatrix m16n16.trans.b8, which gives a thread 4 consecutive keys of one dim;
-// the keys of score columns are permuted to match (key 16 i + 4 (n / 2) + 2 half + n % 2 for
-// column n), so a score fragment is the weight fragment as it stands.
+// Operands: K codes come through ldmatrix, thread (g, t) of a warp taking dims 16 c + 4 t ..+3 of
+// key g for chunk c, and q's fragments use the same order of dims. V codes come through ldmatrix
+// m16n16.trans.b8, which gives a thread 4 consecutive positions of one dim; the keys of score
+// rows are permuted to match (key_at in kv8.h), and movmatrix turns the weights from score rows to
+// the second product's columns. With the TMA swizzle neither ldmatrix meets a bank twice.
+//
+// What bounds the loop next to HBM is instruction issue (2 conversions for 4 codes, 1 MMA for
+// 256 codes and 8 rows), so everything a step does not need is kept out of it: masks are applied only
+// where a step reaches a row's limit, the scales ride in the multiply-add before exp2, and the
+// reference of a row's weights moves (and is agreed on between lanes) only when a score passes it
+// by 2^15.
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -41,34 +49,43 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr float kGrowth = 8.f;  // log2: the running maximum follows when it grew by more
+constexpr int kKeys = kKeysPerStep;  // of a warp: the depth of the second product's MMA
+constexpr int kBlocks = kKeys / 16;
+// Weights are 2^(t - ref) with ref set to 7 below the row's largest t and moved when t passes
+// it by 15: the largest weight then is between 2^7 and 2^15, inside fp16, and what fp16 rounds
+// away at its lower end (2^-25) is at most 2^-32 of it.
+constexpr float kBelow = 7.f, kGrowth = 15.f;
 
-// NJ: head dim in blocks of 64 (row pitch in shared memory: a power of two). MT: 16-row tiles.
-template <int NJ, int MT>
+// NJ: head dim in blocks of 64. NT: tiles of 8 rows.
+template <int NJ, int NT>
 struct Cfg {
   static constexpr int kDim = NJ * 64;
-  static constexpr int kPitch = NJ <= 2 ? NJ * 64 : 256;
-  static constexpr int kKeys = (NJ <= 2 && MT == 1) ? 32 : 16;  // per warp and stage
-  static constexpr int kBlocks = kKeys / 16;
-  static constexpr int kTile = kWarps * kKeys;  // keys per block and step
-  static constexpr int kRows = 16 * MT;
-  static constexpr int kSlot = 2 * kKeys * kPitch;  // K and V bytes of a warp's stage
-  // ~96 KB of stages a block, two blocks a SM
-  static constexpr int kStages = (96 * 1024) / (kWarps * kSlot) < 6 ? (96 * 1024) / (kWarps * kSlot) : 6;
-  // merge: a slot holds kRows x kMergeCols floats
-  static constexpr int kMergeCols = kSlot / (kRows * 4) < kDim ? kSlot / (kRows * 4) : kDim;
+  static constexpr int kPlanes = NJ <= 2 ? 1 : 2;  // columns of a unit: planes of kCols bytes
+  static constexpr int kCols = NJ == 1 ? 64 : 128;
+  static constexpr int kTile = kWarps * kKeys;     // keys per block and step
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kPlane = kKeys * kCols;
+  static constexpr int kUnit = kPlanes * kPlane;   // K or V bytes of a warp's step
+  // Blocks a SM, as the registers allow (the output takes 16 NJ NT of them, q 8 NJ NT where it
+  // is not shared), and the ring's units, as shared memory then allows.
+  static constexpr bool kQShared = NJ * NT > 6;
+  static constexpr int kBlocksPerSm = NJ <= 2 ? (NJ * NT <= 2 ? 4 : NJ * NT <= 4 ? 3 : 2) : 2;
+  static constexpr int kUnits = NJ == 1 ? 6 : NJ == 2 ? (kBlocksPerSm == 4 ? 3 : kBlocksPerSm == 3 ? 4 : 5) : 3;
+  static constexpr int kScaleSteps = 4;  // steps whose scales are kept: more than units ahead / 2
+  // merge: a unit holds kRows x kMergeCols floats
+  static constexpr int kMergeCols = kUnit / (kRows * 4) < kDim ? kUnit / (kRows * 4) : kDim;
   static constexpr int kPasses = (kDim + kMergeCols - 1) / kMergeCols;
-  static constexpr int kScaleOff = kWarps * kStages * kSlot;
-  static constexpr int kScaleBytes = kWarps * kStages * 2 * kBlocks * 4;
+  static constexpr int kQOff = kWarps * kUnits * kUnit;
+  static constexpr int kQBytes = kQShared ? NT * NJ * 2 * 512 : 0;
+  static constexpr int kScaleOff = kQOff + kQBytes;
+  static constexpr int kScaleBytes = kWarps * kScaleSteps * 2 * kBlocks * 4;
   static constexpr int kMlOff = kScaleOff + kScaleBytes;
-  static constexpr int kScanOff = kMlOff + 2 * kWarps * kRows * 4;
-  static constexpr int kBytes = kScanOff + 64;
+  static constexpr int kBarOff = kMlOff + 2 * kWarps * kRows * 4;
+  static constexpr int kScanOff = kBarOff + kWarps * kUnits * 8;
+  static constexpr int kBytes = kScanOff + 64 + 1024;  // slack: units are 1024-byte aligned
 };
+constexpr uint64_t kTimeoutNs = 1000000000ull;  // 1 s per wait for a copy
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-               : "memory");
-}
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -76,6 +93,14 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)),
+      "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
@@ -112,6 +137,11 @@ __device__ __forceinline__ uint4 without_nan(uint4 v) {
   v.w &= ~((nan_bits(v.w) >> 7) * 0xffu);
   return v;
 }
+// Four matrices of 8 rows x 16 codes: r[m] the codes 4t .. 4t+3 of row g of matrix m.
+__device__ __forceinline__ void ldsm_codes(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
 // 16 keys x 32 dims of codes: r[0], r[1] dims g, g + 8 of the first 16, r[2], r[3] of the second,
 // each 4 codes of keys 4t .. 4t+3.
 __device__ __forceinline__ void ldsm_codes_t(uint32_t a, uint32_t (&r)[4]) {
@@ -124,12 +154,18 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
       "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
       : "=r"(lo), "=r"(hi) : "r"(w));
 }
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                         uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transposes an 8 x 8 matrix of 16-bit values held two a thread.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
@@ -198,28 +234,34 @@ __device__ __forceinline__ Scan scan_batch(const AttendParams& p, int tile, int6
 
 // A place on the line of tiles.
 struct Cursor {
-  int b, hr, tile, tiles, length;
+  int b, h, rb, tile, tiles, length;
 };
 
-template <int NJ, int MT>
-__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams p, int d_chunks) {
-  using C = Cfg<NJ, MT>;
-  extern __shared__ __align__(128) uint8_t smem[];
+template <int NJ, int NT>
+__global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
+    attend_kernel(const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const AttendParams p) {
+  using C = Cfg<NJ, NT>;
+  constexpr int kU = C::kUnits;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   float* s_m = reinterpret_cast<float*>(smem + C::kMlOff);
   float* s_l = s_m + kWarps * C::kRows;
   int64_t* s_scan = reinterpret_cast<int64_t*>(smem + C::kScanOff);
   int* s_start = reinterpret_cast<int*>(s_scan + kWarps);
+  volatile int* abort_flag = s_start + 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int hrs = p.Hkv * p.row_blocks;
-
-  // Columns beyond the head dim are never copied: they stay zero.
-  const bool padded = d_chunks != NJ * 4;
-  if (padded)
-    for (int i = threadIdx.x; i < C::kScaleOff / 16; i += kThreads)
-      reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff) + warp * kU;
+  if (lane == 0) {
+    for (int i = 0; i < kU; ++i) mbar_init(full + i, 1);
+    fence_mbar_init();
+    if (warp == 0) *abort_flag = 0;
+  }
 
   // This block's run of the line, and the sequence it begins in.
+  const int hrs = p.Hkv * p.row_blocks;
   int b0, b1;
   const Scan sc = scan_batch(p, C::kTile, hrs, s_scan, blockIdx.x == 0, b0, b1);
   const int64_t total = sc.total;
@@ -227,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x >= parts) return;
   const int64_t w0 = run_begin(blockIdx.x, total, parts);
-  const int64_t w1 = run_begin(blockIdx.x + 1, total, parts);
+  const int steps = static_cast<int>(run_begin(blockIdx.x + 1, total, parts) - w0);
   {
     int64_t at = sc.mine;
     for (int b = b0; b < b1; ++b) {
@@ -247,19 +289,20 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
     const SeqExtent e = extent_of(p, cur.b);
     cur.length = e.length;
     cur.tiles = tiles_of(e, C::kTile);
-    cur.hr = s_start[1] / cur.tiles;
-    cur.tile = s_start[1] - cur.hr * cur.tiles;
+    const int hr = s_start[1] / cur.tiles;
+    cur.tile = s_start[1] - hr * cur.tiles;
+    cur.h = hr / p.row_blocks;
+    cur.rb = hr - cur.h * p.row_blocks;
   }
-  Cursor ahead = cur;  // the place of the next copy
-
-  const uint32_t slots = smem_u32(smem) + warp * (C::kStages * C::kSlot);
-  const uint32_t scales = smem_u32(smem) + C::kScaleOff + warp * (C::kStages * 2 * C::kBlocks * 4);
+  Cursor ahead = cur;  // the step whose K is copied next
 
   auto advance = [&](Cursor& c) {
     if (++c.tile < c.tiles) return;
     c.tile = 0;
-    if (++c.hr < hrs) return;
-    c.hr = 0;
+    if (++c.rb < p.row_blocks) return;
+    c.rb = 0;
+    if (++c.h < p.Hkv) return;
+    c.h = 0;
     do {
       if (++c.b >= p.B) return;
       const SeqExtent e = extent_of(p, c.b);
@@ -268,321 +311,372 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
     } while (c.tiles == 0);
   };
 
-  // Page ids of this warp's 16-key blocks at `ahead`, fetched one step before their use.
-  int page_id[C::kBlocks];
+  // The ring: unit 2 n is K of this warp's keys of step n, unit 2 n + 1 their V. A page id is
+  // fetched a step before its first use. Nothing is copied from the sequence's end on (whole
+  // boxes: the rest of its last page comes along), nor from pages outside the cache, whose
+  // blocks are marked in `left_out`, 4 steps' marks in turn.
+  const uint32_t ring = smem_u32(smem) + warp * (kU * C::kUnit);
+  const uint32_t scales = smem_u32(smem) + C::kScaleOff + warp * (C::kScaleSteps * 2 * kBlocks * 4);
+  const int box = min(p.page, kKeys);
+  uint32_t left_out = 0;
+  int page_next[kBlocks];                      // of `ahead`
+  int plane_at[kBlocks], row_at, boxes = 0;    // of the step whose V is copied next
   auto fetch_pages = [&]() {
 #pragma unroll
-    for (int i = 0; i < C::kBlocks; ++i) {
-      const int key = ahead.tile * C::kTile + warp * C::kKeys + i * 16;
-      page_id[i] = key < ahead.length
-                       ? p.table[ahead.b * p.table_stride + (key >> p.page_shift)] : 0;
+    for (int i = 0; i < kBlocks; ++i) {
+      const int key = ahead.tile * C::kTile + warp * kKeys + i * 16;
+      page_next[i] = key < ahead.length
+                         ? p.table[ahead.b * p.table_stride + (key >> p.page_shift)] : 0;
     }
   };
-  // Starts the copies of this warp's keys at `ahead` into stage st. Rows from the sequence's
-  // end on, and blocks with a page id outside the cache, are filled with zeros.
-  auto copy_stage = [&](int st) {
-    const int h = ahead.hr / p.row_blocks;
-    const int key0 = ahead.tile * C::kTile + warp * C::kKeys;
-    const uint32_t dst = slots + st * C::kSlot;
+  int issue_slot = 0;
+  auto copy_unit = [&](const CUtensorMap* map) {
+    if (lane == 0) {
+      uint64_t* bar = full + issue_slot;
+      const uint32_t dst = ring + issue_slot * C::kUnit;
+      mbar_arrive_expect_tx(bar, boxes * box * (C::kPlanes * C::kCols));
 #pragma unroll
-    for (int i = 0; i < C::kBlocks; ++i) {
-      const int key = key0 + i * 16;
-      if (key >= ahead.length) continue;
-      int id = page_id[i];
-      int rows = min(16, ahead.length - key);
-      if (static_cast<unsigned>(id) >= static_cast<unsigned>(p.num_pages)) {
-        if (lane == 0 && p.status) atomicOr(p.status, TA_DEVSTAT_BAD_PAGE);
-        id = 0;
-        rows = 0;
-      }
-      const int64_t ph = static_cast<int64_t>(id) * p.Hkv + h;
-      const int64_t off = (ph * p.page + (key & (p.page - 1))) * static_cast<int64_t>(p.D);
-      const uint8_t* kp = p.pages[0] + off;
-      const uint8_t* vp = p.pages[1] + off;
-      const int full = rows * d_chunks;  // chunks that exist
-      if (!padded) {
+      for (int i = 0; i < kBlocks; ++i)
+        if (plane_at[i] >= 0 && (i * 16) % box == 0)
 #pragma unroll
-        for (int c0 = 0; c0 < NJ * 2; ++c0) {
-          const int e = c0 * 32 + lane;
-          const int row = e / (NJ * 4), c = e % (NJ * 4);
-          const uint32_t to = dst + chunk_at<C::kPitch>(i * 16 + row, c);
-          const uint32_t n = e < full ? 16u : 0u;
-          const int64_t from = n ? e * 16 : 0;
-          cp_async16(to, kp + from, n);
-          cp_async16(to + C::kKeys * C::kPitch, vp + from, n);
-        }
-      } else {
-        const int recip = (65536 + d_chunks - 1) / d_chunks;  // exact for e < 512
-        for (int e = lane; e < 16 * d_chunks; e += 32) {
-          const int row = (e * recip) >> 16, c = e - row * d_chunks;
-          const uint32_t to = dst + chunk_at<C::kPitch>(i * 16 + row, c);
-          const uint32_t n = e < full ? 16u : 0u;
-          const int64_t from = n ? e * 16 : 0;
-          cp_async16(to, kp + from, n);
-          cp_async16(to + C::kKeys * C::kPitch, vp + from, n);
-        }
-      }
-      if (lane < 2) cp_async4(scales + ((st * 2 + lane) * C::kBlocks + i) * 4, p.scale[lane] + ph);
+          for (int c = 0; c < C::kPlanes; ++c)
+            tma_load_3d(dst + c * C::kPlane + i * 16 * C::kCols, map, bar, c * 128,
+                        (row_at + i * 16) & (p.page - 1), plane_at[i]);
     }
+    issue_slot = issue_slot + 1 == kU ? 0 : issue_slot + 1;
   };
-
-  // ---- the run
-  const int64_t steps = w1 - w0;
-  fetch_pages();
+  auto copy_k = [&](int n) {  // step n, at `ahead`; then `ahead` moves on
+    if (n < steps) {
+      const int key0 = ahead.tile * C::kTile + warp * kKeys;
+      const uint32_t marks = (n & 3) * kBlocks;
+      left_out &= ~(((1u << kBlocks) - 1) << marks);
+      row_at = key0 & (p.page - 1);
+      boxes = 0;
 #pragma unroll
-  for (int s = 0; s < C::kStages - 1; ++s) {
-    if (s < steps) {
-      copy_stage(s);
-      if (s + 1 < steps) {
+      for (int i = 0; i < kBlocks; ++i) {
+        plane_at[i] = -1;
+        if (key0 + i * 16 >= ahead.length) continue;
+        if (static_cast<unsigned>(page_next[i]) >= static_cast<unsigned>(p.num_pages)) {
+          left_out |= 1u << (marks + i);
+          if (lane == 0 && p.status) atomicOr(p.status, TA_DEVSTAT_BAD_PAGE);
+          continue;
+        }
+        plane_at[i] = page_next[i] * p.Hkv + ahead.h;
+        if ((i * 16) % box == 0) ++boxes;
+        if (lane < 2)
+          cp_async4(scales + (((n & 3) * 2 + lane) * kBlocks + i) * 4, p.scale[lane] + plane_at[i]);
+      }
+      copy_unit(&map_k);
+      if (n + 1 < steps) {
         advance(ahead);
         fetch_pages();
       }
     }
     cp_commit();
+  };
+  auto copy_v = [&](int n) {
+    if (n < steps) copy_unit(&map_v);
+  };
+  fetch_pages();
+#pragma unroll
+  for (int u = 0; u < kU - 1; ++u) {
+    if (u % 2 == 0) copy_k(u / 2);
+    else copy_v(u / 2);
   }
 
-  float o[MT][NJ * 8][4];
-  float m_run[MT][2], l_run[MT][2], mul[MT][2];
-  int lim[MT][2];
-  uint32_t qf[MT][NJ][4][4];
+  int slot = 0;
+  uint32_t parity = 0;
+  auto wait_unit = [&]() {
+    if (!mbar_wait_bounded(full + slot, parity, abort_flag, kTimeoutNs) && lane == 0 &&
+        !*abort_flag) {
+      *abort_flag = 1;
+      if (p.status) atomicOr(p.status, TA_DEVSTAT_TIMEOUT_LOAD);
+    }
+    __syncwarp();  // also: every lane is done with the unit before, which is filled again now
+  };
+  auto next_unit = [&]() {
+    if (++slot == kU) {
+      slot = 0;
+      parity ^= 1;
+    }
+  };
+
+  // Of 8-row tile nt a thread holds rows 2t and 2t + 1 of scores and output, row g of q.
+  float o[NJ * 4][NT][4];  // 16 dims: (g, 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1)
+  float ref[NT][2], l_run[NT][2], mul[NT][2];
+  int lim[NT][2];
+  uint32_t qf[C::kQShared ? 1 : NT][NJ * 4][2];  // chunk, pair of dims
+  uint4* s_q = reinterpret_cast<uint4*>(smem + C::kQOff);
+  int safe = 0;  // keys that every row with any keys sees
   bool fresh = true;
   int begin_tile = cur.tile;
-  int st = 0;
-  for (int64_t step = 0; step < steps; ++step) {
-    cp_wait<C::kStages - 2>();
+  for (int step = 0; step < steps; ++step) {
+    wait_unit();
+    if (kU % 2 == 1) copy_k(step + kU / 2);  // unit 2 step + kU - 1
+    else copy_v(step + kU / 2 - 1);
+    cp_wait<(kU - 1) / 2>();
     __syncwarp();
-    {  // the stage freed by the step before is filled again
-      const int64_t next = step + C::kStages - 1;
-      if (next < steps) {
-        copy_stage(st == 0 ? C::kStages - 1 : st - 1);
-        if (next + 1 < steps) {
-          advance(ahead);
-          fetch_pages();
-        }
-      }
-      cp_commit();
-    }
 
-    const int h = cur.hr / p.row_blocks, rb = cur.hr - h * p.row_blocks;
     if (fresh) {  // rows of a new (sequence, head): queries, limits, empty sums
       fresh = false;
       begin_tile = cur.tile;
       const SeqExtent e = extent_of(p, cur.b);
       const int rows = p.group * p.T;
+      int least = 0x7fffffff;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int n = 0; n < NJ * 8; ++n)
+        for (int m = 0; m < NJ * 4; ++m)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) o[mt][n][x] = 0.f;
+          for (int x = 0; x < 4; ++x) o[m][nt][x] = 0.f;
+        const int r = cur.rb * C::kRows + nt * 8 + g;
+        const int tok = r / p.group, hd = cur.h * p.group + (r - tok * p.group);
+        const bool real = r < rows && tok < e.count;
+        const int limit = real ? row_limit(e.length, e.count, tok, p.causal) : 0;
+        if (limit > 0) least = min(least, limit);
+        const uint16_t* q = static_cast<const uint16_t*>(p.q) + cur.b * p.q_sb +
+                            static_cast<int64_t>(hd) * p.q_sh + static_cast<int64_t>(tok) * p.q_ss;
+        uint2 w[NJ * 4];
+        float amax = 0.f;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int r = rb * C::kRows + mt * 16 + half * 8 + g;
-          const int tok = r / p.group, hd = h * p.group + (r - tok * p.group);
-          const bool real = r < rows && tok < e.count;
-          lim[mt][half] = real ? row_limit(e.length, e.count, tok, p.causal) : 0;
-          m_run[mt][half] = -INFINITY;
-          l_run[mt][half] = 0.f;
-          const uint16_t* q = static_cast<const uint16_t*>(p.q) + cur.b * p.q_sb +
-                              static_cast<int64_t>(hd) * p.q_sh + static_cast<int64_t>(tok) * p.q_ss;
-          uint32_t w[NJ][8];
-          float amax = 0.f;
+        for (int c = 0; c < NJ * 4; ++c) {
+          w[c] = make_uint2(0, 0);
+          if (real && c * 16 < p.D) w[c] = *reinterpret_cast<const uint2*>(q + c * 16 + t * 4);
+        }
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) {
+        for (int c = 0; c < NJ * 4; ++c) {
+          const float2 a = unpack16(w[c].x, p.bf16), b = unpack16(w[c].y, p.bf16);
+          amax = fmaxf(fmaxf(amax, fmaxf(fabsf(a.x), fabsf(a.y))), fmaxf(fabsf(b.x), fabsf(b.y)));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        // The row times a power of two, with its largest value in [2^14, 2^15): fp16 then holds
+        // every bf16 or fp16 value of the row to 2^-39 of the largest. Held to exponents whose
+        // factors are normal float32 values.
+        const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 14, -126), 113);
+        const float up = pow2f(-ex), factor = p.scale_log2 * pow2f(ex);
+        uint32_t f[NJ * 4][2];
 #pragma unroll
-            for (int v = 0; v < 2; ++v) {
-              const int c = j * 4 + t;  // 16 dims from 16 c
-              uint4 x = make_uint4(0, 0, 0, 0);
-              if (real && c < d_chunks) x = *reinterpret_cast<const uint4*>(q + c * 16 + v * 8);
-              w[j][4 * v] = x.x;
-              w[j][4 * v + 1] = x.y;
-              w[j][4 * v + 2] = x.z;
-              w[j][4 * v + 3] = x.w;
+        for (int c = 0; c < NJ * 4; ++c) {
+          const float2 a = unpack16(w[c].x, p.bf16), b = unpack16(w[c].y, p.bf16);
+          f[c][0] = pack_f16(a.x * up, a.y * up);
+          f[c][1] = pack_f16(b.x * up, b.y * up);
+        }
+        if constexpr (C::kQShared) {  // one copy for the block
+#pragma unroll
+          for (int c = 0; c < NJ * 4; c += 2)
+            if (c / 2 % kWarps == warp)
+              s_q[(nt * NJ * 2 + c / 2) * 32 + lane] =
+                  make_uint4(f[c][0], f[c][1], f[c + 1][0], f[c + 1][1]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < NJ * 4; ++c) {
+            qf[nt][c][0] = f[c][0];
+            qf[nt][c][1] = f[c][1];
+          }
+        }
+#pragma unroll
+        for (int r2 = 0; r2 < 2; ++r2) {  // from row g's lanes to those of columns 2t, 2t + 1
+          lim[nt][r2] = __shfl_sync(0xffffffffu, limit, (2 * t + r2) * 4);
+          mul[nt][r2] = __shfl_sync(0xffffffffu, factor, (2 * t + r2) * 4);
+          ref[nt][r2] = -INFINITY;
+          l_run[nt][r2] = 0.f;
+        }
+      }
+      safe = __reduce_min_sync(0xffffffffu, least);
+      if constexpr (C::kQShared) __syncthreads();
+    }
+
+    const int key0 = cur.tile * C::kTile + warp * kKeys;
+    const bool any = key0 < cur.length;
+    float s[kBlocks][NT][4];  // keys (set 0, g) and (set 1, g) by rows 2t, 2t + 1
+    if (any) {
+      const uint32_t kb = ring + slot * C::kUnit;
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[i][nt][x] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NJ * 4; c += 2) {
+        uint4 qc[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if constexpr (C::kQShared) qc[nt] = s_q[(nt * NJ * 2 + c / 2) * 32 + lane];
+          else qc[nt] = make_uint4(qf[nt][c][0], qf[nt][c][1], qf[nt][c + 1][0], qf[nt][c + 1][1]);
+        }
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+          uint32_t w[4];  // (set 0, chunk c), (set 1, c), (set 0, c + 1), (set 1, c + 1)
+          ldsm_codes(kb + chunk_at<C::kCols, C::kPlane>(
+                              i * 16 + key_of_column(lane & 7, (lane >> 3) & 1), c + (lane >> 4)), w);
+          uint32_t a[4][2];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) codes_to_f16(w[x], a[x][0], a[x][1]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816(s[i][nt], a[0][0], a[1][0], a[0][1], a[1][1], qc[nt].x, qc[nt].y);
+            mma16816(s[i][nt], a[2][0], a[3][0], a[2][1], a[3][1], qc[nt].z, qc[nt].w);
+          }
+        }
+      }
+    }
+    next_unit();
+
+    uint32_t pf[kBlocks][NT][2];  // weights as the second product's B: set 0, set 1
+    if (any) {
+      // t = score * c + e: the scales of the block's page
+      float c[kBlocks][NT][2], e[kBlocks], back[kBlocks];
+      const uint32_t marks = left_out >> ((step & 3) * kBlocks) & ((1u << kBlocks) - 1);
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) {
+        const uint32_t at = scales + ((step & 3) * 2 * kBlocks + i) * 4;
+        const float ks = lds32(at);
+        const int ev = stored_exponent(__float_as_uint(lds32(at + kBlocks * 4)));
+        back[i] = pow2f(-ev);
+        e[i] = static_cast<float>(ev);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          c[i][nt][0] = mul[nt][0] * ks;
+          c[i][nt][1] = mul[nt][1] * ks;
+        }
+      }
+      if (key0 + kKeys > safe || marks) {  // some row's limit, or pages to leave out
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int key = marks >> i & 1 ? 0x7fffffff : key0 + i * 16 + key_of_column(g, x >> 1);
+              s[i][nt][x] = key < lim[nt][x & 1] ? fmaf(s[i][nt][x], c[i][nt][x & 1], e[i]) : -INFINITY;
             }
 #pragma unroll
-            for (int v = 0; v < 8; ++v) {
-              const float2 a = unpack16(w[j][v], p.bf16);
-              amax = fmaxf(amax, fmaxf(fabsf(a.x), fabsf(a.y)));
+          for (int nt = 0; nt < NT; ++nt) c[i][nt][0] = c[i][nt][1] = 1.f;
+          e[i] = 0.f;
+        }
+      }
+      float cand[NT][2];
+      bool grow = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float m = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kBlocks; ++i)
+            m = fmaxf(m, fmaf(fmaxf(s[i][nt][r], s[i][nt][2 + r]), c[i][nt][r], e[i]));
+          cand[nt][r] = m;
+          grow |= m > ref[nt][r] + kGrowth;
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float a[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float m = cand[nt][r];  // over the row's keys: the lanes of one t
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            a[r] = 1.f;
+            if (m > ref[nt][r] + kGrowth) {
+              const float to = m - kBelow;
+              a[r] = ex2_approx(ref[nt][r] - to);  // 0 from -inf
+              ref[nt][r] = to;
+              l_run[nt][r] *= a[r];
             }
           }
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-          // The row times a power of two, with its largest value in [2^13, 2^14): fp16 then
-          // holds every bf16 or fp16 value of the row to 2^-38 of the largest. Held to
-          // exponents whose factors are normal float32 values.
-          const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 13, -126), 113);
-          const float up = pow2f(-ex);
-          mul[mt][half] = p.scale_log2 * pow2f(ex);
 #pragma unroll
-          for (int j = 0; j < NJ; ++j)
+          for (int m = 0; m < NJ * 4; ++m) {
+            o[m][nt][0] *= a[0];
+            o[m][nt][1] *= a[1];
+            o[m][nt][2] *= a[0];
+            o[m][nt][3] *= a[1];
+          }
+        }
+      }
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              const float2 a = unpack16(w[j][2 * v], p.bf16);
-              const float2 c = unpack16(w[j][2 * v + 1], p.bf16);
-              qf[mt][j][v][half] = pack_f16(a.x * up, a.y * up);
-              qf[mt][j][v][2 + half] = pack_f16(c.x * up, c.y * up);
-            }
+      for (int nt = 0; nt < NT; ++nt) {
+        const float r0 = ref[nt][0] == -INFINITY ? 0.f : ref[nt][0];
+        const float r1 = ref[nt][1] == -INFINITY ? 0.f : ref[nt][1];
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+          const float(&x)[4] = s[i][nt];
+          const float w0 = ex2_approx(fmaf(x[0], c[i][nt][0], e[i] - r0));
+          const float w1 = ex2_approx(fmaf(x[1], c[i][nt][1], e[i] - r1));
+          const float w2 = ex2_approx(fmaf(x[2], c[i][nt][0], e[i] - r0));
+          const float w3 = ex2_approx(fmaf(x[3], c[i][nt][1], e[i] - r1));
+          l_run[nt][0] = fmaf(w0 + w2, back[i], l_run[nt][0]);
+          l_run[nt][1] = fmaf(w1 + w3, back[i], l_run[nt][1]);
+          pf[i][nt][0] = transpose8(pack_f16(w0, w1));
+          pf[i][nt][1] = transpose8(pack_f16(w2, w3));
         }
       }
     }
 
-    const int key0 = cur.tile * C::kTile + warp * C::kKeys;
-    if (key0 < cur.length) {
-      const uint32_t kb = slots + st * C::kSlot;
-      const uint32_t vb = kb + C::kKeys * C::kPitch;
-      // scores
-      float s[MT][2 * C::kBlocks][4];
-#pragma unroll
-      for (int nt = 0; nt < 2 * C::kBlocks; ++nt) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) s[mt][nt][x] = 0.f;
-        const int row = (nt >> 1) * 16 + key_of_column(g, nt & 1);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const uint4 kw = lds128(kb + chunk_at<C::kPitch>(row, j * 4 + t));
-          const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            uint32_t f0, f1;
-            codes_to_f16(w[v], f0, f1);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) mma16816(s[mt][nt], qf[mt][j][v], f0, f1);
-          }
-        }
-      }
-      // t = score * scales + exponent of the value scale; maxima
-      float back[C::kBlocks];
-#pragma unroll
-      for (int i = 0; i < C::kBlocks; ++i) {
-        const float ks = lds32(scales + (st * 2 * C::kBlocks + i) * 4);
-        const int ev = stored_exponent(__float_as_uint(lds32(scales + ((st * 2 + 1) * C::kBlocks + i) * 4)));
-        back[i] = pow2f(-ev);
-        const float evf = static_cast<float>(ev);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const float c0 = mul[mt][0] * ks, c1 = mul[mt][1] * ks;
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const int key = key0 + i * 16 + 4 * t + 2 * hf;
-            float(&x)[4] = s[mt][2 * i + hf];
-            x[0] = key < lim[mt][0] ? fmaf(x[0], c0, evf) : -INFINITY;
-            x[1] = key + 1 < lim[mt][0] ? fmaf(x[1], c0, evf) : -INFINITY;
-            x[2] = key < lim[mt][1] ? fmaf(x[2], c1, evf) : -INFINITY;
-            x[3] = key + 1 < lim[mt][1] ? fmaf(x[3], c1, evf) : -INFINITY;
-          }
-        }
-      }
-      float cand[MT][2];
-      bool grow = false;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float c = -INFINITY;
-#pragma unroll
-          for (int nt = 0; nt < 2 * C::kBlocks; ++nt)
-            c = fmaxf(c, fmaxf(s[mt][nt][2 * half], s[mt][nt][2 * half + 1]));
-          c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, 1));
-          c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, 2));
-          cand[mt][half] = c;
-          grow |= c > m_run[mt][half] + kGrowth;
-        }
-      if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          float a[2];
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            a[half] = 1.f;
-            if (cand[mt][half] > m_run[mt][half] + kGrowth) {
-              a[half] = ex2_approx(m_run[mt][half] - cand[mt][half]);  // 0 from -inf
-              m_run[mt][half] = cand[mt][half];
-              l_run[mt][half] *= a[half];
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NJ * 8; ++n) {
-            o[mt][n][0] *= a[0];
-            o[mt][n][1] *= a[0];
-            o[mt][n][2] *= a[1];
-            o[mt][n][3] *= a[1];
-          }
-        }
-      }
-      // weights and the second product
-#pragma unroll
-      for (int i = 0; i < C::kBlocks; ++i) {
-        // Blocks from the sequence's end on were not copied: what their stage holds must not
-        // meet a weight of zero (0 * NaN).
-        if (i > 0 && key0 + i * 16 >= cur.length) break;
-        // A key that some row may not see yet (later tokens of the same call) must not reach
-        // that row through 0 * NaN either.
-        bool later = false;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-            later |= lim[mt][half] > 0 && lim[mt][half] < min(cur.length, key0 + i * 16 + 16);
-        if (__any_sync(0xffffffffu, later)) {
-          bool nan = false;
-          for (int e = lane; e < 64 * NJ; e += 32)
-            nan |= any_nan(lds128(vb + chunk_at<C::kPitch>(i * 16 + e / (NJ * 4), e % (NJ * 4))));
-          if (__any_sync(0xffffffffu, nan)) {
+    wait_unit();
+    if (kU % 2 == 1) copy_v(step + kU / 2);  // unit 2 step + 1 + kU - 1
+    else copy_k(step + kU / 2);
+    if (any) {
+      const uint32_t vb = ring + slot * C::kUnit;
+      // What a stage holds must not meet a weight of zero where it may be NaN (0 * NaN): blocks
+      // that were not copied, and keys that some row does not see (the rest of the last page,
+      // later tokens of the same call).
+      const uint32_t marks = left_out >> ((step & 3) * kBlocks) & ((1u << kBlocks) - 1);
+      if (key0 + kKeys > safe || marks) {
+#pragma unroll 1
+        for (int i = 0; i < kBlocks; ++i) {
+          const bool copied = key0 + i * 16 < cur.length && !(marks >> i & 1);
+          bool nan = !copied;
+          if (copied && key0 + i * 16 + 16 > safe)
+            for (int x = lane; x < 64 * NJ; x += 32)
+              nan |= any_nan(lds128(vb + chunk_at<C::kCols, C::kPlane>(i * 16 + x / (NJ * 4), x % (NJ * 4))));
+          if (!__any_sync(0xffffffffu, nan)) continue;
+          if (copied) {
 #pragma unroll 1
             for (int key = 0; key < 16; ++key)
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt)
+              for (int m = 0; m < NJ * 4; ++m)
 #pragma unroll
-                for (int n = 0; n < NJ * 8; ++n)
+                for (int hi = 0; hi < 2; ++hi) {
+                  const uint32_t code =
+                      lds8(vb + chunk_at<C::kCols, C::kPlane>(i * 16 + key, m) + g + 8 * hi);
+                  if ((code & 0x7fu) != 0x7fu) continue;
 #pragma unroll
-                  for (int x = 0; x < 4; ++x) {
-                    const int d = n * 8 + 2 * t + (x & 1);
-                    const uint32_t c = lds8(vb + chunk_at<C::kPitch>(i * 16 + key, d >> 4) + (d & 15));
-                    if ((c & 0x7fu) == 0x7fu && key0 + i * 16 + key < lim[mt][x >> 1])
-                      o[mt][n][x] = __int_as_float(0x7fffffff);
-                  }
-            __syncwarp();
-            for (int e = lane; e < 64 * NJ; e += 32) {
-              const uint32_t at = vb + chunk_at<C::kPitch>(i * 16 + e / (NJ * 4), e % (NJ * 4));
-              sts128(at, without_nan(lds128(at)));
-            }
+                  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                      if (key0 + i * 16 + key < lim[nt][r])
+                        o[m][nt][2 * hi + r] = __int_as_float(0x7fffffff);
+                }
             __syncwarp();
           }
-        }
-        uint32_t pf[MT][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const float m0 = m_run[mt][0] == -INFINITY ? 0.f : m_run[mt][0];
-          const float m1 = m_run[mt][1] == -INFINITY ? 0.f : m_run[mt][1];
-          float e[2][4];
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const float(&x)[4] = s[mt][2 * i + hf];
-            e[hf][0] = ex2_approx(x[0] - m0);
-            e[hf][1] = ex2_approx(x[1] - m0);
-            e[hf][2] = ex2_approx(x[2] - m1);
-            e[hf][3] = ex2_approx(x[3] - m1);
-            pf[mt][2 * hf] = pack_f16(e[hf][0], e[hf][1]);
-            pf[mt][2 * hf + 1] = pack_f16(e[hf][2], e[hf][3]);
+          for (int x = lane; x < 64 * NJ; x += 32) {
+            const uint32_t at = vb + chunk_at<C::kCols, C::kPlane>(i * 16 + x / (NJ * 4), x % (NJ * 4));
+            sts128(at, copied ? without_nan(lds128(at)) : make_uint4(0, 0, 0, 0));
           }
-          l_run[mt][0] = fmaf((e[0][0] + e[0][1]) + (e[1][0] + e[1][1]), back[i], l_run[mt][0]);
-          l_run[mt][1] = fmaf((e[0][2] + e[0][3]) + (e[1][2] + e[1][3]), back[i], l_run[mt][1]);
-        }
-#pragma unroll
-        for (int n = 0; n < NJ * 2; ++n) {  // 32 dims
-          uint32_t w[4];
-          ldsm_codes_t(vb + chunk_at<C::kPitch>(i * 16 + (lane & 15), n * 2 + (lane >> 4)), w);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            uint32_t f0, f1;
-            codes_to_f16(w[x], f0, f1);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][n * 4 + x], pf[mt], f0, f1);
-          }
+          fence_proxy_async_shared();  // before the next copy into this unit
+          __syncwarp();
         }
       }
+#pragma unroll
+      for (int n = 0; n < NJ * 2; ++n)  // 32 dims
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+          uint32_t w[4];
+          ldsm_codes_t(vb + chunk_at<C::kCols, C::kPlane>(i * 16 + key_at(lane & 15), n * 2 + (lane >> 4)),
+                       w);
+          uint32_t a[4][2];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) codes_to_f16(w[x], a[x][0], a[x][1]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816(o[2 * n][nt], a[0][0], a[1][0], a[0][1], a[1][1], pf[i][nt][0], pf[i][nt][1]);
+            mma16816(o[2 * n + 1][nt], a[2][0], a[3][0], a[2][1], a[3][1], pf[i][nt][0], pf[i][nt][1]);
+          }
+        }
     }
 
     // ---- the end of this (sequence, head) or of the run: merge the warps
@@ -590,56 +684,57 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
     if (seq_end || step + 1 == steps) {
       const bool whole = seq_end && begin_tile == 0;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float l = l_run[mt][half];
-          l += __shfl_xor_sync(0xffffffffu, l, 1);
-          l += __shfl_xor_sync(0xffffffffu, l, 2);
-          if (t == 0) {
-            s_m[warp * C::kRows + mt * 16 + half * 8 + g] = m_run[mt][half];
-            s_l[warp * C::kRows + mt * 16 + half * 8 + g] = l;
+        for (int r = 0; r < 2; ++r) {
+          if (lim[nt][r] == 0) {  // a row without keys: its unmasked scores were of no row
+            ref[nt][r] = -INFINITY;
+            l_run[nt][r] = 0.f;
+          }
+          float l = l_run[nt][r];
+          l += __shfl_xor_sync(0xffffffffu, l, 4);
+          l += __shfl_xor_sync(0xffffffffu, l, 8);
+          l += __shfl_xor_sync(0xffffffffu, l, 16);
+          if (g == 0) {
+            s_m[warp * C::kRows + nt * 8 + 2 * t + r] = ref[nt][r];
+            s_l[warp * C::kRows + nt * 8 + 2 * t + r] = l;
           }
         }
       __syncthreads();
-      float f[MT][2];
+      float f[NT][2];  // the warp's share of a row; outputs without a reference are none
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int r = mt * 16 + half * 8 + g;
-          float m = s_m[r];
+        for (int r = 0; r < 2; ++r) {
+          float m = s_m[nt * 8 + 2 * t + r];
 #pragma unroll
-          for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w * C::kRows + r]);
-          f[mt][half] = ex2_approx(m_run[mt][half] - m);  // unused where the maximum is -inf
+          for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w * C::kRows + nt * 8 + 2 * t + r]);
+          f[nt][r] = ex2_approx(ref[nt][r] - m);
         }
-      // A warp's just-read stage is free until the next step's copies: it takes the warp's
+      // A warp's just-read unit is free until the next step's copies: it takes the warp's
       // output, kMergeCols dims at a time, and all threads add the four.
-      float* mine = reinterpret_cast<float*>(smem + (warp * C::kStages + st) * C::kSlot);
-      constexpr int kMask = C::kMergeCols / 8 < 8 ? C::kMergeCols / 8 - 1 : 7;
+      float* mine = reinterpret_cast<float*>(smem + (warp * kU + slot) * C::kUnit);
+      constexpr int kMask = C::kMergeCols / 8 < 4 ? C::kMergeCols / 8 - 1 : 3;  // banks: see below
       const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + (begin_tile == 0 ? 1 : 0)) * C::kRows;
 #pragma unroll
       for (int pass = 0; pass < C::kPasses; ++pass) {
         if (pass > 0) __syncthreads();
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int m = 0; m < NJ * 8; ++m) {  // 8 dims
+          if (m * 8 / C::kMergeCols != pass) continue;
+          const int col = (m * 8 - pass * C::kMergeCols + g) ^ ((t & kMask) * 8);  // t: row / 2
 #pragma unroll
-          for (int n = 0; n < NJ * 8; ++n) {
-            if (n * 8 / C::kMergeCols != pass) continue;
-            const int col = n * 8 - pass * C::kMergeCols + 2 * t;
-            const int r0 = mt * 16 + g;
-            const int x = (r0 & kMask) * 8;  // rows r0 and r0 + 8 alike
-            const bool any0 = m_run[mt][0] != -INFINITY, any1 = m_run[mt][1] != -INFINITY;
-            *reinterpret_cast<float2*>(mine + r0 * C::kMergeCols + (col ^ x)) =
-                make_float2(any0 ? o[mt][n][0] * f[mt][0] : 0.f, any0 ? o[mt][n][1] * f[mt][0] : 0.f);
-            *reinterpret_cast<float2*>(mine + (r0 + 8) * C::kMergeCols + (col ^ x)) =
-                make_float2(any1 ? o[mt][n][2] * f[mt][1] : 0.f, any1 ? o[mt][n][3] * f[mt][1] : 0.f);
-          }
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+              mine[(nt * 8 + 2 * t + r) * C::kMergeCols + col] =
+                  ref[nt][r] != -INFINITY ? o[m / 2][nt][2 * (m & 1) + r] * f[nt][r] : 0.f;
+        }
         __syncthreads();
         for (int i = threadIdx.x; i < C::kRows * C::kMergeCols / 4; i += kThreads) {
           const int r = i / (C::kMergeCols / 4), c4 = (i % (C::kMergeCols / 4)) * 4;
           const int d = pass * C::kMergeCols + c4;
-          const int row = rb * C::kRows + r;
+          const int row = cur.rb * C::kRows + r;
           if (row >= p.group * p.T || d >= p.D) continue;
           float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
           float m = -INFINITY, l = 0.f;
@@ -648,18 +743,18 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
             const float4 v = *reinterpret_cast<const float4*>(
-                smem + (w * C::kStages + st) * C::kSlot +
-                4 * (r * C::kMergeCols + (c4 ^ ((r & kMask) * 8))));
+                smem + (w * kU + slot) * C::kUnit +
+                4 * (r * C::kMergeCols + (c4 ^ (((r >> 1) & kMask) * 8))));
             a.x += v.x;
             a.y += v.y;
             a.z += v.z;
             a.w += v.w;
             const float mw = s_m[w * C::kRows + r];
-            // A sum without a maximum is 0, or NaN where every score was NaN: it is kept.
+            // A sum without a reference is 0, or NaN where every score was NaN: it is kept.
             l = fmaf(s_l[w * C::kRows + r], mw == -INFINITY ? 1.f : ex2_approx(mw - m), l);
           }
           if (whole) {
-            const int tok = row / p.group, hd = h * p.group + (row - tok * p.group);
+            const int tok = row / p.group, hd = cur.h * p.group + (row - tok * p.group);
             const float inv = l == 0.f ? 0.f : 1.f / l;
             uint16_t* out = static_cast<uint16_t*>(p.o) + cur.b * p.o_sb + hd * p.o_sh + tok * p.o_ss + d;
             *reinterpret_cast<uint2*>(out) = make_uint2(pack16(a.x * inv, a.y * inv, p.bf16),
@@ -673,26 +768,29 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const AttendParams 
           }
         }
       }
+      fence_proxy_async_shared();  // before the next copy into this unit
       __syncthreads();
-      if (padded) {  // the merge wrote over the zero columns of this warp's stage
-        uint4* z = reinterpret_cast<uint4*>(mine);
-        for (int i = lane; i < C::kSlot / 16; i += 32) z[i] = make_uint4(0, 0, 0, 0);
-        __syncwarp();
-      }
       fresh = true;
     }
+    next_unit();
     advance(cur);
-    st = st + 1 == C::kStages ? 0 : st + 1;
+  }
+  if (*abort_flag) {  // a copy was late: every issued one must land before the block ends
+    volatile int no_abort = 0;
+    for (int u = max(0, 2 * steps - kU); u < 2 * steps; ++u)
+      if (!mbar_wait_bounded(full + u % kU, (u / kU) & 1, &no_abort, kTimeoutNs) && lane == 0 &&
+          p.status)
+        atomicOr(p.status, TA_DEVSTAT_TIMEOUT_DRAIN);
   }
 }
 
 // Merges the partial results of (sequence, head)s that several runs share, and writes the rows
 // of sequences without keys. One block: kWarps rows, a warp each, or with `spread` one row
 // whose runs the warps divide (few rows, many runs).
-template <int NJ, int MT>
+template <int NJ, int NT>
 __global__ void __launch_bounds__(kThreads) merge_kernel(const AttendParams p, int parts_max,
                                                          int spread) {
-  using C = Cfg<NJ, MT>;
+  using C = Cfg<NJ, NT>;
   constexpr int kVec = NJ <= 2 ? 1 : 2;  // float4 a lane: 32 lanes cover the head dim
   __shared__ int64_t s_scan[kWarps];
   __shared__ float s_o[kWarps][NJ * 64];
@@ -813,15 +911,12 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const AttendParams p, i
     p.lse[(static_cast<int64_t>(b) * p.Hq + hd) * p.T + tok] = lse_of(m, l);
 }
 
-// Rows per block: one 16-row tile while they fit, else (up to head dim 128) two, so that a
-// cache read serves 32 rows.
-int m_tiles(int rows, int D) { return rows > 16 && D <= 128 ? 2 : 1; }
-
-template <int NJ, int MT>
-cudaError_t launch(AttendParams p, int sm_count, cudaStream_t stream) {
-  using C = Cfg<NJ, MT>;
-  static_assert(C::kStages >= 2, "two stages at least");
-  auto kern = attend_kernel<NJ, MT>;
+template <int NJ, int NT>
+cudaError_t launch(AttendParams p, const CUtensorMap& map_k, const CUtensorMap& map_v, int sm_count,
+                   cudaStream_t stream) {
+  using C = Cfg<NJ, NT>;
+  static_assert(C::kUnits >= 3 && (C::kUnits - 1) / 2 + 1 < C::kScaleSteps, "ring and scales");
+  auto kern = attend_kernel<NJ, NT>;
   static int configured = 0;  // one bit per device ordinal (< 32)
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
@@ -838,10 +933,11 @@ cudaError_t launch(AttendParams p, int sm_count, cudaStream_t stream) {
   const int64_t per_seq = seq_tiles * p.Hkv * p.row_blocks;
   if (per_seq > 0x7fffffffll) return cudaErrorInvalidValue;
   const int64_t most = per_seq * p.B;
-  const int parts = static_cast<int>(most < 2ll * sm_count ? most : 2ll * sm_count);
-  const int64_t part_rows = static_cast<int64_t>(2 * sm_count) * 2 * C::kRows;
+  const int64_t resident = static_cast<int64_t>(C::kBlocksPerSm) * sm_count;
+  const int parts = static_cast<int>(most < resident ? most : resident);
+  const int64_t part_rows = resident * 2 * C::kRows;
   p.part_ml = p.part_o + part_rows * C::kDim;
-  kern<<<parts, kThreads, C::kBytes, stream>>>(p, p.D / 16);
+  kern<<<parts, kThreads, C::kBytes, stream>>>(map_k, map_v, p);
   if ((err = cudaGetLastError()) != cudaSuccess) return err;
 
   const int64_t few = static_cast<int64_t>(p.B) * p.Hkv * rows;
@@ -857,28 +953,53 @@ cudaError_t launch(AttendParams p, int sm_count, cudaStream_t stream) {
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, merge_kernel<NJ, MT>, p, parts, spread);
+  return cudaLaunchKernelEx(&cfg, merge_kernel<NJ, NT>, p, parts, spread);
+}
+
+// One configuration, as an argument.
+template <int NJ, int NT>
+struct Shape {
+  using Config = Cfg<NJ, NT>;
+  static cudaError_t launch(const AttendParams& p, const CUtensorMap& k, const CUtensorMap& v, int sms,
+                            cudaStream_t stream) {
+    return kv8::launch<NJ, NT>(p, k, v, sms, stream);
+  }
+};
+
+// Calls f with the configuration that serves `rows` rows of head dim D: up to 8 rows one tile, up to
+// 16 two, more four while the head dim leaves registers for them, so that a cache read serves
+// 32 rows.
+template <class F>
+auto with_config(int rows, int D, F f) {
+  const int nj = (D + 63) / 64;
+  if (rows <= 8) {
+    if (nj == 1) return f(Shape<1, 1>());
+    if (nj == 2) return f(Shape<2, 1>());
+    if (nj == 3) return f(Shape<3, 1>());
+    return f(Shape<4, 1>());
+  }
+  if (rows > 16 && nj == 1) return f(Shape<1, 4>());
+  if (rows > 16 && nj == 2) return f(Shape<2, 4>());
+  if (nj == 1) return f(Shape<1, 2>());
+  if (nj == 2) return f(Shape<2, 2>());
+  if (nj == 3) return f(Shape<3, 2>());
+  return f(Shape<4, 2>());
 }
 
 }  // namespace
 
 size_t attend_workspace_bytes(int, int Hq, int Hkv, int T, int D, int sm_count) {
-  const int64_t rows = static_cast<int64_t>(2 * sm_count) * 2 * 16 *
-                       m_tiles((Hq / Hkv) * T, D);
-  const int dim = (D + 63) / 64 * 64;
-  return static_cast<size_t>(rows) * (dim + 2) * sizeof(float);
+  return with_config((Hq / Hkv) * T, D, [&](auto shape) {
+    using C = typename decltype(shape)::Config;
+    return static_cast<size_t>(C::kBlocksPerSm) * sm_count * 2 * C::kRows * (C::kDim + 2) * sizeof(float);
+  });
 }
 
-cudaError_t launch_attend(const AttendParams& p, int sm_count, cudaStream_t stream) {
-  const int nj = (p.D + 63) / 64;
-  const int mt = m_tiles(p.group * p.T, p.D);
-  if (mt == 2) return nj == 1 ? launch<1, 2>(p, sm_count, stream) : launch<2, 2>(p, sm_count, stream);
-  switch (nj) {
-    case 1: return launch<1, 1>(p, sm_count, stream);
-    case 2: return launch<2, 1>(p, sm_count, stream);
-    case 3: return launch<3, 1>(p, sm_count, stream);
-    default: return launch<4, 1>(p, sm_count, stream);
-  }
+cudaError_t launch_attend(const AttendParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v,
+                          int sm_count, cudaStream_t stream) {
+  return with_config(p.group * p.T, p.D, [&](auto shape) {
+    return decltype(shape)::launch(p, map_k, map_v, sm_count, stream);
+  });
 }
 
 }  // namespace kv8

@@ -222,8 +222,8 @@ def sdpa_kv_cache(q, cache: KVCache8, page_table, lengths, *, counts=None, causa
     Returns a new [B, Hq, T, D] tensor of q's dtype (with return_lse also the float32
     [B, Hq, T] natural-log log-sum-exp), computed asynchronously on the current torch stream.
     Rows that see no key, and rows from counts[b] on, are 0 with lse -inf. Not differentiable.
-    Page ids outside the cache read as zeros and lengths and counts outside their range are held
-    in range: both are reported by check_device_status().
+    Tokens of page ids outside the cache are left out, and lengths and counts outside their range
+    held in range: both are reported by check_device_status().
     """
     fast = _native._fast
     # -1.0 is the launcher's code for the default scale: a caller's own must be positive.
