@@ -155,6 +155,39 @@ def test_rotary_gradient(inter):
     assert torch.equal(g, q.grad)
     with torch.no_grad():
         assert not ta.rotary(q, None, pos, freq)[0].requires_grad
+    # a gradient that is one value everywhere comes without strides
+    (g,) = torch.autograd.grad(ta.rotary(q, None, pos, freq, interleaved=inter)[0].sum(), q)
+    want, tol = plain.rotary64(torch.ones_like(q), pos, freq, inter, 1.0, True)
+    _within(g, want, tol)
+
+
+@pytest.mark.parametrize("fast", [True, False])
+def test_rotary_second_gradient_and_both_launchers(fast, monkeypatch):
+    """The gradient is differentiable too: turning there and back gives the gradient's own."""
+    import tiledattention_b200 as ta
+    from tiledattention_b200 import _native
+
+    freq, _ = ta.rotary_frequencies(64, device=DEV)
+    pos = torch.arange(5, device=DEV)
+    q = _randn(2, 3, 5, 64, dtype=FP16, seed=1).requires_grad_()
+    k = _randn(2, 1, 5, 64, dtype=FP16, seed=2).requires_grad_()
+    ta.rotary(q, k, pos, freq)
+    if not fast:
+        monkeypatch.setattr(_native, "_fast", None)
+    gq = _randn(2, 3, 5, 64, dtype=FP16, seed=3).requires_grad_()
+    gk = _randn(2, 1, 5, 64, dtype=FP16, seed=4)
+    oq, ok = ta.rotary(q, k, pos, freq, magnitude=1.5)
+    dq, dk = torch.autograd.grad((oq, ok), (q, k), (gq, gk), create_graph=True)
+    for d, g in ((dq, gq), (dk, gk)):
+        want, tol = plain.rotary64(g.detach(), pos, freq, False, 1.5, True)
+        _within(d, want, tol)
+    u = _randn(2, 3, 5, 64, dtype=FP16, seed=5)
+    (dd,) = torch.autograd.grad(dq, gq, u)
+    want, tol = plain.rotary64(u, pos, freq, False, 1.5, False)
+    _within(dd, want, tol)
+    (only,) = torch.autograd.grad(ta.rotary(q.detach(), k, pos, freq)[1], k, gk)
+    want, tol = plain.rotary64(gk, pos, freq, False, 1.0, True)
+    _within(only, want, tol)
 
 
 def test_rotary_stream_graph_and_python_path(monkeypatch):

@@ -37,9 +37,11 @@
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
+#include <optional>
 #include <tuple>
 
 #include "tiledattention_b200.h"
@@ -234,8 +236,98 @@ bool int_vector(const at::Tensor* t, int64_t n, c10::Device dev) {
          t->device() == dev && (n <= 1 || t->stride(0) == 1);
 }
 
+// rotary(q, k, positions, inv_freq) on tensors as the kernel takes them: false, having done
+// nothing, for everything else.
+struct RotaryHow {
+  bool interleaved;
+  double magnitude;
+  bool inverse;
+};
+bool rotary_launch(const at::Tensor& q, const at::Tensor* k, const at::Tensor& pos,
+                   const at::Tensor& freq, const RotaryHow& how, at::Tensor& qo, at::Tensor& ko) {
+  if (g_rotary == nullptr || q.dim() != 4 || !q.is_cuda() || !std::isfinite(how.magnitude))
+    return false;
+  const int dtype = dtype_code(q);
+  const c10::Device dev = q.device();
+  const int64_t B = q.size(0), H = q.size(1), S = q.size(2), D = q.size(3);
+  if (dtype < 0 || !fits_int(B) || !fits_int(H) || !fits_int(S) || !fits_int(D) || q.stride(3) != 1)
+    return false;
+  if (k && (k->dim() != 4 || k->device() != dev || dtype_code(*k) != dtype || k->size(0) != B ||
+            !fits_int(k->size(1)) || k->size(2) != S || k->size(3) != D || k->stride(3) != 1))
+    return false;
+  const auto pt = pos.scalar_type();
+  if (pos.device() != dev || (pt != at::kInt && pt != at::kLong)) return false;
+  const bool row = pos.dim() == 1;
+  if (!(row ? pos.size(0) == S
+            : pos.dim() == 2 && (pos.size(0) == B || pos.size(0) == 1) && pos.size(1) == S))
+    return false;
+  if (freq.device() != dev || freq.scalar_type() != at::kDouble || freq.dim() != 1 ||
+      freq.size(0) < 1 || 2 * freq.size(0) > D || (freq.size(0) > 1 && freq.stride(0) != 1))
+    return false;
+  c10::cuda::CUDAGuard guard(dev);
+  qo = at::empty({B, H, S, D}, q.options());
+  if (k) ko = at::empty({B, k->size(1), S, D}, k->options());
+  const Strides4 qs(q), qos(qo), ks(k ? *k : q), kos(k ? ko : qo);
+  const int64_t ps[2] = {row || pos.size(0) == 1 ? 0 : pos.stride(0), pos.stride(row ? 0 : 1)};
+  const int rc = g_rotary(
+      q.data_ptr(), qo.data_ptr(), qs.v, qos.v, static_cast<int>(H), k ? k->data_ptr() : nullptr,
+      k ? ko.data_ptr() : nullptr, k ? ks.v : nullptr, k ? kos.v : nullptr,
+      k ? static_cast<int>(k->size(1)) : 0, static_cast<int>(B), static_cast<int>(S),
+      static_cast<int>(D), static_cast<int>(2 * freq.size(0)), pos.data_ptr(), pt == at::kLong, ps,
+      freq.data_ptr<double>(), how.interleaved, how.inverse, static_cast<float>(how.magnitude),
+      dtype, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  if (rc != 0) return false;
+  ++g_launches;
+  return true;
+}
+
+// The differentiable form: a rotation's gradient is the rotation the other way, and so is the
+// gradient's.
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
+                                                const at::Tensor& q,
+                                                const std::optional<at::Tensor>& k,
+                                                const at::Tensor& pos, const at::Tensor& freq,
+                                                bool interleaved, double magnitude, bool inverse) {
+    at::Tensor qo, ko;
+    TORCH_CHECK(rotary_launch(q, k ? &*k : nullptr, pos, freq,
+                              {interleaved, magnitude, inverse}, qo, ko),
+                "rotary: ", g_last_error ? g_last_error() : "", " (launch)");
+    ctx->save_for_backward({pos, freq});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["magnitude"] = magnitude;
+    ctx->saved_data["inverse"] = inverse;
+    ctx->saved_data["has_k"] = k.has_value();
+    if (!k) return {qo};
+    return {qo, ko};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool();
+    const double magnitude = ctx->saved_data["magnitude"].toDouble();
+    const bool inverse = !ctx->saved_data["inverse"].toBool();
+    const bool has_k = ctx->saved_data["has_k"].toBool();
+    // A gradient that nobody needs, or that never came, costs nothing.
+    at::Tensor gq = ctx->needs_input_grad(0) ? grads[0] : at::Tensor();
+    at::Tensor gk = has_k && ctx->needs_input_grad(1) ? grads[1] : at::Tensor();
+    for (at::Tensor* g : {&gq, &gk})
+      if (g->defined() && g->stride(3) != 1) *g = g->contiguous();
+    const std::optional<at::Tensor> none, second = gk.defined() ? std::optional<at::Tensor>(gk) : none;
+    if (gq.defined()) {
+      auto out = apply(gq, second, saved[0], saved[1], interleaved, magnitude, inverse);
+      gq = out[0];
+      if (gk.defined()) gk = out[1];
+    } else if (gk.defined()) {
+      gk = apply(gk, none, saved[0], saved[1], interleaved, magnitude, inverse)[0];
+    }
+    return {gq, gk, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  if (nargs != 7 || g_rotary == nullptr) Py_RETURN_NONE;
+  if (nargs != 7) Py_RETURN_NONE;
   const at::Tensor* q = tensor_arg(args[0]);
   const bool has_k = args[1] != Py_None;
   const at::Tensor* k = has_k ? tensor_arg(args[1]) : nullptr;
@@ -243,63 +335,30 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const at::Tensor* freq = tensor_arg(args[3]);
   if (!q || (has_k && !k) || !pos || !freq) Py_RETURN_NONE;
   if (!PyBool_Check(args[4]) || !PyFloat_Check(args[5]) || !PyBool_Check(args[6])) Py_RETURN_NONE;
-  const double magnitude = PyFloat_AS_DOUBLE(args[5]);
+  const RotaryHow how{args[4] == Py_True, PyFloat_AS_DOUBLE(args[5]), args[6] == Py_True};
+  at::Tensor qo, ko;
   try {
-    if (q->dim() != 4 || !q->is_cuda() || !std::isfinite(magnitude)) Py_RETURN_NONE;
-    if (at::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad())))
+    if (at::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad()))) {
+      auto out = RotaryFunction::apply(*q, k ? std::optional<at::Tensor>(*k) : std::nullopt, *pos, *freq, how.interleaved,
+                                       how.magnitude, how.inverse);
+      qo = out[0];
+      if (k) ko = out[1];
+    } else if (!rotary_launch(*q, k, *pos, *freq, how, qo, ko)) {
       Py_RETURN_NONE;
-    const int dtype = dtype_code(*q);
-    const c10::Device dev = q->device();
-    const int64_t B = q->size(0), H = q->size(1), S = q->size(2), D = q->size(3);
-    if (dtype < 0 || !fits_int(B) || !fits_int(H) || !fits_int(S) || !fits_int(D) ||
-        q->stride(3) != 1)
-      Py_RETURN_NONE;
-    if (k && (k->dim() != 4 || k->device() != dev || dtype_code(*k) != dtype || k->size(0) != B ||
-              !fits_int(k->size(1)) || k->size(2) != S || k->size(3) != D || k->stride(3) != 1))
-      Py_RETURN_NONE;
-    const auto pt = pos->scalar_type();
-    if (pos->device() != dev || (pt != at::kInt && pt != at::kLong)) Py_RETURN_NONE;
-    const bool row = pos->dim() == 1;
-    if (!(row ? pos->size(0) == S
-              : pos->dim() == 2 && (pos->size(0) == B || pos->size(0) == 1) && pos->size(1) == S))
-      Py_RETURN_NONE;
-    if (freq->device() != dev || freq->scalar_type() != at::kDouble || freq->dim() != 1 ||
-        freq->size(0) < 1 || 2 * freq->size(0) > D || (freq->size(0) > 1 && freq->stride(0) != 1))
-      Py_RETURN_NONE;
-
-    c10::cuda::CUDAGuard guard(dev);
-    at::Tensor qo = at::empty({B, H, S, D}, q->options());
-    at::Tensor ko;
-    if (k) ko = at::empty({B, k->size(1), S, D}, k->options());
-    const Strides4 qs(*q), qos(qo), ks(k ? *k : *q), kos(k ? ko : qo);
-    const int64_t ps[2] = {row || pos->size(0) == 1 ? 0 : pos->stride(0),
-                           pos->stride(row ? 0 : 1)};
-    cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-    int rc;
-    Py_BEGIN_ALLOW_THREADS
-    rc = g_rotary(q->data_ptr(), qo.data_ptr(), qs.v, qos.v, static_cast<int>(H),
-                  k ? k->data_ptr() : nullptr, k ? ko.data_ptr() : nullptr, k ? ks.v : nullptr,
-                  k ? kos.v : nullptr, k ? static_cast<int>(k->size(1)) : 0, static_cast<int>(B),
-                  static_cast<int>(S), static_cast<int>(D), static_cast<int>(2 * freq->size(0)),
-                  pos->data_ptr(), pt == at::kLong, ps, freq->data_ptr<double>(),
-                  args[4] == Py_True, args[6] == Py_True, static_cast<float>(magnitude), dtype,
-                  stream);
-    Py_END_ALLOW_THREADS
-    if (rc != 0) Py_RETURN_NONE;
-    ++g_launches;
-    PyObject* out = PyTuple_New(2);
-    if (out == nullptr) return nullptr;
-    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(qo)));
-    if (k) {
-      PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(ko)));
-    } else {
-      Py_INCREF(Py_None);
-      PyTuple_SET_ITEM(out, 1, Py_None);
     }
-    return out;
   } catch (const std::exception&) {
     Py_RETURN_NONE;
   }
+  PyObject* out = PyTuple_New(2);
+  if (out == nullptr) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(qo)));
+  if (k) {
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(ko)));
+  } else {
+    Py_INCREF(Py_None);
+    PyTuple_SET_ITEM(out, 1, Py_None);
+  }
+  return out;
 }
 
 // The cache's four tensors (args) and the page table, where they are as the kernels take them.

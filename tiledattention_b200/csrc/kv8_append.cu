@@ -109,22 +109,15 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendParams p, int s
   const int64_t slot = start / p.page + blockIdx.x % slots;
   const SlotSpan span = slot_span(start, count, slot, p.page);
   if (span.row1 <= span.row0) return;
-  const int page = checked_page(p.table + b * p.table_stride, slot, p.width, p.num_pages);
-  if (page < 0) {
-    if (h == 0 && kind == 0 && threadIdx.x == 0 && p.status)
-      atomicOr(p.status, TA_DEVSTAT_BAD_PAGE);
-    return;
-  }
 
   const int vecs = p.D / 8;  // vectors per token
   const int n = (span.row1 - span.row0) * vecs;
   const uint16_t* x = static_cast<const uint16_t*>(p.x[kind]) + b * p.sb[kind] + h * p.sh[kind] +
                       span.t0 * p.ss[kind];
   const int64_t ss = p.ss[kind];
-  uint8_t* out = p.pages[kind] +
-                 ((static_cast<int64_t>(page) * p.Hkv + h) * p.page) * static_cast<int64_t>(p.D);
+  const int recip = ((1 << 20) + vecs - 1) / vecs;  // i / vecs, exact for i < 4096 = 128 * 32
   auto load = [&](int i) {
-    const int row = i / vecs;
+    const int row = (i * recip) >> 20;
     return *reinterpret_cast<const uint4*>(x + row * ss + (i - row * vecs) * 8);
   };
 
@@ -135,6 +128,17 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendParams p, int s
     const int i = threadIdx.x + k * 128;
     held[k] = i < n ? load(i) : make_uint4(0, 0, 0, 0);
   }
+  // The page's id and old scale while the values are on their way.
+  const int page = checked_page(p.table + b * p.table_stride, slot, p.width, p.num_pages);
+  if (page < 0) {
+    if (h == 0 && kind == 0 && threadIdx.x == 0 && p.status)
+      atomicOr(p.status, TA_DEVSTAT_BAD_PAGE);
+    return;
+  }
+  uint8_t* out = p.pages[kind] +
+                 ((static_cast<int64_t>(page) * p.Hkv + h) * p.page) * static_cast<int64_t>(p.D);
+  float* scale = p.scale[kind] + static_cast<int64_t>(page) * p.Hkv + h;
+  const int before = span.row0 > 0 ? stored_exponent(__float_as_uint(*scale)) : kScaleExpMin;
 #pragma unroll
   for (int k = 0; k < kHeld; ++k) m = max_magnitude(held[k], m);
   for (int i = threadIdx.x + kHeld * 128; i < n; i += 128) m = max_magnitude(load(i), m);
@@ -156,10 +160,7 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendParams p, int s
   }
 
   int e = scale_exponent(f32_bits<BF16>(m));
-  float* scale = p.scale[kind] + static_cast<int64_t>(page) * p.Hkv + h;
-  if (span.row0 > 0) {
-    const int before = stored_exponent(__float_as_uint(*scale));
-    __syncthreads();  // every thread has read the old scale before thread 0 replaces it
+  if (span.row0 > 0) {  // every thread has the old scale: a barrier lies between
     if (e > before) {
       const float mul = pow2f(before - e);
       uint4* old = reinterpret_cast<uint4*>(out);

@@ -72,68 +72,102 @@ __device__ __forceinline__ HeadAt head_at(const RotaryParams& p, int h, int b, i
           static_cast<uint16_t*>(t.y) + b * t.y_sb + hh * t.y_sh + s * t.y_ss};
 }
 
+// Token and slot of a thread: a block covers the whole tokens that fit its threads.
+struct Place {
+  int b, s, slot;
+  bool ok;
+};
+__device__ __forceinline__ Place place_of(const RotaryParams& p, int n_slots) {
+  const int per_block = max(1, kThreads / n_slots);
+  const int slots_here = min(n_slots, kThreads);  // n_slots > kThreads: only without vectors
+  const int local = threadIdx.x / slots_here;
+  const int64_t token = static_cast<int64_t>(blockIdx.x) * per_block + local;
+  const int64_t tokens = static_cast<int64_t>(p.B) * p.S;
+  Place at;
+  at.slot = threadIdx.x - local * slots_here;
+  at.ok = local < per_block && token < tokens;
+  if (tokens <= 0xffffffffll) {  // a 64-bit division costs as much as the rotation
+    at.b = static_cast<uint32_t>(token) / static_cast<uint32_t>(p.S);
+    at.s = static_cast<int>(static_cast<uint32_t>(token) - static_cast<uint32_t>(at.b) * p.S);
+  } else {
+    at.b = static_cast<int>(token / p.S);
+    at.s = static_cast<int>(token - static_cast<int64_t>(at.b) * p.S);
+  }
+  return at;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t turned(uint32_t a, uint32_t b, float c0, float c1, float s0,
+                                           float s1) {  // a cos + b sin of two lanes
+  const float2 x = unpack2<BF16>(a), y = unpack2<BF16>(b);
+  return pack2<BF16>(fmaf(x.x, c0, y.x * s0), fmaf(x.y, c1, y.y * s1));
+}
+
 // 16-byte path. A token's head has n_slots slots: with the half layout half/8 slots of 8 pairs
 // (two vectors each), interleaved half/4 slots of 4 pairs (one vector), then one slot for
 // each 8 copied dims. Thread = (token, slot), blockIdx.y = group of heads_per_thread heads;
-// consecutive threads cover consecutive bytes of one head's tokens.
+// consecutive threads cover consecutive bytes of one head's tokens. The loads of kAhead heads are
+// issued before their stores (which may be to the same memory, so the compiler cannot).
 template <bool BF16, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads)
     rotary_vector_kernel(const RotaryParams p, int n_slots, int heads_per_thread) {
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t token = id / n_slots;
-  const int slot = static_cast<int>(id - token * n_slots);
-  if (token >= static_cast<int64_t>(p.B) * p.S) return;
-  const int b = static_cast<int>(token / p.S);
-  const int s = static_cast<int>(token - static_cast<int64_t>(b) * p.S);
+  constexpr int kAhead = 4;
+  const Place at = place_of(p, n_slots);
+  if (!at.ok) return;
   const int heads = p.t[0].heads + p.t[1].heads;
   const int h0 = blockIdx.y * heads_per_thread;
   const int h1 = min(heads, h0 + heads_per_thread);
   constexpr int kPairs = INTERLEAVED ? 4 : 8;
   const int turning = p.half / kPairs;
-  if (slot >= turning) {
-    const int d = 2 * p.half + (slot - turning) * 8;
-    for (int h = h0; h < h1; ++h) {
-      const HeadAt at = head_at(p, h, b, s);
-      *reinterpret_cast<uint4*>(at.y + d) = *reinterpret_cast<const uint4*>(at.x + d);
+  const bool turns = at.slot < turning;
+  const int d = turns ? at.slot * 8 : 2 * p.half + (at.slot - turning) * 8;
+  uint4 va[kAhead], vb[kAhead];
+  uint16_t* y[kAhead];
+  auto load = [&](int h) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (h + k >= h1) break;
+      const HeadAt x = head_at(p, h + k, at.b, at.s);
+      y[k] = x.y + d;
+      va[k] = *reinterpret_cast<const uint4*>(x.x + d);
+      if (!INTERLEAVED && turns) vb[k] = *reinterpret_cast<const uint4*>(x.x + p.half + d);
     }
-    return;
-  }
+  };
+  load(h0);  // on their way while the angles are computed
   float c[kPairs], sn[kPairs];
-  const double position = position_of(p, b, s);
+  if (turns) {
+    const double position = position_of(p, at.b, at.s);
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) turn_of(p, position, slot * kPairs + i, c[i], sn[i]);
-  const int d = slot * 8;
-  if constexpr (INTERLEAVED) {
-#pragma unroll 4
-    for (int h = h0; h < h1; ++h) {
-      const HeadAt at = head_at(p, h, b, s);
-      const uint4 v = *reinterpret_cast<const uint4*>(at.x + d);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    for (int i = 0; i < kPairs; ++i) turn_of(p, position, at.slot * kPairs + i, c[i], sn[i]);
+  }
+  for (int h = h0; h < h1; h += kAhead) {
+    if (h > h0) load(h);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (h + k >= h1) break;
+      if (!turns) {
+        *reinterpret_cast<uint4*>(y[k]) = va[k];
+        continue;
+      }
+      const uint32_t a[4] = {va[k].x, va[k].y, va[k].z, va[k].w};
       uint32_t r[4];
+      if constexpr (INTERLEAVED) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 a = unpack2<BF16>(w[i]);
-        r[i] = pack2<BF16>(a.x * c[i] - a.y * sn[i], a.y * c[i] + a.x * sn[i]);
-      }
-      *reinterpret_cast<uint4*>(at.y + d) = make_uint4(r[0], r[1], r[2], r[3]);
-    }
-  } else {
-#pragma unroll 2
-    for (int h = h0; h < h1; ++h) {
-      const HeadAt at = head_at(p, h, b, s);
-      const uint4 va = *reinterpret_cast<const uint4*>(at.x + d);
-      const uint4 vb = *reinterpret_cast<const uint4*>(at.x + p.half + d);
-      const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
-      uint32_t ra[4], rb[4];
+        for (int i = 0; i < 4; ++i) {
+          const float2 v = unpack2<BF16>(a[i]);
+          r[i] = pack2<BF16>(fmaf(v.x, c[i], -v.y * sn[i]), fmaf(v.y, c[i], v.x * sn[i]));
+        }
+      } else {
+        const uint32_t b[4] = {vb[k].x, vb[k].y, vb[k].z, vb[k].w};
+        uint32_t q[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 a = unpack2<BF16>(wa[i]), e = unpack2<BF16>(wb[i]);
-        const float c0 = c[2 * i], c1 = c[2 * i + 1], s0 = sn[2 * i], s1 = sn[2 * i + 1];
-        ra[i] = pack2<BF16>(a.x * c0 - e.x * s0, a.y * c1 - e.y * s1);
-        rb[i] = pack2<BF16>(e.x * c0 + a.x * s0, e.y * c1 + a.y * s1);
+        for (int i = 0; i < 4; ++i) {
+          r[i] = turned<BF16>(a[i], b[i], c[2 * i], c[2 * i + 1], -sn[2 * i], -sn[2 * i + 1]);
+          q[i] = turned<BF16>(b[i], a[i], c[2 * i], c[2 * i + 1], sn[2 * i], sn[2 * i + 1]);
+        }
+        *reinterpret_cast<uint4*>(y[k] + p.half) = make_uint4(q[0], q[1], q[2], q[3]);
       }
-      *reinterpret_cast<uint4*>(at.y + d) = make_uint4(ra[0], ra[1], ra[2], ra[3]);
-      *reinterpret_cast<uint4*>(at.y + p.half + d) = make_uint4(rb[0], rb[1], rb[2], rb[3]);
+      *reinterpret_cast<uint4*>(y[k]) = make_uint4(r[0], r[1], r[2], r[3]);
     }
   }
 }
@@ -142,33 +176,32 @@ __global__ void __launch_bounds__(kThreads)
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads)
     rotary_scalar_kernel(const RotaryParams p, int n_slots, int heads_per_thread) {
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t token = id / n_slots;
-  const int slot = static_cast<int>(id - token * n_slots);
-  if (token >= static_cast<int64_t>(p.B) * p.S) return;
-  const int b = static_cast<int>(token / p.S);
-  const int s = static_cast<int>(token - static_cast<int64_t>(b) * p.S);
+  const Place at = place_of(p, n_slots);
+  if (!at.ok) return;
+  const int b = at.b, s = at.s;
   const int h0 = blockIdx.y * heads_per_thread;
   const int h1 = min(p.t[0].heads + p.t[1].heads, h0 + heads_per_thread);
-  if (slot >= p.half) {
-    const int d = p.half + slot;
-    for (int h = h0; h < h1; ++h) {
-      const HeadAt at = head_at(p, h, b, s);
-      at.y[d] = at.x[d];
+  for (int slot = at.slot; slot < n_slots; slot += kThreads) {
+    if (slot >= p.half) {
+      const int d = p.half + slot;
+      for (int h = h0; h < h1; ++h) {
+        const HeadAt x = head_at(p, h, b, s);
+        x.y[d] = x.x[d];
+      }
+      continue;
     }
-    return;
-  }
-  float c, sn;
-  turn_of(p, position_of(p, b, s), slot, c, sn);
-  const int da = p.interleaved ? 2 * slot : slot;
-  const int db = p.interleaved ? 2 * slot + 1 : p.half + slot;
-  for (int h = h0; h < h1; ++h) {
-    const HeadAt at = head_at(p, h, b, s);
-    const float2 v = unpack2<BF16>(static_cast<uint32_t>(at.x[da]) |
-                                   (static_cast<uint32_t>(at.x[db]) << 16));
-    const uint32_t r = pack2<BF16>(v.x * c - v.y * sn, v.y * c + v.x * sn);
-    at.y[da] = static_cast<uint16_t>(r);
-    at.y[db] = static_cast<uint16_t>(r >> 16);
+    float c, sn;
+    turn_of(p, position_of(p, b, s), slot, c, sn);
+    const int da = p.interleaved ? 2 * slot : slot;
+    const int db = p.interleaved ? 2 * slot + 1 : p.half + slot;
+    for (int h = h0; h < h1; ++h) {
+      const HeadAt x = head_at(p, h, b, s);
+      const float2 v = unpack2<BF16>(static_cast<uint32_t>(x.x[da]) |
+                                     (static_cast<uint32_t>(x.x[db]) << 16));
+      const uint32_t r = pack2<BF16>(fmaf(v.x, c, -v.y * sn), fmaf(v.y, c, v.x * sn));
+      x.y[da] = static_cast<uint16_t>(r);
+      x.y[db] = static_cast<uint16_t>(r >> 16);
+    }
   }
 }
 
@@ -178,14 +211,14 @@ cudaError_t launch_rotary(const RotaryParams& p, bool vector, int sm_count, cuda
   const int pairs = vector ? (p.interleaved ? 4 : 8) : 1;
   const int n_slots = p.half / pairs + (p.D - 2 * p.half) / (vector ? 8 : 1);
   const int heads = p.t[0].heads + p.t[1].heads;
-  const int64_t blocks =
-      (static_cast<int64_t>(p.B) * p.S * n_slots + kThreads - 1) / kThreads;
+  const int per_block = kThreads / n_slots > 1 ? kThreads / n_slots : 1;
+  const int64_t blocks = (static_cast<int64_t>(p.B) * p.S + per_block - 1) / per_block;
   if (blocks == 0 || heads == 0) return cudaSuccess;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-  // Heads per thread: as many as leave two full waves of resident threads (more heads spread
-  // the cost of cos and sin, fewer fill the GPU when tokens are few), 16 at most.
+  // Heads per thread: as many as leave a full wave of resident threads (more heads spread the
+  // cost of cos and sin, fewer fill the GPU when tokens are few), 16 at most.
   int hpt = 16;
-  const int64_t want = 2ll * sm_count * (2048 / kThreads);
+  const int64_t want = static_cast<int64_t>(sm_count) * (2048 / kThreads);
   while (hpt > 1 && blocks * ((heads + hpt - 1) / hpt) < want) hpt /= 2;
   while ((heads + hpt - 1) / hpt > 65535) hpt *= 2;
   const dim3 grid(static_cast<unsigned>(blocks), (heads + hpt - 1) / hpt);

@@ -142,24 +142,20 @@ def run_rotary(q, k, positions, inv_freq, interleaved, magnitude, inverse):
 
 
 def _fast_launch(q, k, positions, inv_freq, interleaved, magnitude, inverse):
-    """The one-call native launcher for the common case, or None (a gradient is wanted, an
-    argument is not as it should be, or the launcher is not there): see sdpa._fast_launch."""
+    """The one-call native launcher, which differentiates too, or None (an argument is not as it
+    should be, or the launcher is not there): see sdpa._fast_launch."""
     fast = _native._fast
     if fast is None or not _runtime._runtime_ready or not _async_mode():
         return None
     return fast.rotary(q, k, positions, inv_freq, interleaved, magnitude, inverse)
 
 
-def _launch(*args):
-    out = _fast_launch(*args)
-    return out if out is not None else run_rotary(*args)
-
-
 _function = None
 
 
 def _autograd_function():
-    """The autograd function (made once torch is there): the gradient turns the other way."""
+    """The autograd function of the Python path (made once torch is there): the gradient turns
+    the other way."""
     global _function
     if _function is not None:
         return _function
@@ -170,11 +166,10 @@ def _autograd_function():
         def forward(ctx, q, k, positions, inv_freq, interleaved, magnitude, inverse):
             ctx.save_for_backward(positions, inv_freq)
             ctx.how = (interleaved, magnitude, inverse)
-            out_q, out_k = _launch(q, k, positions, inv_freq, interleaved, magnitude, inverse)
+            out_q, out_k = run_rotary(q, k, positions, inv_freq, interleaved, magnitude, inverse)
             return out_q if k is None else (out_q, out_k)
 
         @staticmethod
-        @torch_mod.autograd.function.once_differentiable
         def backward(ctx, grad_q, grad_k=None):
             positions, inv_freq = ctx.saved_tensors
             interleaved, magnitude, inverse = ctx.how
@@ -182,10 +177,12 @@ def _autograd_function():
             # A gradient that nobody needs, or that never came, costs nothing.
             need_q = ctx.needs_input_grad[0] and grad_q is not None
             need_k = ctx.needs_input_grad[1] and grad_k is not None
-            if need_q:
-                grad_q, grad_k = _launch(grad_q, grad_k if need_k else None, *rest)
+            if need_q and need_k:
+                grad_q, grad_k = Rotary.apply(grad_q, grad_k, *rest)
+            elif need_q:
+                grad_q = Rotary.apply(grad_q, None, *rest)
             elif need_k:
-                grad_k = _launch(grad_k, None, *rest)[0]
+                grad_k = Rotary.apply(grad_k, None, *rest)
             return (grad_q if need_q else None, grad_k if need_k else None, *[None] * 5)
 
     _function = Rotary
@@ -206,7 +203,7 @@ def rotary(q, k, positions, inv_freq, *, interleaved: bool = False, magnitude: f
     inverse:     turn the other way (what the gradient does).
 
     Returns new contiguous tensors, computed asynchronously on the current torch stream;
-    differentiable (once) in q and k.
+    differentiable in q and k.
     """
     out = _fast_launch(q, k, positions, inv_freq, interleaved, magnitude, inverse)
     if out is not None:
@@ -223,5 +220,5 @@ def rotary(q, k, positions, inv_freq, *, interleaved: bool = False, magnitude: f
     if torch_mod.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         out = _autograd_function().apply(q, k, positions, inv_freq, interleaved, magnitude, inverse)
         return (out, None) if k is None else out
-    q_out, k_out = _launch(q, k, positions, inv_freq, interleaved, magnitude, inverse)
+    q_out, k_out = run_rotary(q, k, positions, inv_freq, interleaved, magnitude, inverse)
     return q_out, k_out
