@@ -105,6 +105,25 @@ int main() {
         }
     }
 
+  // tiles of a block of rows: the last key that any of its rows sees, against a walk over rows
+  for (int group : {1, 3, 4, 8})
+    for (int T : {1, 5, 64, 100})
+      for (int length : {0, 1, 60, 129, 1000})
+        for (int count : {0, 1, 3, 100})
+          for (int causal : {0, 1})
+            for (int n : {128, 256}) {
+              if (count > T) continue;
+              const SeqExtent e = checked_extent(length, count, T, 1 << 20);
+              for (int row0 = 0; row0 < group * T + n; row0 += n) {
+                int lim = 0;
+                for (int r = row0; r < row0 + n && r < group * T; ++r) {
+                  const int l = row_limit(e.length, e.count, r / group, causal);
+                  if (l > lim) lim = l;
+                }
+                CHECK(block_tiles(e, group, row0, n, T, causal, 128) == (lim + 127) / 128);
+              }
+            }
+
   // runs: they tile the line, none empty, and run_of finds the run of every tile
   for (int64_t total : {1, 2, 7, 295, 296, 297, 1000, 4096, 100003})
     for (int64_t grid : {1, 3, 148, 296}) {

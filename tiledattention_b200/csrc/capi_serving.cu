@@ -91,7 +91,21 @@ int make_pages_map(CUtensorMap* map, const void* pages, int D, int page, int64_t
                            : ta_capi_fail(TA_ERR_LAYOUT, "cuTensorMapEncodeTiled rejected the cache");
 }
 
+int64_t workspace_bytes_of(int B, int Hq, int Hkv, int T, int D, int sms) {
+  const int64_t rows = static_cast<int64_t>(Hq / Hkv) * T;
+  if (rows > (1 << 24)) return 0;
+  return static_cast<int64_t>(ta::kv8::uses_chunk(static_cast<int>(rows), D)
+                                  ? ta::kv8::chunk_workspace_bytes(D, sms)
+                                  : ta::kv8::attend_workspace_bytes(B, Hq, Hkv, T, D, sms));
+}
+
 }  // namespace
+
+namespace ta {
+namespace kv8 {
+bool uses_chunk(int rows, int) { return rows > 32; }
+}  // namespace kv8
+}  // namespace ta
 
 extern "C" {
 
@@ -199,7 +213,7 @@ int ta_kv8_append(const void* k, const void* v, const int64_t* k_strides, const 
 int64_t ta_sdpa_kv8_workspace(int B, int Hq, int Hkv, int T, int D) {
   ta_capi_clear_error();
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || D <= 0 || D > 256 || Hq % Hkv != 0) return 0;
-  return static_cast<int64_t>(ta::kv8::attend_workspace_bytes(B, Hq, Hkv, T, D, sm_count()));
+  return workspace_bytes_of(B, Hq, Hkv, T, D, sm_count());
 }
 
 int ta_sdpa_kv8(const void* q, const int64_t* q_strides, void* o, const int64_t* o_strides,
@@ -229,7 +243,7 @@ int ta_sdpa_kv8(const void* q, const int64_t* q_strides, void* o, const int64_t*
   if ((rc = ta_capi_check_device())) return rc;
   const int sms = sm_count();
   if (!aligned(workspace, 16) ||
-      workspace_bytes < static_cast<int64_t>(ta::kv8::attend_workspace_bytes(B, Hq, Hkv, T, D, sms)))
+      workspace_bytes < workspace_bytes_of(B, Hq, Hkv, T, D, sms))
     return ta_capi_fail(TA_ERR_INVALID_ARGUMENT, "workspace too small or not 16-byte aligned");
   ta::kv8::AttendParams p{};
   p.q = q;
@@ -264,6 +278,9 @@ int ta_sdpa_kv8(const void* q, const int64_t* q_strides, void* o, const int64_t*
   p.causal = causal != 0;
   p.group = Hq / Hkv;
   p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+  if (ta::kv8::uses_chunk(p.group * T, D))
+    return launched(ta::kv8::launch_chunk(p, sms, static_cast<cudaStream_t>(stream)),
+                    "cache attention launch failed");
   CUtensorMap map_k, map_v;
   const int box = page < ta::kv8::kKeysPerStep ? page : ta::kv8::kKeysPerStep;
   const int64_t planes = static_cast<int64_t>(num_pages) * Hkv;

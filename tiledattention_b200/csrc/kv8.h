@@ -70,6 +70,12 @@ struct AppendParams {
 
 cudaError_t launch_append(const AppendParams& p, cudaStream_t stream);
 
+// Where the chunk kernel's runs cut a block of rows: the block, and the first of the runs that
+// share it (-1: nothing to merge).
+struct Cut {
+  int b, h, rb, first;
+};
+
 struct AttendParams {
   const void* q;                  // [B, Hq, T, D], 16-bit
   int64_t q_sb, q_sh, q_ss;
@@ -85,6 +91,7 @@ struct AttendParams {
   unsigned int* status;
   float* part_o;                  // partial outputs, maxima and sums (see sdpa_kv8.cu)
   float* part_ml;
+  Cut* cuts;
   int B, Hq, Hkv, T, D, page, page_shift, width, num_pages, bf16, causal;
   int group;                      // Hq / Hkv
   int row_blocks;                 // blocks of rows (token, head of the group) per kv head
@@ -111,6 +118,18 @@ __host__ __device__ __forceinline__ SeqExtent checked_extent(int length, int cou
   if (e.count < 0) e.count = 0, e.bad = true;
   if (e.count > T) e.count = T, e.bad = true;
   return e;
+}
+
+// Key tiles of rows [row0, row0 + n) of a sequence's T * group rows (token, head of the group):
+// up to the last key that any of them sees.
+__host__ __device__ __forceinline__ int block_tiles(const SeqExtent& e, int group, int row0, int n,
+                                                    int T, int causal, int tile) {
+  const int end = row0 + n < group * T ? row0 + n : group * T;
+  if (row0 >= end) return 0;
+  const int first = row0 / group, last = (end - 1) / group;
+  if (first >= e.count) return 0;
+  const int lim = row_limit(e.length, e.count, last < e.count ? last : e.count - 1, causal);
+  return (lim + tile - 1) / tile;
 }
 
 // Work of the split kernel is a line of `total` tiles (sequence, then head and row block, then
@@ -153,6 +172,13 @@ size_t attend_workspace_bytes(int B, int Hq, int Hkv, int T, int D, int sm_count
 // swizzle) or 128 columns (128-byte swizzle) x min(page, kKeysPerStep) rows.
 cudaError_t launch_attend(const AttendParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v,
                           int sm_count, cudaStream_t stream);
+
+// The kernel for many rows (sdpa_kv8_chunk.cu) and its workspace.
+size_t chunk_workspace_bytes(int D, int sm_count);
+cudaError_t launch_chunk(const AttendParams& p, int sm_count, cudaStream_t stream);
+
+// Which kernel serves `rows` query rows per cache head: see capi_serving.cu.
+bool uses_chunk(int rows, int D);
 
 }  // namespace kv8
 }  // namespace ta

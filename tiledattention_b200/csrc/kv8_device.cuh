@@ -1,0 +1,93 @@
+// What the kernels that attend over the 8-bit cache share on the device (sdpa_kv8.cu for few query
+// rows, sdpa_kv8_chunk.cu for many): 16-bit values, a batch's line of work.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "kv8.h"
+#include "sm100_ptx.cuh"
+#include "tiledattention_b200.h"
+
+namespace ta {
+namespace kv8 {
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 unpack16(uint32_t w, bool bf16) {
+  if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
+  uint32_t r;
+  if (bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float pow2f(int e) {
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+// Natural-log log-sum-exp of a row from its maximum (log2) and sum; -inf without a key.
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l == 0.f ? -INFINITY : (fmaxf(m, -3.4e38f) + log2f(l)) * 0.69314718055994531f;
+}
+
+__device__ __forceinline__ SeqExtent extent_of(const AttendParams& p, int b) {
+  return checked_extent(p.lengths[b], p.counts ? p.counts[b] : p.T, p.T,
+                        static_cast<int64_t>(p.width) * p.page);
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)),
+      "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+// A batch-wide exclusive sum by one block of WARPS warps. `work(b, extent)`: the work of sequence b. Every
+// thread gets the total and the work before its own share [b0, b1) of the batch; `report`:
+// record lengths and counts out of range.
+struct Scan {
+  int64_t total, mine;
+  int b0, b1;
+};
+template <int WARPS, class F>
+__device__ __forceinline__ Scan scan_batch(const AttendParams& p, int64_t* s_warp, bool report, F work) {
+  Scan r;
+  const int share = (p.B + WARPS * 32 - 1) / (WARPS * 32);
+  r.b0 = min(p.B, static_cast<int>(threadIdx.x) * share);
+  r.b1 = min(p.B, r.b0 + share);
+  int64_t sum = 0;
+  for (int b = r.b0; b < r.b1; ++b) {
+    const SeqExtent e = extent_of(p, b);
+    if (e.bad && report && p.status) atomicOr(p.status, TA_DEVSTAT_BAD_LENGTH);
+    sum += work(e);
+  }
+  int64_t incl = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, incl, d);
+    if ((threadIdx.x & 31) >= d) incl += up;
+  }
+  if ((threadIdx.x & 31) == 31) s_warp[threadIdx.x >> 5] = incl;
+  __syncthreads();
+  int64_t before = 0;
+  r.total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < static_cast<int>(threadIdx.x >> 5)) before += s_warp[w];
+    r.total += s_warp[w];
+  }
+  r.mine = before + incl - sum;
+  return r;
+}
+
+}  // namespace kv8
+}  // namespace ta

@@ -34,14 +34,9 @@
 // reference of a row's weights moves (and is agreed on between lanes) only when a score passes it
 // by 2^15.
 #include <cuda.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
-#include <math.h>
-#include <stdint.h>
 
-#include "kv8.h"
-#include "sm100_ptx.cuh"
-#include "tiledattention_b200.h"
+#include "kv8_device.cuh"
 
 namespace ta {
 namespace kv8 {
@@ -94,15 +89,6 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar,
-                                            int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)),
-      "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
-
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -167,69 +153,8 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float2 unpack16(uint32_t w, bool bf16) {
-  if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  return __half22float2(*reinterpret_cast<__half2*>(&w));
-}
-__device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
-  uint32_t r;
-  if (bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float pow2f(int e) {
-  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
-}
-
-// Natural-log log-sum-exp of a row from its maximum (log2) and sum; -inf without a key.
-__device__ __forceinline__ float lse_of(float m, float l) {
-  return l == 0.f ? -INFINITY : (fmaxf(m, -3.4e38f) + log2f(l)) * 0.69314718055994531f;
-}
-
-__device__ __forceinline__ SeqExtent extent_of(const AttendParams& p, int b) {
-  return checked_extent(p.lengths[b], p.counts ? p.counts[b] : p.T, p.T,
-                        static_cast<int64_t>(p.width) * p.page);
-}
 __device__ __forceinline__ int tiles_of(const SeqExtent& e, int tile) {
   return e.count > 0 ? (e.length + tile - 1) / tile : 0;
-}
-
-// Tiles of the whole batch, and those before this thread's share [b0, b1) of it. Called by
-// all threads of a block; `report`: record lengths and counts out of range.
-struct Scan {
-  int64_t total, mine;
-};
-__device__ __forceinline__ Scan scan_batch(const AttendParams& p, int tile, int64_t per_tile,
-                                           int64_t* s_warp, bool report, int& b0, int& b1) {
-  const int share = (p.B + blockDim.x - 1) / blockDim.x;
-  b0 = min(p.B, static_cast<int>(threadIdx.x) * share);
-  b1 = min(p.B, b0 + share);
-  int64_t sum = 0;
-  for (int b = b0; b < b1; ++b) {
-    const SeqExtent e = extent_of(p, b);
-    if (e.bad && report && p.status) atomicOr(p.status, TA_DEVSTAT_BAD_LENGTH);
-    sum += static_cast<int64_t>(tiles_of(e, tile)) * per_tile;
-  }
-  int64_t incl = sum;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, incl, d);
-    if ((threadIdx.x & 31) >= d) incl += up;
-  }
-  if ((threadIdx.x & 31) == 31) s_warp[threadIdx.x >> 5] = incl;
-  __syncthreads();
-  int64_t before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < static_cast<int>(threadIdx.x >> 5)) before += s_warp[w];
-    total += s_warp[w];
-  }
-  return {total, before + incl - sum};
 }
 
 // A place on the line of tiles.
@@ -262,8 +187,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
 
   // This block's run of the line, and the sequence it begins in.
   const int hrs = p.Hkv * p.row_blocks;
-  int b0, b1;
-  const Scan sc = scan_batch(p, C::kTile, hrs, s_scan, blockIdx.x == 0, b0, b1);
+  const Scan sc = scan_batch<kWarps>(p, s_scan, blockIdx.x == 0, [&](const SeqExtent& e) {
+    return static_cast<int64_t>(tiles_of(e, C::kTile)) * hrs;
+  });
   const int64_t total = sc.total;
   const int64_t parts = min(static_cast<int64_t>(gridDim.x), total);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -272,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
   const int steps = static_cast<int>(run_begin(blockIdx.x + 1, total, parts) - w0);
   {
     int64_t at = sc.mine;
-    for (int b = b0; b < b1; ++b) {
+    for (int b = sc.b0; b < sc.b1; ++b) {
       const int64_t n = static_cast<int64_t>(tiles_of(extent_of(p, b), C::kTile)) * hrs;
       if (at <= w0 && w0 < at + n) {
         s_start[0] = b;
@@ -805,11 +731,12 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const AttendParams p, i
   const int h = (blockIdx.x / row_groups) % p.Hkv;
   const int b = blockIdx.x / row_groups / p.Hkv;
   const int hrs = p.Hkv * p.row_blocks;
-  int b0, b1;
-  const Scan sc = scan_batch(p, C::kTile, hrs, s_scan, false, b0, b1);
+  const Scan sc = scan_batch<kWarps>(p, s_scan, false, [&](const SeqExtent& e) {
+    return static_cast<int64_t>(tiles_of(e, C::kTile)) * hrs;
+  });
   {
     int64_t at = sc.mine;
-    for (int i = b0; i < b1; ++i) {
+    for (int i = sc.b0; i < sc.b1; ++i) {
       const int n = tiles_of(extent_of(p, i), C::kTile);
       if (i == b) {
         s_at = at;

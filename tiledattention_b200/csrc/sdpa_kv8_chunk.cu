@@ -1,0 +1,870 @@
+// Attention of many query rows over the paged 8-bit cache (a prompt's chunk against the context
+// before it): the maths of sdpa_kv8.cu on tcgen05 with accumulators in tensor memory.
+//
+//   t_j = log2(e) scale (q . k_j) 2^ek_j + ev_j,  o = sum_j 2^(t_j - r) v_j / sum_j 2^(t_j - r - ev_j)
+//
+// Tensor-bound: 4 D operations a row and key, 2 D bytes a key for all rows. One CTA an SM
+// covers two 128-row tiles (one at head dim 256, whose output takes half the tensor memory) that
+// share every 128-key tile; rows are (token, head of the group), so all heads of a group share
+// the keys too. Roles:
+//   warps 0-3, 4-7  softmax and epilogue of row tile 0, 1 (thread = row); they also bring the
+//                   rows of q into shared memory as fp16 times a power of two
+//   warps 8-11      converters: codes from the pages straight into registers (the next unit's
+//                   while this one is converted), fp16 (exact) into the 128-byte-swizzled tiles
+//                   that tcgen05 reads, a unit being one tile's K or V
+//   warp 12         tensor memory and MMA issue (kind::f16, fp16 operands)
+//   warps 13-15     zero the rows of blocks without keys
+// Converting once in shared memory costs 2 D x 128 conversions a tile for 256 rows; fp8
+// MMAs would take e4m3 as it is, but then the weights have to be cut into several fp8 parts,
+// which costs the softmax warps, the tightest role, about three operations more an element.
+// The scales of a page cost nothing an element: softmax's multiply-add takes them 16 keys
+// at a time.
+//
+// Work is a line of key tiles over (sequence, head, block of rows), cut into equal runs, one a
+// CTA: causal blocks of different length and uneven sequences fill the GPU evenly. A block that is
+// cut leaves partial results, merged by a second kernel that starts before this one ends.
+//
+// Every wait is bounded: on expiry the kernel records TA_DEVSTAT_* bits, drains its MMAs, frees
+// tensor memory and returns.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "kv8_device.cuh"
+
+namespace ta {
+namespace kv8 {
+namespace chunk {
+namespace {
+
+constexpr int kTileRows = 128, kTileKeys = 128;
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+// Register split of the launch's 512 x 128 registers: softmax, converters, MMA and idle.
+constexpr int kLaunchRegs = 128;
+constexpr int kSoftmaxRegs = 192, kConvertRegs = 80, kSideRegs = 48;
+static_assert(128 * (2 * kSoftmaxRegs + kConvertRegs + kSideRegs) == kThreads * kLaunchRegs,
+              "register split must match the launch allocation");
+constexpr uint32_t kTmemCols = 512;
+constexpr float kBelow = 7.f, kGrowth = 15.f;  // see sdpa_kv8.cu
+constexpr uint64_t kTimeoutNs = 1000000000ull;  // 1 s per wait
+constexpr int kMeta = 8;                       // tiles whose pages and scales are kept
+constexpr int kGroups = kTileKeys / 16;        // blocks of 16 keys: one page each
+constexpr int kNan = 8;                        // segments whose NaN values are kept (see Segment)
+
+template <int D>
+struct Cfg {
+  static constexpr int kTiles = D == 256 ? 1 : 2;
+  static constexpr int kRows = kTiles * kTileRows;
+  static constexpr int kTileBytes = kTileRows * D * 2;  // a q tile, or a K or V unit
+  static constexpr int kStages = D == 64 ? 6 : D == 128 ? 4 : 2;
+  static constexpr int kChunks = D / 16;                // 16-code chunks of a key
+  static constexpr int kQOff = 0;
+  static constexpr int kKvOff = kTiles * kTileBytes;
+  static constexpr int kMetaOff = kKvOff + kStages * kTileBytes;
+  static constexpr int kNanOff = kMetaOff + kMeta * kGroups * 16;
+  static constexpr int kBarOff = kNanOff + kNan * D * 4;
+  static constexpr int kBytes = kBarOff + 512 + 1024;  // slack: 1024-byte alignment
+};
+
+struct Meta {  // of 16 keys: where they are, and their scales in softmax's terms
+  int plane;   // page * Hkv + head, or -1: no key here, or a page outside the cache
+  float ks;    // scale of K
+  float e;     // exponent of V's scale; -inf where plane is -1: such keys have no weight
+  float back;  // 2^-e
+};
+
+struct Barriers {
+  uint64_t q_full[2], s_full[2], p_full[2], o_final[2];
+  uint64_t drain;
+  uint64_t kv_full[6], kv_empty[6], meta_full[kMeta];
+  int any_nan[kNan];
+  int64_t scan[kWarps];
+  int start_b;
+  int64_t start_w;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(Barriers) <= 512, "barrier block");
+
+// A block of rows on the line and the part of it that this run has. Where some of its rows do not
+// see a key, that key's value must not reach them as 0 * NaN: the converters write such NaNs as
+// zeros and note, for each dim, the first key that has one, and the epilogue gives the NaN to the
+// rows that see it. Notes are kept for kNan segments: the converters are at most three tiles ahead.
+struct Segment {
+  int b, h, rb, t0, n, tiles;  // key tiles [t0, t0 + n) of `tiles`
+};
+
+template <int D>
+struct Walk {
+  const AttendParams& p;
+  int64_t at, end;
+  Segment s;
+  SeqExtent e;
+  __device__ Walk(const AttendParams& pp, int64_t w0, int64_t w1, int b, int64_t before)
+      : p(pp), at(w0), end(w1) {
+    s.b = b;
+    e = extent_of(p, b);
+    int64_t rem = w0 - before;
+    const int64_t head = head_tiles();
+    s.h = static_cast<int>(rem / head);
+    rem -= s.h * head;
+    s.rb = 0;
+    s.tiles = block();
+    while (rem >= s.tiles) {
+      rem -= s.tiles;
+      ++s.rb;
+      s.tiles = block();
+    }
+    s.t0 = static_cast<int>(rem);
+    s.n = static_cast<int>(min(end - at, static_cast<int64_t>(s.tiles - s.t0)));
+  }
+  __device__ int block() const { return block_tiles(e, p.group, s.rb * Cfg<D>::kRows, Cfg<D>::kRows, p.T, p.causal, kTileKeys); }
+  __device__ int64_t head_tiles() const {
+    int64_t n = 0;
+    for (int rb = 0; rb < p.row_blocks; ++rb)
+      n += block_tiles(e, p.group, rb * Cfg<D>::kRows, Cfg<D>::kRows, p.T, p.causal, kTileKeys);
+    return n;
+  }
+  __device__ bool valid() const { return at < end; }
+  __device__ void next() {
+    at += s.n;
+    if (at >= end) return;
+    do {  // the next block with any tiles; there is one, since the run goes on
+      if (++s.rb == p.row_blocks) {
+        s.rb = 0;
+        if (++s.h == p.Hkv) {
+          s.h = 0;
+          if (++s.b >= p.B) {
+            at = end;
+            return;
+          }
+          e = extent_of(p, s.b);
+        }
+      }
+      s.tiles = block();
+    } while (s.tiles == 0);
+    s.t0 = 0;
+    s.n = static_cast<int>(min(end - at, static_cast<int64_t>(s.tiles)));
+  }
+  // Whether the second row tile has any rows.
+  __device__ bool two() const {
+    return Cfg<D>::kTiles == 2 && p.group * p.T - s.rb * Cfg<D>::kRows > kTileRows;
+  }
+};
+
+__device__ __forceinline__ void report(const AttendParams& p, uint32_t code, volatile int* abort_flag) {
+  *abort_flag = 1;
+  if (p.status) atomicOr(p.status, code);
+}
+
+// Whether all 128 converters say so; a barrier among them.
+__device__ __forceinline__ bool converters_agree(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r) : "r"(ok ? 1u : 0u) : "memory");
+  return r != 0;
+}
+
+__device__ __forceinline__ void sts128(void* a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  *reinterpret_cast<uint4*>(a) = make_uint4(x, y, z, w);
+}
+
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ uint32_t nan_bits(uint32_t w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p) {
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* q_smem = smem + C::kQOff;
+  uint8_t* kv_smem = smem + C::kKvOff;
+  Meta* meta = reinterpret_cast<Meta*>(smem + C::kMetaOff);
+  int* nan_key = reinterpret_cast<int*>(smem + C::kNanOff);  // [kNan][D]
+  Barriers* bars = reinterpret_cast<Barriers*>(smem + C::kBarOff);
+  volatile int* abort_flag = &bars->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&bars->q_full[t], kTileRows);
+      mbar_init(&bars->s_full[t], 1);
+      mbar_init(&bars->p_full[t], kTileRows);
+      mbar_init(&bars->o_final[t], 1);
+    }
+    mbar_init(&bars->drain, 1);
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&bars->kv_full[s], 128);
+      mbar_init(&bars->kv_empty[s], 1);
+    }
+    for (int i = 0; i < kMeta; ++i) mbar_init(&bars->meta_full[i], kGroups);
+    bars->abort_flag = 0;
+    p.cuts[blockIdx.x] = Cut{0, 0, 0, -1};  // until this thread knows better
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(&bars->tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  const auto per_seq = [&](const SeqExtent& e) {
+    int64_t n = 0;
+    for (int rb = 0; rb < p.row_blocks; ++rb)
+      n += block_tiles(e, p.group, rb * C::kRows, C::kRows, p.T, p.causal, kTileKeys);
+    return n * p.Hkv;
+  };
+  const Scan sc = scan_batch<kWarps>(p, bars->scan, blockIdx.x == 0, per_seq);  // has a barrier
+  tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = bars->tmem_base;
+  const int64_t parts = min(static_cast<int64_t>(gridDim.x), sc.total);
+  const bool has_run = blockIdx.x < parts;
+  const int64_t w0 = has_run ? run_begin(blockIdx.x, sc.total, parts) : 0;
+  const int64_t w1 = has_run ? run_begin(blockIdx.x + 1, sc.total, parts) : 0;
+  if (has_run) {
+    int64_t at = sc.mine;
+    for (int b = sc.b0; b < sc.b1; ++b) {
+      const int64_t n = per_seq(extent_of(p, b));
+      if (at <= w0 && w0 < at + n) {
+        bars->start_b = b;
+        bars->start_w = at;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  const int start_b = bars->start_b;
+  const int64_t start_w = bars->start_w;
+
+  if (warp >= 12) {
+    regs_dec<kSideRegs>();
+    if (warp == 12) {
+      // ------------------------------------------------------------ MMA issuer
+      if (lane == 0 && has_run) {
+        constexpr uint32_t kIdescQK = idesc_f16(kTileRows, kTileKeys, false, false, false);
+        constexpr uint32_t kIdescPV = idesc_f16(kTileRows, D, false, false, true);
+        const uint64_t q_desc = sdesc_sw128(smem_u32(q_smem), 16, 1024);
+        const uint64_t kv_desc_k = sdesc_sw128(smem_u32(kv_smem), 16, 1024);
+        const uint64_t kv_desc_v = sdesc_sw128(smem_u32(kv_smem), kTileKeys * 128, 1024);
+        auto issue_qk = [&](int t, int st) {
+          const uint64_t qd = q_desc + static_cast<uint64_t>((t * C::kTileBytes) >> 4);
+          const uint64_t kd = kv_desc_k + static_cast<uint64_t>((st * C::kTileBytes) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t off =
+                static_cast<uint64_t>(((kk >> 2) * (kTileRows * 128) + (kk & 3) * 32) >> 4);
+            mma_ss(tmem + t * 128, qd + off, kd + off, kIdescQK, kk > 0 ? 1u : 0u);
+          }
+          mma_commit(&bars->s_full[t]);
+        };
+        auto issue_pv = [&](int t, int st, bool acc) {
+          const uint64_t vd = kv_desc_v + static_cast<uint64_t>((st * C::kTileBytes) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kTileKeys / 16; ++kk)
+            mma_ts(tmem + 256 + t * D, tmem + t * 128 + kk * 8,
+                   vd + static_cast<uint64_t>((kk * 16 * 128) >> 4), kIdescPV,
+                   (acc || kk > 0) ? 1u : 0u);
+        };
+        int it = 0;                // units taken
+        int seen[2] = {0, 0};      // tiles of each row tile
+        int segs[2] = {0, 0};
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, int phase) {
+          ok = ok && mbar_wait_bounded(bar, phase & 1, abort_flag, kTimeoutNs);
+          return ok;
+        };
+        auto wait_unit = [&](int unit) {
+          return wait(&bars->kv_full[unit % C::kStages], unit / C::kStages);
+        };
+        for (Walk<D> w(p, w0, w1, start_b, start_w); ok && w.valid(); w.next()) {
+          const int nt = w.two() ? 2 : 1;
+          const int n = w.s.n;
+          for (int t = 0; t < nt; ++t) wait(&bars->q_full[t], segs[t]++);
+          if (!wait_unit(it)) break;
+          tc_fence_after();
+          for (int t = 0; t < nt; ++t) issue_qk(t, it % C::kStages);
+          mma_commit(&bars->kv_empty[it % C::kStages]);
+          ++it;
+          for (int j = 0; j < n; ++j) {
+            if (!wait_unit(it)) break;
+            const int st_v = it++ % C::kStages;
+            const bool more = j + 1 < n;
+            const int unit_k = it;
+            for (int t = 0; t < nt; ++t) {
+              if (!wait(&bars->p_full[t], seen[t]++)) break;
+              tc_fence_after();
+              issue_pv(t, st_v, j > 0);
+              if (t == nt - 1) mma_commit(&bars->kv_empty[st_v]);
+              if (more) {
+                if (t == 0 && !wait_unit(unit_k)) break;
+                tc_fence_after();
+                issue_qk(t, unit_k % C::kStages);
+                if (t == nt - 1) mma_commit(&bars->kv_empty[unit_k % C::kStages]);
+              } else {
+                mma_commit(&bars->o_final[t]);
+              }
+            }
+            if (!ok) break;
+            if (more) ++it;
+          }
+        }
+        if (!ok && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_MMA, abort_flag);
+        // All MMAs this thread issued complete before tensor memory is freed.
+        mma_commit(&bars->drain);
+        volatile int no_abort = 0;
+        if (!mbar_wait_bounded(&bars->drain, 0, &no_abort, kTimeoutNs) && p.status)
+          atomicOr(p.status, TA_DEVSTAT_TIMEOUT_DRAIN);
+      }
+      __syncwarp();
+    } else {
+      // ------------------------------------------------------------ rows of blocks without keys
+      const int rows = p.group * p.T;
+      const int64_t blocks = static_cast<int64_t>(p.B) * p.Hkv * p.row_blocks;
+      for (int64_t i = blockIdx.x; i < blocks; i += gridDim.x) {
+        const int rb = static_cast<int>(i % p.row_blocks);
+        const int h = static_cast<int>(i / p.row_blocks % p.Hkv);
+        const int b = static_cast<int>(i / p.row_blocks / p.Hkv);
+        if (block_tiles(extent_of(p, b), p.group, rb * C::kRows, C::kRows, p.T, p.causal, kTileKeys))
+          continue;
+        const int r1 = min(rows, (rb + 1) * C::kRows);
+        for (int r = rb * C::kRows + warp - 13; r < r1; r += 3) {
+          const int tok = r / p.group, hd = h * p.group + (r - tok * p.group);
+          uint16_t* out = static_cast<uint16_t*>(p.o) + b * p.o_sb + hd * p.o_sh + tok * p.o_ss;
+          for (int d = lane * 8; d < p.D; d += 256) sts128(out + d, 0, 0, 0, 0);
+          if (p.lse && lane == 0)
+            p.lse[(static_cast<int64_t>(b) * p.Hq + hd) * p.T + tok] = -INFINITY;
+        }
+      }
+    }
+  } else if (warp >= 8) {
+    // ------------------------------------------------------------ converters
+    regs_dec<kConvertRegs>();
+    if (has_run) {
+      constexpr int kRowsPerPass = 128 / C::kChunks;  // of 128 threads, 16 codes each
+      constexpr int kHeld = C::kChunks < 8 ? C::kChunks : 8;  // passes in flight
+      const int tid = threadIdx.x - 256;
+      // Lanes: 4 chunks of one 128-byte row of the tile and the next key's, so that 8
+      // lanes' 16-byte stores meet 8 different banks.
+      const int c = (lane & 3) | (C::kChunks == 4 ? 0 : (lane >> 3 & (C::kChunks / 4 - 1)) << 2);
+      const int row_in_warp = C::kChunks == 4 ? lane >> 2
+                              : C::kChunks == 8 ? ((lane >> 2) & 1) | (lane >> 4 << 1)
+                                                : (lane >> 2) & 1;
+      const int row0 = (warp - 8) * (kRowsPerPass / 4) + row_in_warp;
+      const bool real = c * 16 < p.D;
+      uint8_t* const store = kv_smem + (c >> 2) * (kTileKeys * 128);  // 64 dims: 128 bytes a key
+      bool ok = true;
+      int it = 0, tile_no = 0, seg = 0;
+
+      // Pages and scales are published a tile ahead by lanes 0-7 of the first warp, one a
+      // block of 16 keys. `ahead` walks in front of `w`.
+      Walk<D> w(p, w0, w1, start_b, start_w), ahead(p, w0, w1, start_b, start_w);
+      int ahead_tile = 0, published = 0;
+      auto publish = [&]() {
+        if (!ahead.valid()) return;
+        if (tid < kGroups) {
+          const int key = (ahead.s.t0 + ahead_tile) * kTileKeys + tid * 16;
+          Meta m{-1, 1.f, -INFINITY, 0.f};
+          if (key < ahead.e.length) {
+            const int id = p.table[ahead.s.b * p.table_stride + (key >> p.page_shift)];
+            if (static_cast<unsigned>(id) < static_cast<unsigned>(p.num_pages)) {
+              m.plane = id * p.Hkv + ahead.s.h;
+              m.ks = p.scale[0][m.plane];
+              const int ev = stored_exponent(__float_as_uint(p.scale[1][m.plane]));
+              m.e = static_cast<float>(ev);
+              m.back = pow2f(-ev);
+            } else if (p.status) {
+              atomicOr(p.status, TA_DEVSTAT_BAD_PAGE);
+            }
+          }
+          meta[(published % kMeta) * kGroups + tid] = m;
+          mbar_arrive(&bars->meta_full[published % kMeta]);
+        }
+        ++published;
+        if (++ahead_tile == ahead.s.n) {
+          ahead_tile = 0;
+          ahead.next();
+        }
+      };
+      publish();
+      converters_agree(true);
+
+      uint4 held[kHeld];
+      // Codes of pass i of a unit: kind 0 K, 1 V, of the tile in meta slot `slot` whose first key is
+      // key0, of a sequence of `length` keys. Rows without a key read as zeros.
+      auto fetch = [&](int i, int kind, int slot, int key0, int length) {
+        const int row = i * kRowsPerPass + row0;
+        const int plane = meta[slot * kGroups + (row >> 4)].plane;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (real && plane >= 0 && key0 + row < length)
+          v = __ldg(reinterpret_cast<const uint4*>(
+              p.pages[kind] +
+              (static_cast<int64_t>(plane) * p.page + ((key0 + row) & (p.page - 1))) * p.D + c * 16));
+        return v;
+      };
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        held[i] = fetch(i, 0, 0, w.s.t0 * kTileKeys, w.e.length);
+      while (ok && w.valid()) {
+        const Segment s = w.s;
+        const SeqExtent e = w.e;
+        // Keys that every row of the block with any keys sees: tiles beyond need care with NaN.
+        const int rows = min(p.group * p.T, (s.rb + 1) * C::kRows);
+        int safe = e.length;
+        if (p.causal) {
+          const int first = s.rb * C::kRows / p.group;
+          for (int tok = first; tok <= (rows - 1) / p.group; ++tok) {
+            const int lim = row_limit(e.length, e.count, tok, 1);
+            if (lim > 0) {
+              safe = lim;
+              break;
+            }
+          }
+        }
+        w.next();
+        int* const nan_here = nan_key + (seg % kNan) * D;
+        int* const any_nan = &bars->any_nan[seg % kNan];
+        ++seg;
+        for (int d = tid; d < D; d += 128) nan_here[d] = 0x7fffffff;
+        if (tid == 0) *any_nan = 0;  // the barrier before the first unit lies between
+        for (int j = 0; ok && j < s.n; ++j, ++tile_no) {
+          publish();  // the tile after this one
+          const int key0 = (s.t0 + j) * kTileKeys;
+          const bool edge = key0 + kTileKeys > safe;
+          const bool last_tile = j + 1 == s.n;
+          const int slot = tile_no % kMeta, next_slot = (tile_no + 1) % kMeta;
+          const int next_key0 = last_tile ? w.s.t0 * kTileKeys : key0 + kTileKeys;
+          const int next_length = last_tile ? (w.valid() ? w.e.length : 0) : e.length;
+#pragma unroll 1
+          for (int kind = 0; kind < 2; ++kind, ++it) {
+            const int st = it % C::kStages;
+            ok = mbar_wait_bounded(&bars->kv_empty[st], ((it / C::kStages) & 1) ^ 1, abort_flag, kTimeoutNs);
+            ok = converters_agree(ok);  // and the next tile's pages are there
+            if (!ok) break;
+            uint8_t* const dst = store + st * C::kTileBytes;
+#pragma unroll
+            for (int i = 0; i < C::kChunks; ++i) {
+              const int row = i * kRowsPerPass + row0;
+              uint4 v = held[i % kHeld];
+              // the register's next load: a later pass of this unit, or the next unit's
+              if (i + kHeld < C::kChunks) held[i % kHeld] = fetch(i + kHeld, kind, slot, key0, e.length);
+              else if (kind == 0) held[i % kHeld] = fetch(i + kHeld - C::kChunks, 1, slot, key0, e.length);
+              else held[i % kHeld] = fetch(i + kHeld - C::kChunks, 0, next_slot, next_key0, next_length);
+              uint32_t f[8];
+              if (edge && kind == 1) {
+                uint32_t x[4] = {v.x, v.y, v.z, v.w};
+                if ((nan_bits(x[0]) | nan_bits(x[1]) | nan_bits(x[2]) | nan_bits(x[3])) != 0) {
+#pragma unroll
+                  for (int k = 0; k < 16; ++k)
+                    if ((x[k >> 2] >> (8 * (k & 3)) & 0x7fu) == 0x7fu) {
+                      atomicMin(nan_here + c * 16 + k, key0 + row);
+                      x[k >> 2] &= ~(0xffu << (8 * (k & 3)));
+                    }
+                  *any_nan = 1;
+                  v = make_uint4(x[0], x[1], x[2], x[3]);
+                }
+              }
+              codes_to_f16(v.x, f[0], f[1]);
+              codes_to_f16(v.y, f[2], f[3]);
+              codes_to_f16(v.z, f[4], f[5]);
+              codes_to_f16(v.w, f[6], f[7]);
+              uint8_t* const at = dst + row * 128;
+              sts128(at + (((2 * c) & 7) ^ (row & 7)) * 16, f[0], f[1], f[2], f[3]);
+              sts128(at + (((2 * c + 1) & 7) ^ (row & 7)) * 16, f[4], f[5], f[6], f[7]);
+            }
+            fence_proxy_async_shared();
+            mbar_arrive(&bars->kv_full[st]);
+          }
+        }
+      }
+      if (!ok && tid == 0 && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_LOAD, abort_flag);
+    }
+  } else {
+    regs_inc<kSoftmaxRegs>();
+    // ------------------------------------------------------------ softmax + epilogue
+    const int t = warp >> 2;  // row tile of this warpgroup
+    if (t < C::kTiles && has_run) {
+      const int quarter = warp & 3;  // TMEM lanes this warp may access
+      const int r_in_tile = quarter * 32 + lane;
+      const uint32_t lane_bits = static_cast<uint32_t>(quarter * 32) << 16;
+      const uint32_t t_s = tmem + lane_bits + t * 128;
+      const uint32_t t_o = tmem + lane_bits + 256 + t * D;
+      const int rows = p.group * p.T;
+      bool ok = true;
+      int tile_no = 0, seen = 0, segs = 0, seg = 0;
+      for (Walk<D> w(p, w0, w1, start_b, start_w); ok && w.valid(); w.next()) {
+        const Segment s = w.s;
+        const int nan_slot = seg++ % kNan;
+        if (t == 1 && !w.two()) {
+          tile_no += s.n;
+          continue;
+        }
+        const int row = s.rb * C::kRows + t * kTileRows + r_in_tile;
+        const int tok = row / p.group, hd = s.h * p.group + (row - tok * p.group);
+        const bool real = row < rows && tok < w.e.count;
+        const int lim = real ? row_limit(w.e.length, w.e.count, tok, p.causal) : 0;
+        const int safe = __reduce_min_sync(0xffffffffu, lim > 0 ? lim : 0x7fffffff);
+
+        // The row of q times a power of two, with its largest value in [2^14, 2^15), as fp16.
+        float mul;
+        {
+          const uint4* q = reinterpret_cast<const uint4*>(
+              static_cast<const uint16_t*>(p.q) + s.b * p.q_sb + static_cast<int64_t>(hd) * p.q_sh +
+              static_cast<int64_t>(tok) * p.q_ss);
+          float amax = 0.f;
+          if (real)
+#pragma unroll 8
+            for (int i = 0; i < p.D / 8; ++i) {
+              const uint4 v = q[i];
+              const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 a = unpack16(x[k], p.bf16);
+                amax = fmaxf(amax, fmaxf(fabsf(a.x), fabsf(a.y)));
+              }
+            }
+          const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 14, -126), 113);
+          const float up = pow2f(-ex);
+          mul = p.scale_log2 * pow2f(ex);
+          uint8_t* dst = q_smem + t * C::kTileBytes + r_in_tile * 128;
+#pragma unroll 4
+          for (int i = 0; i < D / 8; ++i) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (real && i * 8 < p.D) v = q[i];
+            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+            uint32_t y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 a = unpack16(x[k], p.bf16);
+              y[k] = pack_f16(a.x * up, a.y * up);
+            }
+            sts128(dst + (i >> 3) * (kTileRows * 128) + ((i & 7) ^ (r_in_tile & 7)) * 16, y[0], y[1],
+                   y[2], y[3]);
+          }
+          fence_proxy_async_shared();
+          mbar_arrive(&bars->q_full[t]);
+        }
+
+        float ref = -INFINITY, l_run = 0.f;
+        for (int j = 0; j < s.n; ++j, ++tile_no, ++seen) {
+          const int slot = tile_no % kMeta;
+          ok = mbar_wait_bounded(&bars->meta_full[slot], (tile_no / kMeta) & 1, abort_flag, kTimeoutNs) &&
+               mbar_wait_bounded(&bars->s_full[t], seen & 1, abort_flag, kTimeoutNs);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          float x[kTileKeys];
+          {
+            uint32_t r0[32], r1[32], r2[32], r3[32];
+            tmem_ld32(t_s + 0, r0);
+            tmem_ld32(t_s + 32, r1);
+            tmem_ld32(t_s + 64, r2);
+            tmem_ld32(t_s + 96, r3);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              x[i] = __uint_as_float(r0[i]);
+              x[32 + i] = __uint_as_float(r1[i]);
+              x[64 + i] = __uint_as_float(r2[i]);
+              x[96 + i] = __uint_as_float(r3[i]);
+            }
+          }
+          const int key0 = (s.t0 + j) * kTileKeys;
+          if (key0 + kTileKeys > safe) {
+#pragma unroll
+            for (int i = 0; i < kTileKeys; ++i)
+              if (key0 + i >= lim) x[i] = -INFINITY;
+          }
+          const Meta* m = meta + slot * kGroups;
+          // t = score * c + e, c held above zero so that a masked score stays -inf
+          float cand = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) {
+            float a = fmaxf(x[16 * g], x[16 * g + 1]), b = fmaxf(x[16 * g + 2], x[16 * g + 3]);
+#pragma unroll
+            for (int i = 4; i < 16; i += 4) {
+              a = fmax3(a, x[16 * g + i], x[16 * g + i + 1]);
+              b = fmax3(b, x[16 * g + i + 2], x[16 * g + i + 3]);
+            }
+            cand = fmaxf(cand, fmaf(fmaxf(a, b), fmaxf(mul * m[g].ks, 1e-37f), m[g].e));
+          }
+          const bool grow = cand > ref + kGrowth;
+          if (__any_sync(0xffffffffu, grow)) {
+            float alpha = 1.f;
+            if (grow) {
+              alpha = ex2_approx(ref - (cand - kBelow));  // 0 from -inf
+              ref = cand - kBelow;
+              l_run *= alpha;
+            }
+            if (j > 0) {
+              const uint64_t alpha2 = f2_pack(alpha, alpha);
+#pragma unroll
+              for (int cc = 0; cc < D / 32; ++cc) {
+                uint32_t o[32];
+                tmem_ld32(t_o + cc * 32, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                  float a0, a1;
+                  f2_unpack(f2_mul(f2_pack(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), alpha2),
+                            a0, a1);
+                  o[i] = __float_as_uint(a0);
+                  o[i + 1] = __float_as_uint(a1);
+                }
+                tmem_st32(t_o + cc * 32, o);
+              }
+            }
+          }
+          const float r = ref == -INFINITY ? 0.f : ref;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int gg = 0; gg < 4; ++gg) {
+              const int g = half * 4 + gg;
+              const float cs = fmaxf(mul * m[g].ks, 1e-37f), sh = m[g].e - r;
+              const uint64_t c2 = f2_pack(cs, cs), s2 = f2_pack(sh, sh);
+              uint64_t sum = f2_pack(0.f, 0.f);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                float a0, a1;
+                f2_unpack(f2_fma(f2_pack(x[16 * g + 2 * i], x[16 * g + 2 * i + 1]), c2, s2), a0, a1);
+                a0 = ex2_approx(a0);
+                a1 = ex2_approx(a1);
+                pk[gg * 8 + i] = pack_f16(a0, a1);
+                sum = f2_add(sum, f2_pack(a0, a1));
+              }
+              float s0, s1;
+              f2_unpack(sum, s0, s1);
+              l_run = fmaf(s0 + s1, m[g].back, l_run);
+            }
+            tmem_st32(t_s + 32 * half, pk);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&bars->p_full[t]);
+        }
+        if (!ok) {
+          if (lane == 0 && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_SOFTMAX, abort_flag);
+          break;
+        }
+        ok = mbar_wait_bounded(&bars->o_final[t], segs & 1, abort_flag, kTimeoutNs);
+        ++segs;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          if (lane == 0 && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_EPILOG, abort_flag);
+          break;
+        }
+        tc_fence_after();
+        const bool whole = s.n == s.tiles;
+        if (lim == 0) {  // a row without keys: its unmasked scores were of no row
+          ref = -INFINITY;
+          l_run = 0.f;
+        }
+        const bool has = ref != -INFINITY;
+        const float inv = !whole ? 1.f : l_run == 0.f ? 0.f : 1.f / l_run;
+        const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + (s.t0 == 0 ? 1 : 0)) * C::kRows +
+                             t * kTileRows + r_in_tile;
+        uint16_t* out = static_cast<uint16_t*>(p.o) + s.b * p.o_sb + static_cast<int64_t>(hd) * p.o_sh +
+                        static_cast<int64_t>(tok) * p.o_ss;
+        const bool any_nan = *static_cast<volatile int*>(&bars->any_nan[nan_slot]) != 0;
+        const int* nan_here = nan_key + nan_slot * D;
+#pragma unroll
+        for (int cc = 0; cc < D / 32; ++cc) {
+          uint32_t o[32];
+          tmem_ld32(t_o + cc * 32, o);
+          tmem_wait_ld();
+          if (any_nan) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (nan_here[cc * 32 + i] < lim) o[i] = 0x7fffffffu;
+          }
+          if (row < rows) {
+            if (!whole) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                if (cc * 32 + i < p.D)
+                  *reinterpret_cast<float4*>(p.part_o + part * D + cc * 32 + i) =
+                      has ? make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
+                                        __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]))
+                          : make_float4(0.f, 0.f, 0.f, 0.f);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 8)
+                if (cc * 32 + i < p.D) {
+                  uint32_t y[4];
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    const float a = has ? __uint_as_float(o[i + 2 * k]) : 0.f;
+                    const float b = has ? __uint_as_float(o[i + 2 * k + 1]) : 0.f;
+                    y[k] = pack16(a * inv, b * inv, p.bf16);
+                  }
+                  sts128(out + cc * 32 + i, y[0], y[1], y[2], y[3]);
+                }
+            }
+          }
+        }
+        if (row < rows) {
+          if (!whole)
+            *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(ref, l_run);
+          else if (p.lse)
+            p.lse[(static_cast<int64_t>(s.b) * p.Hq + hd) * p.T + tok] = lse_of(ref, l_run);
+        }
+        // The run that ends a cut block leaves its merge's address.
+        if (t == 0 && threadIdx.x == 0 && s.t0 > 0 && s.t0 + s.n == s.tiles) {
+          p.cuts[blockIdx.x] =
+              Cut{s.b, s.h, s.rb, static_cast<int>(run_of(w.at - s.t0, sc.total, parts))};
+        }
+        // The next block's MMAs write the accumulator that was just read.
+        tc_fence_before();
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Merges the blocks that several runs share: blockIdx.x = the run that ends the block,
+// blockIdx.y = 32 of its rows, four a warp.
+template <int D>
+__global__ void __launch_bounds__(256) merge_kernel(const AttendParams p) {
+  using C = Cfg<D>;
+  constexpr int kVec = D <= 128 ? 1 : 2;  // float4 a lane
+  constexpr int kPer = 4;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Cut cut = p.cuts[blockIdx.x];
+  if (cut.first < 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rows = min(p.group * p.T - cut.rb * C::kRows, C::kRows);
+  const int r0 = blockIdx.y * 32 + warp * kPer;
+  if (r0 >= rows) return;
+  float m[kPer], l[kPer];
+  float4 a[kPer][kVec];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    m[k] = -INFINITY;
+    l[k] = 0.f;
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) a[k][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll 2
+  for (int i = cut.first; i <= static_cast<int>(blockIdx.x); ++i) {
+    // the block's first run has it in its second slot, the others in their first
+    const int64_t at = (static_cast<int64_t>(i) * 2 + (i == cut.first ? 1 : 0)) * C::kRows + r0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      if (r0 + k >= rows) break;
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (at + k) * 2);
+      // without a reference: sums of 0 or NaN and outputs of 0, kept as they are
+      const float mn = fmaxf(m[k], ml.x);
+      const float fa = m[k] == -INFINITY ? 1.f : exp2f(m[k] - mn);
+      const float fb = ml.x == -INFINITY ? 1.f : exp2f(ml.x - mn);
+      l[k] = l[k] * fa + ml.y * fb;
+      m[k] = mn;
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) {
+        const int d = (v * 32 + lane) * 4;
+        if (d < p.D) {
+          const float4 x = *reinterpret_cast<const float4*>(p.part_o + (at + k) * D + d);
+          a[k][v].x = a[k][v].x * fa + x.x * fb;
+          a[k][v].y = a[k][v].y * fa + x.y * fb;
+          a[k][v].z = a[k][v].z * fa + x.z * fb;
+          a[k][v].w = a[k][v].w * fa + x.w * fb;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    if (r0 + k >= rows) break;
+    const int row = cut.rb * C::kRows + r0 + k;
+    const int tok = row / p.group, hd = cut.h * p.group + (row - tok * p.group);
+    const float inv = l[k] == 0.f ? 0.f : 1.f / l[k];
+    uint16_t* out = static_cast<uint16_t*>(p.o) + cut.b * p.o_sb + static_cast<int64_t>(hd) * p.o_sh +
+                    static_cast<int64_t>(tok) * p.o_ss;
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) {
+      const int d = (v * 32 + lane) * 4;
+      if (d < p.D)
+        *reinterpret_cast<uint2*>(out + d) =
+            make_uint2(pack16(a[k][v].x * inv, a[k][v].y * inv, p.bf16),
+                       pack16(a[k][v].z * inv, a[k][v].w * inv, p.bf16));
+    }
+    if (p.lse && lane == 0)
+      p.lse[(static_cast<int64_t>(cut.b) * p.Hq + hd) * p.T + tok] = lse_of(m[k], l[k]);
+  }
+}
+
+template <int D>
+size_t workspace(int sm_count) {
+  return static_cast<size_t>(sm_count) * (2 * Cfg<D>::kRows * (D + 2) * sizeof(float) + sizeof(Cut));
+}
+
+template <int D>
+cudaError_t launch(AttendParams p, int sm_count, cudaStream_t stream) {
+  using C = Cfg<D>;
+  auto kern = chunk_kernel<D>;
+  static int configured = 0;  // one bit per device ordinal (< 32)
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev >= 32 || !(__atomic_load_n(&configured, __ATOMIC_ACQUIRE) & (1 << dev))) {
+    // setmaxnreg.inc would wait forever if the block were launched with fewer registers than
+    // the split assumes: check the built register count first.
+    cudaFuncAttributes attr;
+    if ((err = cudaFuncGetAttributes(&attr, kern)) != cudaSuccess) return err;
+    if (attr.numRegs != kLaunchRegs) return cudaErrorInvalidKernelImage;
+    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+    if (err != cudaSuccess) return err;
+    if (dev < 32) __atomic_fetch_or(&configured, 1 << dev, __ATOMIC_ACQ_REL);
+  }
+  const int64_t rows = static_cast<int64_t>(p.group) * p.T;
+  p.row_blocks = static_cast<int>((rows + C::kRows - 1) / C::kRows);
+  const int64_t seq_tiles = (static_cast<int64_t>(p.width) * p.page + kTileKeys - 1) / kTileKeys;
+  const int64_t most = seq_tiles * p.Hkv * p.row_blocks * p.B;
+  const int parts = static_cast<int>(most < sm_count ? most : sm_count);
+  const int64_t part_rows = static_cast<int64_t>(sm_count) * 2 * C::kRows;
+  p.part_ml = p.part_o + part_rows * D;
+  p.cuts = reinterpret_cast<Cut*>(p.part_ml + part_rows * 2);
+  kern<<<parts, kThreads, C::kBytes, stream>>>(p);
+  if ((err = cudaGetLastError()) != cudaSuccess) return err;
+  cudaLaunchConfig_t cfg{};
+  const int merged = static_cast<int>(rows < C::kRows ? rows : C::kRows);
+  cfg.gridDim = dim3(parts, (merged + 31) / 32);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, merge_kernel<D>, p);
+}
+
+}  // namespace
+}  // namespace chunk
+
+size_t chunk_workspace_bytes(int D, int sm_count) {
+  return D <= 64 ? chunk::workspace<64>(sm_count)
+                 : D <= 128 ? chunk::workspace<128>(sm_count) : chunk::workspace<256>(sm_count);
+}
+
+cudaError_t launch_chunk(const AttendParams& p, int sm_count, cudaStream_t stream) {
+  if (p.D <= 64) return chunk::launch<64>(p, sm_count, stream);
+  if (p.D <= 128) return chunk::launch<128>(p, sm_count, stream);
+  return chunk::launch<256>(p, sm_count, stream);
+}
+
+}  // namespace kv8
+}  // namespace ta
