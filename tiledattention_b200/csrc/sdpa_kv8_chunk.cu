@@ -9,11 +9,12 @@
 // the keys too. Roles:
 //   warps 0-3, 4-7  softmax and epilogue of row tile 0, 1 (thread = row); they also bring the
 //                   rows of q into shared memory as fp16 times a power of two
-//   warps 8-11      converters: codes from the pages straight into registers (the next unit's
-//                   while this one is converted), fp16 (exact) into the 128-byte-swizzled tiles
-//                   that tcgen05 reads, a unit being one tile's K or V
+//   warps 8-11      converters: codes from the pages straight into registers (up to a tile
+//                   ahead), fp16 (exact) into the 128-byte-swizzled tiles that tcgen05 reads, a
+//                   unit being one tile's K or V
 //   warp 12         tensor memory and MMA issue (kind::f16, fp16 operands)
-//   warps 13-15     zero the rows of blocks without keys
+//   warp 13         walks ahead through page table and scales
+//   warps 14-15     zero the rows of blocks without keys
 // Converting once in shared memory costs 2 D x 128 conversions a tile for 256 rows; fp8
 // MMAs would take e4m3 as it is, but then the weights have to be cut into several fp8 parts,
 // which costs the softmax warps, the tightest role, about three operations more an element.
@@ -41,7 +42,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 // Register split of the launch's 512 x 128 registers: softmax, converters, MMA and idle.
 constexpr int kLaunchRegs = 128;
-constexpr int kSoftmaxRegs = 192, kConvertRegs = 80, kSideRegs = 48;
+constexpr int kSoftmaxRegs = 168, kConvertRegs = 128, kSideRegs = 48;
 static_assert(128 * (2 * kSoftmaxRegs + kConvertRegs + kSideRegs) == kThreads * kLaunchRegs,
               "register split must match the launch allocation");
 constexpr uint32_t kTmemCols = 512;
@@ -49,7 +50,7 @@ constexpr float kBelow = 7.f, kGrowth = 15.f;  // see sdpa_kv8.cu
 constexpr uint64_t kTimeoutNs = 1000000000ull;  // 1 s per wait
 constexpr int kMeta = 8;                       // tiles whose pages and scales are kept
 constexpr int kGroups = kTileKeys / 16;        // blocks of 16 keys: one page each
-constexpr int kNan = 8;                        // segments whose NaN values are kept (see Segment)
+constexpr int kNan = 16;                       // segments whose NaN values are kept (see Segment)
 
 template <int D>
 struct Cfg {
@@ -76,7 +77,7 @@ struct Meta {  // of 16 keys: where they are, and their scales in softmax's term
 struct Barriers {
   uint64_t q_full[2], s_full[2], p_full[2], o_final[2];
   uint64_t drain;
-  uint64_t kv_full[6], kv_empty[6], meta_full[kMeta];
+  uint64_t kv_full[6], kv_empty[6], meta_full[kMeta], meta_empty[kMeta];
   int any_nan[kNan];
   int64_t scan[kWarps];
   int start_b;
@@ -89,7 +90,7 @@ static_assert(sizeof(Barriers) <= 512, "barrier block");
 // A block of rows on the line and the part of it that this run has. Where some of its rows do not
 // see a key, that key's value must not reach them as 0 * NaN: the converters write such NaNs as
 // zeros and note, for each dim, the first key that has one, and the epilogue gives the NaN to the
-// rows that see it. Notes are kept for kNan segments: the converters are at most three tiles ahead.
+// rows that see it. Notes are kept for kNan segments, more than the 8 tiles that warp 13 (which clears them) is ahead.
 struct Segment {
   int b, h, rb, t0, n, tiles;  // key tiles [t0, t0 + n) of `tiles`
 };
@@ -157,16 +158,6 @@ __device__ __forceinline__ void report(const AttendParams& p, uint32_t code, vol
   if (p.status) atomicOr(p.status, code);
 }
 
-// Whether all 128 converters say so; a barrier among them.
-__device__ __forceinline__ bool converters_agree(bool ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r) : "r"(ok ? 1u : 0u) : "memory");
-  return r != 0;
-}
-
 __device__ __forceinline__ void sts128(void* a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   *reinterpret_cast<uint4*>(a) = make_uint4(x, y, z, w);
 }
@@ -206,7 +197,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       mbar_init(&bars->kv_full[s], 128);
       mbar_init(&bars->kv_empty[s], 1);
     }
-    for (int i = 0; i < kMeta; ++i) mbar_init(&bars->meta_full[i], kGroups);
+    for (int i = 0; i < kMeta; ++i) {
+      mbar_init(&bars->meta_full[i], 32);
+      mbar_init(&bars->meta_empty[i], 1);
+    }
     bars->abort_flag = 0;
     p.cuts[blockIdx.x] = Cut{0, 0, 0, -1};  // until this thread knows better
     fence_mbar_init();
@@ -277,6 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         int it = 0;                // units taken
         int seen[2] = {0, 0};      // tiles of each row tile
         int segs[2] = {0, 0};
+        int tile_no = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, int phase) {
           ok = ok && mbar_wait_bounded(bar, phase & 1, abort_flag, kTimeoutNs);
@@ -314,6 +309,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
               }
             }
             if (!ok) break;
+            // Softmax has taken this tile's scales and the converters its pages.
+            mbar_arrive(&bars->meta_empty[tile_no++ % kMeta]);
             if (more) ++it;
           }
         }
@@ -325,6 +322,75 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           atomicOr(p.status, TA_DEVSTAT_TIMEOUT_DRAIN);
       }
       __syncwarp();
+    } else if (warp == 13) {
+      // ------------------------------------------------------------ pages and scales
+      // Lane i < 8: block i of 16 keys of a tile. Page ids are fetched two tiles and scales one
+      // tile before they are published.
+      if (has_run) {
+        Walk<D> w(p, w0, w1, start_b, start_w);
+        int j = 0, seg = 0;
+        bool first = true;
+        struct Ahead {
+          int id, h;       // page id, -1: no key, -2: outside the cache
+          bool first;
+          int seg;
+        };
+        auto next_ids = [&](Ahead& a) {  // of the next tile of the run, and on
+          a.id = -1;
+          a.first = first;
+          a.seg = seg;
+          if (!w.valid()) return false;
+          a.h = w.s.h;
+          const int key = (w.s.t0 + j) * kTileKeys + lane * 16;
+          if (lane < kGroups && key < w.e.length) {
+            a.id = p.table[w.s.b * p.table_stride + (key >> p.page_shift)];
+            if (static_cast<unsigned>(a.id) >= static_cast<unsigned>(p.num_pages)) a.id = -2;
+          }
+          first = ++j == w.s.n;
+          if (first) {
+            j = 0;
+            ++seg;
+            w.next();
+          }
+          return true;
+        };
+        Ahead a0, a1;
+        float ks = 1.f, vs = 1.f;
+        auto fetch_scales = [&](const Ahead& a) {
+          if (a.id >= 0) {
+            const int64_t plane = static_cast<int64_t>(a.id) * p.Hkv + a.h;
+            ks = p.scale[0][plane];
+            vs = p.scale[1][plane];
+          }
+        };
+        bool have0 = next_ids(a0), have1 = next_ids(a1);
+        fetch_scales(a0);
+        bool ok = true;
+        for (int n = 0; ok && have0; ++n) {
+          Meta m{-1, 1.f, -INFINITY, 0.f};
+          if (a0.id >= 0) {
+            const int ev = stored_exponent(__float_as_uint(vs));
+            m = Meta{a0.id * p.Hkv + a0.h, ks, static_cast<float>(ev), pow2f(-ev)};
+          } else if (a0.id == -2 && p.status) {
+            atomicOr(p.status, TA_DEVSTAT_BAD_PAGE);
+          }
+          const Ahead now = a0;
+          a0 = a1;
+          have0 = have1;
+          have1 = next_ids(a1);
+          fetch_scales(a0);
+          ok = mbar_wait_bounded(&bars->meta_empty[n % kMeta], ((n / kMeta) & 1) ^ 1, abort_flag, kTimeoutNs);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (now.first) {  // a segment's first tile: no NaN noted yet
+            for (int d = lane; d < D; d += 32) nan_key[(now.seg % kNan) * D + d] = 0x7fffffff;
+            if (lane == 0) bars->any_nan[now.seg % kNan] = 0;
+          }
+          if (lane < kGroups) meta[(n % kMeta) * kGroups + lane] = m;
+          mbar_arrive(&bars->meta_full[n % kMeta]);
+        }
+        if (!ok && lane == 0 && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_LOAD, abort_flag);
+      }
     } else {
       // ------------------------------------------------------------ rows of blocks without keys
       const int rows = p.group * p.T;
@@ -336,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         if (block_tiles(extent_of(p, b), p.group, rb * C::kRows, C::kRows, p.T, p.causal, kTileKeys))
           continue;
         const int r1 = min(rows, (rb + 1) * C::kRows);
-        for (int r = rb * C::kRows + warp - 13; r < r1; r += 3) {
+        for (int r = rb * C::kRows + warp - 14; r < r1; r += 2) {
           const int tok = r / p.group, hd = h * p.group + (r - tok * p.group);
           uint16_t* out = static_cast<uint16_t*>(p.o) + b * p.o_sb + hd * p.o_sh + tok * p.o_ss;
           for (int d = lane * 8; d < p.D; d += 256) sts128(out + d, 0, 0, 0, 0);
@@ -350,7 +416,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
     regs_dec<kConvertRegs>();
     if (has_run) {
       constexpr int kRowsPerPass = 128 / C::kChunks;  // of 128 threads, 16 codes each
-      constexpr int kHeld = C::kChunks < 8 ? C::kChunks : 8;  // passes in flight
+      // Passes in flight: those of a tile (K and V), at head dim 256 of a unit.
+      constexpr bool kWholeTile = C::kChunks <= 8;
+      constexpr int kHeld = kWholeTile ? 2 * C::kChunks : C::kChunks;
       const int tid = threadIdx.x - 256;
       // Lanes: 4 chunks of one 128-byte row of the tile and the next key's, so that 8
       // lanes' 16-byte stores meet 8 different banks.
@@ -364,40 +432,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       bool ok = true;
       int it = 0, tile_no = 0, seg = 0;
 
-      // Pages and scales are published a tile ahead by lanes 0-7 of the first warp, one a
-      // block of 16 keys. `ahead` walks in front of `w`.
-      Walk<D> w(p, w0, w1, start_b, start_w), ahead(p, w0, w1, start_b, start_w);
-      int ahead_tile = 0, published = 0;
-      auto publish = [&]() {
-        if (!ahead.valid()) return;
-        if (tid < kGroups) {
-          const int key = (ahead.s.t0 + ahead_tile) * kTileKeys + tid * 16;
-          Meta m{-1, 1.f, -INFINITY, 0.f};
-          if (key < ahead.e.length) {
-            const int id = p.table[ahead.s.b * p.table_stride + (key >> p.page_shift)];
-            if (static_cast<unsigned>(id) < static_cast<unsigned>(p.num_pages)) {
-              m.plane = id * p.Hkv + ahead.s.h;
-              m.ks = p.scale[0][m.plane];
-              const int ev = stored_exponent(__float_as_uint(p.scale[1][m.plane]));
-              m.e = static_cast<float>(ev);
-              m.back = pow2f(-ev);
-            } else if (p.status) {
-              atomicOr(p.status, TA_DEVSTAT_BAD_PAGE);
-            }
-          }
-          meta[(published % kMeta) * kGroups + tid] = m;
-          mbar_arrive(&bars->meta_full[published % kMeta]);
-        }
-        ++published;
-        if (++ahead_tile == ahead.s.n) {
-          ahead_tile = 0;
-          ahead.next();
-        }
-      };
-      publish();
-      converters_agree(true);
-
-      uint4 held[kHeld];
       // Codes of pass i of a unit: kind 0 K, 1 V, of the tile in meta slot `slot` whose first key is
       // key0, of a sequence of `length` keys. Rows without a key read as zeros.
       auto fetch = [&](int i, int kind, int slot, int key0, int length) {
@@ -410,19 +444,27 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
               (static_cast<int64_t>(plane) * p.page + ((key0 + row) & (p.page - 1))) * p.D + c * 16));
         return v;
       };
+      auto wait_meta = [&](int n) {
+        return mbar_wait_bounded(&bars->meta_full[n % kMeta], (n / kMeta) & 1, abort_flag, kTimeoutNs);
+      };
+
+      Walk<D> w(p, w0, w1, start_b, start_w);
+      uint4 held[kHeld];
+      ok = wait_meta(0);
+      if (ok) {
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i)
-        held[i] = fetch(i, 0, 0, w.s.t0 * kTileKeys, w.e.length);
+        for (int i = 0; i < kHeld; ++i)
+          held[i] = fetch(i % C::kChunks, i / C::kChunks, 0, w.s.t0 * kTileKeys, w.e.length);
+      }
       while (ok && w.valid()) {
         const Segment s = w.s;
-        const SeqExtent e = w.e;
-        // Keys that every row of the block with any keys sees: tiles beyond need care with NaN.
+        const int length = w.e.length;
+        // Keys that every row of the block with any keys sees: values beyond need care with NaN.
         const int rows = min(p.group * p.T, (s.rb + 1) * C::kRows);
-        int safe = e.length;
+        int safe = length;
         if (p.causal) {
-          const int first = s.rb * C::kRows / p.group;
-          for (int tok = first; tok <= (rows - 1) / p.group; ++tok) {
-            const int lim = row_limit(e.length, e.count, tok, 1);
+          for (int tok = s.rb * C::kRows / p.group; tok <= (rows - 1) / p.group; ++tok) {
+            const int lim = row_limit(length, w.e.count, tok, 1);
             if (lim > 0) {
               safe = lim;
               break;
@@ -433,45 +475,50 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         int* const nan_here = nan_key + (seg % kNan) * D;
         int* const any_nan = &bars->any_nan[seg % kNan];
         ++seg;
-        for (int d = tid; d < D; d += 128) nan_here[d] = 0x7fffffff;
-        if (tid == 0) *any_nan = 0;  // the barrier before the first unit lies between
         for (int j = 0; ok && j < s.n; ++j, ++tile_no) {
-          publish();  // the tile after this one
           const int key0 = (s.t0 + j) * kTileKeys;
           const bool edge = key0 + kTileKeys > safe;
           const bool last_tile = j + 1 == s.n;
           const int slot = tile_no % kMeta, next_slot = (tile_no + 1) % kMeta;
           const int next_key0 = last_tile ? w.s.t0 * kTileKeys : key0 + kTileKeys;
-          const int next_length = last_tile ? (w.valid() ? w.e.length : 0) : e.length;
-#pragma unroll 1
-          for (int kind = 0; kind < 2; ++kind, ++it) {
+          const int next_length = last_tile ? (w.valid() ? w.e.length : 0) : length;
+          if (next_length > 0) ok = wait_meta(tile_no + 1);
+#pragma unroll
+          for (int kind = 0; kind < 2; ++kind) {
             const int st = it % C::kStages;
-            ok = mbar_wait_bounded(&bars->kv_empty[st], ((it / C::kStages) & 1) ^ 1, abort_flag, kTimeoutNs);
-            ok = converters_agree(ok);  // and the next tile's pages are there
+            ok = ok && mbar_wait_bounded(&bars->kv_empty[st], ((it / C::kStages) & 1) ^ 1, abort_flag,
+                                         kTimeoutNs);
             if (!ok) break;
+            ++it;
             uint8_t* const dst = store + st * C::kTileBytes;
 #pragma unroll
             for (int i = 0; i < C::kChunks; ++i) {
               const int row = i * kRowsPerPass + row0;
-              uint4 v = held[i % kHeld];
-              // the register's next load: a later pass of this unit, or the next unit's
-              if (i + kHeld < C::kChunks) held[i % kHeld] = fetch(i + kHeld, kind, slot, key0, e.length);
-              else if (kind == 0) held[i % kHeld] = fetch(i + kHeld - C::kChunks, 1, slot, key0, e.length);
-              else held[i % kHeld] = fetch(i + kHeld - C::kChunks, 0, next_slot, next_key0, next_length);
-              uint32_t f[8];
+              uint4& h = held[kWholeTile ? kind * C::kChunks + i : i];
+              uint4 v = h;
+              // the register's next load
+              if (kWholeTile) h = fetch(i, kind, next_slot, next_key0, next_length);
+              else if (kind == 0) h = fetch(i, 1, slot, key0, length);
+              else h = fetch(i, 0, next_slot, next_key0, next_length);
               if (edge && kind == 1) {
                 uint32_t x[4] = {v.x, v.y, v.z, v.w};
                 if ((nan_bits(x[0]) | nan_bits(x[1]) | nan_bits(x[2]) | nan_bits(x[3])) != 0) {
-#pragma unroll
-                  for (int k = 0; k < 16; ++k)
-                    if ((x[k >> 2] >> (8 * (k & 3)) & 0x7fu) == 0x7fu) {
-                      atomicMin(nan_here + c * 16 + k, key0 + row);
-                      x[k >> 2] &= ~(0xffu << (8 * (k & 3)));
-                    }
                   *any_nan = 1;
-                  v = make_uint4(x[0], x[1], x[2], x[3]);
+#pragma unroll 1
+                  for (int k = 0; k < 4; ++k) {
+                    uint32_t y = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w;
+                    for (int b = 0; b < 4; ++b)
+                      if ((y >> (8 * b) & 0x7fu) == 0x7fu)
+                        atomicMin(nan_here + c * 16 + k * 4 + b, key0 + row);
+                    y &= ~((nan_bits(y) >> 7) * 0xffu);
+                    if (k == 0) v.x = y;
+                    else if (k == 1) v.y = y;
+                    else if (k == 2) v.z = y;
+                    else v.w = y;
+                  }
                 }
               }
+              uint32_t f[8];
               codes_to_f16(v.x, f[0], f[1]);
               codes_to_f16(v.y, f[2], f[3]);
               codes_to_f16(v.z, f[4], f[5]);
@@ -561,40 +608,37 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
-          float x[kTileKeys];
-          {
-            uint32_t r0[32], r1[32], r2[32], r3[32];
-            tmem_ld32(t_s + 0, r0);
-            tmem_ld32(t_s + 32, r1);
-            tmem_ld32(t_s + 64, r2);
-            tmem_ld32(t_s + 96, r3);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              x[i] = __uint_as_float(r0[i]);
-              x[32 + i] = __uint_as_float(r1[i]);
-              x[64 + i] = __uint_as_float(r2[i]);
-              x[96 + i] = __uint_as_float(r3[i]);
-            }
-          }
+          // Two passes over the scores, 32 columns in registers at a time (reading tensor memory
+          // twice costs less than holding 128 scores).
           const int key0 = (s.t0 + j) * kTileKeys;
-          if (key0 + kTileKeys > safe) {
-#pragma unroll
-            for (int i = 0; i < kTileKeys; ++i)
-              if (key0 + i >= lim) x[i] = -INFINITY;
-          }
+          const int visible = key0 + kTileKeys > safe ? lim - key0 : kTileKeys;  // of this tile's
+          const bool edge = key0 + kTileKeys > safe;
           const Meta* m = meta + slot * kGroups;
           // t = score * c + e, c held above zero so that a masked score stays -inf
           float cand = -INFINITY;
 #pragma unroll
-          for (int g = 0; g < kGroups; ++g) {
-            float a = fmaxf(x[16 * g], x[16 * g + 1]), b = fmaxf(x[16 * g + 2], x[16 * g + 3]);
+          for (int q4 = 0; q4 < 4; ++q4) {
+            uint32_t y[32];
+            tmem_ld32(t_s + 32 * q4, y);
+            tmem_wait_ld();
+            if (edge) {
 #pragma unroll
-            for (int i = 4; i < 16; i += 4) {
-              a = fmax3(a, x[16 * g + i], x[16 * g + i + 1]);
-              b = fmax3(b, x[16 * g + i + 2], x[16 * g + i + 3]);
+              for (int i = 0; i < 32; ++i)
+                if (q4 * 32 + i >= visible) y[i] = 0xff800000u;
             }
-            cand = fmaxf(cand, fmaf(fmaxf(a, b), fmaxf(mul * m[g].ks, 1e-37f), m[g].e));
+#pragma unroll
+            for (int gg = 0; gg < 2; ++gg) {
+              const uint32_t* x = y + 16 * gg;
+              float a = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+              float b = fmaxf(__uint_as_float(x[2]), __uint_as_float(x[3]));
+#pragma unroll
+              for (int i = 4; i < 16; i += 4) {
+                a = fmax3(a, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                b = fmax3(b, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+              }
+              const int g = q4 * 2 + gg;
+              cand = fmaxf(cand, fmaf(fmaxf(a, b), fmaxf(mul * m[g].ks, 1e-37f), m[g].e));
+            }
           }
           const bool grow = cand > ref + kGrowth;
           if (__any_sync(0xffffffffu, grow)) {
@@ -623,30 +667,44 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
               }
             }
           }
+          // The weights (16-bit, two a column) go over the first 64 columns: the second pass reads
+          // ahead of them.
           const float r = ref == -INFINITY ? 0.f : ref;
+          uint32_t pk[32], y[32];
+          tmem_ld32(t_s, y);
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t pk[32];
+          for (int q4 = 0; q4 < 4; ++q4) {
+            tmem_wait_ld();
+            reg_fence32(y);
+            if (edge) {
 #pragma unroll
-            for (int gg = 0; gg < 4; ++gg) {
-              const int g = half * 4 + gg;
+              for (int i = 0; i < 32; ++i)
+                if (q4 * 32 + i >= visible) y[i] = 0xff800000u;
+            }
+#pragma unroll
+            for (int gg = 0; gg < 2; ++gg) {
+              const int g = q4 * 2 + gg;
               const float cs = fmaxf(mul * m[g].ks, 1e-37f), sh = m[g].e - r;
               const uint64_t c2 = f2_pack(cs, cs), s2 = f2_pack(sh, sh);
               uint64_t sum = f2_pack(0.f, 0.f);
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 float a0, a1;
-                f2_unpack(f2_fma(f2_pack(x[16 * g + 2 * i], x[16 * g + 2 * i + 1]), c2, s2), a0, a1);
+                f2_unpack(f2_fma(f2_pack(__uint_as_float(y[16 * gg + 2 * i]),
+                                         __uint_as_float(y[16 * gg + 2 * i + 1])), c2, s2), a0, a1);
                 a0 = ex2_approx(a0);
                 a1 = ex2_approx(a1);
-                pk[gg * 8 + i] = pack_f16(a0, a1);
+                pk[(q4 & 1) * 16 + gg * 8 + i] = pack_f16(a0, a1);
                 sum = f2_add(sum, f2_pack(a0, a1));
               }
               float s0, s1;
               f2_unpack(sum, s0, s1);
               l_run = fmaf(s0 + s1, m[g].back, l_run);
             }
-            tmem_st32(t_s + 32 * half, pk);
+            if (q4 < 3) tmem_ld32(t_s + 32 * (q4 + 1), y);
+            // columns 0-31 are written once 0-63 have been read, 32-63 at the end
+            if (q4 == 1) tmem_st32(t_s, pk);
+            if (q4 == 3) tmem_st32(t_s + 32, pk);
           }
           tmem_wait_st();
           tc_fence_before();
