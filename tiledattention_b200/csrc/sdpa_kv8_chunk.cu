@@ -42,15 +42,15 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 // Register split of the launch's 512 x 128 registers: softmax, converters, MMA and idle.
 constexpr int kLaunchRegs = 128;
-constexpr int kSoftmaxRegs = 168, kConvertRegs = 128, kSideRegs = 48;
+constexpr int kSoftmaxRegs = 152, kConvertRegs = 128, kSideRegs = 80;
 static_assert(128 * (2 * kSoftmaxRegs + kConvertRegs + kSideRegs) == kThreads * kLaunchRegs,
               "register split must match the launch allocation");
 constexpr uint32_t kTmemCols = 512;
 constexpr float kBelow = 7.f, kGrowth = 15.f;  // see sdpa_kv8.cu
 constexpr uint64_t kTimeoutNs = 1000000000ull;  // 1 s per wait
-constexpr int kMeta = 8;                       // tiles whose pages and scales are kept
+constexpr int kMeta = 8;                       // tiles whose places, pages and scales are kept
 constexpr int kGroups = kTileKeys / 16;        // blocks of 16 keys: one page each
-constexpr int kNan = 16;                       // segments whose NaN values are kept (see Segment)
+constexpr int kSegs = 8;                       // segments that are kept
 
 template <int D>
 struct Cfg {
@@ -63,8 +63,8 @@ struct Cfg {
   static constexpr int kKvOff = kTiles * kTileBytes;
   static constexpr int kMetaOff = kKvOff + kStages * kTileBytes;
   static constexpr int kNanOff = kMetaOff + kMeta * kGroups * 16;
-  static constexpr int kBarOff = kNanOff + kNan * D * 4;
-  static constexpr int kBytes = kBarOff + 512 + 1024;  // slack: 1024-byte alignment
+  static constexpr int kBarOff = kNanOff + kSegs * D * 4;
+  static constexpr int kBytes = kBarOff + 1024 + 1024;  // slack: 1024-byte alignment
 };
 
 struct Meta {  // of 16 keys: where they are, and their scales in softmax's terms
@@ -74,39 +74,55 @@ struct Meta {  // of 16 keys: where they are, and their scales in softmax's term
   float back;  // 2^-e
 };
 
+// A key tile on the line, as the converters need it; length -1: the run is over.
+struct Tile {
+  int key0, length, safe, seg;
+};
+
+// A block of rows on the line and the part of it that this run has; n = 0: the run is over. Where
+// some of its rows do not see a key (keys from `safe` on), that key's value must not reach them
+// as 0 * NaN: the converters write such NaNs as zeros and note, for each dim, the first key
+// that has one, and the epilogue gives the NaN to the rows that see it.
+struct Segment {
+  int b, h, rb, t0, n, tiles;  // key tiles [t0, t0 + n) of `tiles`
+  int length, count, safe;
+  int first_run;               // of those that share the block
+};
+
 struct Barriers {
   uint64_t q_full[2], s_full[2], p_full[2], o_final[2];
   uint64_t drain;
-  uint64_t kv_full[6], kv_empty[6], meta_full[kMeta], meta_empty[kMeta];
-  int any_nan[kNan];
-  int64_t scan[kWarps];
-  int start_b;
-  int64_t start_w;
+  uint64_t kv_full[6], kv_empty[6], meta_full[kMeta], meta_empty[kMeta], seg_full[kSegs], seg_empty[kSegs];
+  Segment segs[kSegs];
+  Tile tiles[kMeta];
+  int any_nan[kSegs];
   uint32_t tmem_base;
   int abort_flag;
 };
-static_assert(sizeof(Barriers) <= 512, "barrier block");
-
-// A block of rows on the line and the part of it that this run has. Where some of its rows do not
-// see a key, that key's value must not reach them as 0 * NaN: the converters write such NaNs as
-// zeros and note, for each dim, the first key that has one, and the epilogue gives the NaN to the
-// rows that see it. Notes are kept for kNan segments, more than the 8 tiles that warp 13 (which clears them) is ahead.
-struct Segment {
-  int b, h, rb, t0, n, tiles;  // key tiles [t0, t0 + n) of `tiles`
+struct Start {  // where the run begins; its memory is the accumulator's notes' (kNanOff) until then
+  int64_t scan[kWarps];
+  int64_t w;
+  int b;
 };
+static_assert(sizeof(Barriers) <= 1024 && sizeof(Start) <= kSegs * 64 * 4, "shared memory blocks");
 
+// The run's walk over the line (warp 13's).
 template <int D>
 struct Walk {
   const AttendParams& p;
-  int64_t at, end;
+  int64_t at, end;  // tiles
   Segment s;
   SeqExtent e;
+  __device__ int block() const {
+    return block_tiles(e, p.group, s.rb * Cfg<D>::kRows, Cfg<D>::kRows, p.T, p.causal, kTileKeys);
+  }
   __device__ Walk(const AttendParams& pp, int64_t w0, int64_t w1, int b, int64_t before)
       : p(pp), at(w0), end(w1) {
     s.b = b;
     e = extent_of(p, b);
+    int64_t head = 0;
+    for (s.rb = 0; s.rb < p.row_blocks; ++s.rb) head += block();
     int64_t rem = w0 - before;
-    const int64_t head = head_tiles();
     s.h = static_cast<int>(rem / head);
     rem -= s.h * head;
     s.rb = 0;
@@ -116,42 +132,43 @@ struct Walk {
       ++s.rb;
       s.tiles = block();
     }
-    s.t0 = static_cast<int>(rem);
-    s.n = static_cast<int>(min(end - at, static_cast<int64_t>(s.tiles - s.t0)));
+    begin(static_cast<int>(rem));
   }
-  __device__ int block() const { return block_tiles(e, p.group, s.rb * Cfg<D>::kRows, Cfg<D>::kRows, p.T, p.causal, kTileKeys); }
-  __device__ int64_t head_tiles() const {
-    int64_t n = 0;
-    for (int rb = 0; rb < p.row_blocks; ++rb)
-      n += block_tiles(e, p.group, rb * Cfg<D>::kRows, Cfg<D>::kRows, p.T, p.causal, kTileKeys);
-    return n;
+  __device__ void begin(int t0) {
+    s.t0 = t0;
+    s.n = static_cast<int>(min(end - at, static_cast<int64_t>(s.tiles - t0)));
+    s.length = e.length;
+    s.count = e.count;
+    s.safe = e.length;
+    if (p.causal) {  // the first token with any keys sees the fewest
+      const int tok = max(s.rb * Cfg<D>::kRows / p.group, e.count - e.length);
+      s.safe = row_limit(e.length, e.count, tok, 1);
+    }
   }
-  __device__ bool valid() const { return at < end; }
-  __device__ void next() {
+  __device__ bool next() {
     at += s.n;
-    if (at >= end) return;
+    if (at >= end) return false;
     do {  // the next block with any tiles; there is one, since the run goes on
       if (++s.rb == p.row_blocks) {
         s.rb = 0;
         if (++s.h == p.Hkv) {
           s.h = 0;
-          if (++s.b >= p.B) {
-            at = end;
-            return;
-          }
+          if (++s.b >= p.B) return false;
           e = extent_of(p, s.b);
         }
       }
       s.tiles = block();
     } while (s.tiles == 0);
-    s.t0 = 0;
-    s.n = static_cast<int>(min(end - at, static_cast<int64_t>(s.tiles)));
-  }
-  // Whether the second row tile has any rows.
-  __device__ bool two() const {
-    return Cfg<D>::kTiles == 2 && p.group * p.T - s.rb * Cfg<D>::kRows > kTileRows;
+    begin(0);
+    return true;
   }
 };
+
+// Whether the second row tile of a block has any rows.
+template <int D>
+__device__ __forceinline__ bool has_two(const AttendParams& p, int rb) {
+  return Cfg<D>::kTiles == 2 && p.group * p.T - rb * Cfg<D>::kRows > kTileRows;
+}
 
 __device__ __forceinline__ void report(const AttendParams& p, uint32_t code, volatile int* abort_flag) {
   *abort_flag = 1;
@@ -180,7 +197,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
   uint8_t* q_smem = smem + C::kQOff;
   uint8_t* kv_smem = smem + C::kKvOff;
   Meta* meta = reinterpret_cast<Meta*>(smem + C::kMetaOff);
-  int* nan_key = reinterpret_cast<int*>(smem + C::kNanOff);  // [kNan][D]
+  int* nan_key = reinterpret_cast<int*>(smem + C::kNanOff);  // [kSegs][D]
+  Start* start = reinterpret_cast<Start*>(nan_key);
   Barriers* bars = reinterpret_cast<Barriers*>(smem + C::kBarOff);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -201,6 +219,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       mbar_init(&bars->meta_full[i], 32);
       mbar_init(&bars->meta_empty[i], 1);
     }
+    for (int i = 0; i < kSegs; ++i) {
+      mbar_init(&bars->seg_full[i], 32);
+      mbar_init(&bars->seg_empty[i], 4 * C::kTiles + 1);  // softmax warps and the MMA warp
+    }
     bars->abort_flag = 0;
     p.cuts[blockIdx.x] = Cut{0, 0, 0, -1};  // until this thread knows better
     fence_mbar_init();
@@ -216,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       n += block_tiles(e, p.group, rb * C::kRows, C::kRows, p.T, p.causal, kTileKeys);
     return n * p.Hkv;
   };
-  const Scan sc = scan_batch<kWarps>(p, bars->scan, blockIdx.x == 0, per_seq);  // has a barrier
+  const Scan sc = scan_batch<kWarps>(p, start->scan, blockIdx.x == 0, per_seq);  // has a barrier
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = bars->tmem_base;
@@ -229,15 +251,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
     for (int b = sc.b0; b < sc.b1; ++b) {
       const int64_t n = per_seq(extent_of(p, b));
       if (at <= w0 && w0 < at + n) {
-        bars->start_b = b;
-        bars->start_w = at;
+        start->b = b;
+        start->w = at;
       }
       at += n;
     }
   }
   __syncthreads();
-  const int start_b = bars->start_b;
-  const int64_t start_w = bars->start_w;
 
   if (warp >= 12) {
     regs_dec<kSideRegs>();
@@ -268,42 +288,48 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
                    vd + static_cast<uint64_t>((kk * 16 * 128) >> 4), kIdescPV,
                    (acc || kk > 0) ? 1u : 0u);
         };
-        int it = 0;                // units taken
+        int st = 0, phase = 0;     // of the next unit
         int seen[2] = {0, 0};      // tiles of each row tile
         int segs[2] = {0, 0};
         int tile_no = 0;
         bool ok = true;
-        auto wait = [&](uint64_t* bar, int phase) {
-          ok = ok && mbar_wait_bounded(bar, phase & 1, abort_flag, kTimeoutNs);
+        auto wait = [&](uint64_t* bar, int parity) {
+          ok = ok && mbar_wait_bounded(bar, parity & 1, abort_flag, kTimeoutNs);
           return ok;
         };
-        auto wait_unit = [&](int unit) {
-          return wait(&bars->kv_full[unit % C::kStages], unit / C::kStages);
+        auto next_unit = [&]() {
+          if (++st == C::kStages) {
+            st = 0;
+            phase ^= 1;
+          }
         };
-        for (Walk<D> w(p, w0, w1, start_b, start_w); ok && w.valid(); w.next()) {
-          const int nt = w.two() ? 2 : 1;
-          const int n = w.s.n;
+        for (int seg = 0; ok; ++seg) {
+          if (!wait(&bars->seg_full[seg % kSegs], seg / kSegs)) break;
+          const int n = bars->segs[seg % kSegs].n;
+          const int nt = has_two<D>(p, bars->segs[seg % kSegs].rb) ? 2 : 1;
+          mbar_arrive(&bars->seg_empty[seg % kSegs]);
+          if (n == 0) break;
           for (int t = 0; t < nt; ++t) wait(&bars->q_full[t], segs[t]++);
-          if (!wait_unit(it)) break;
+          if (!wait(&bars->kv_full[st], phase)) break;
           tc_fence_after();
-          for (int t = 0; t < nt; ++t) issue_qk(t, it % C::kStages);
-          mma_commit(&bars->kv_empty[it % C::kStages]);
-          ++it;
+          for (int t = 0; t < nt; ++t) issue_qk(t, st);
+          mma_commit(&bars->kv_empty[st]);
+          next_unit();
           for (int j = 0; j < n; ++j) {
-            if (!wait_unit(it)) break;
-            const int st_v = it++ % C::kStages;
+            if (!wait(&bars->kv_full[st], phase)) break;
+            const int st_v = st;
+            next_unit();
             const bool more = j + 1 < n;
-            const int unit_k = it;
             for (int t = 0; t < nt; ++t) {
               if (!wait(&bars->p_full[t], seen[t]++)) break;
               tc_fence_after();
               issue_pv(t, st_v, j > 0);
               if (t == nt - 1) mma_commit(&bars->kv_empty[st_v]);
               if (more) {
-                if (t == 0 && !wait_unit(unit_k)) break;
+                if (t == 0 && !wait(&bars->kv_full[st], phase)) break;
                 tc_fence_after();
-                issue_qk(t, unit_k % C::kStages);
-                if (t == nt - 1) mma_commit(&bars->kv_empty[unit_k % C::kStages]);
+                issue_qk(t, st);
+                if (t == nt - 1) mma_commit(&bars->kv_empty[st]);
               } else {
                 mma_commit(&bars->o_final[t]);
               }
@@ -311,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             if (!ok) break;
             // Softmax has taken this tile's scales and the converters its pages.
             mbar_arrive(&bars->meta_empty[tile_no++ % kMeta]);
-            if (more) ++it;
+            if (more) next_unit();
           }
         }
         if (!ok && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_MMA, abort_flag);
@@ -327,34 +353,54 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       // Lane i < 8: block i of 16 keys of a tile. Page ids are fetched two tiles and scales one
       // tile before they are published.
       if (has_run) {
-        Walk<D> w(p, w0, w1, start_b, start_w);
-        int j = 0, seg = 0;
-        bool first = true;
-        struct Ahead {
-          int id, h;       // page id, -1: no key, -2: outside the cache
-          bool first;
-          int seg;
+        const int64_t before = start->w;
+        Walk<D> w(p, w0, w1, start->b, before);
+        __syncwarp();  // `start` may be written over
+        bool ok = true;
+        int seg = 0, j = 0;
+        auto wait = [&](uint64_t* bar, int parity) {
+          ok = mbar_wait_bounded(bar, parity & 1, abort_flag, kTimeoutNs);
+          ok = __all_sync(0xffffffffu, ok);
+          return ok;
         };
-        auto next_ids = [&](Ahead& a) {  // of the next tile of the run, and on
-          a.id = -1;
-          a.first = first;
-          a.seg = seg;
-          if (!w.valid()) return false;
+        auto publish_segment = [&](bool over) {
+          const int slot = seg % kSegs;
+          if (!wait(&bars->seg_empty[slot], (seg / kSegs) ^ 1)) return;
+          if (lane == 0) {
+            Segment& to = bars->segs[slot];
+            to = w.s;
+            if (over) to.n = 0;
+            else to.first_run = static_cast<int>(run_of(w.at - w.s.t0, sc.total, parts));
+            bars->any_nan[slot] = 0;
+          }
+          for (int d = lane; d < D; d += 32) nan_key[slot * D + d] = 0x7fffffff;
+          mbar_arrive(&bars->seg_full[slot]);
+          ++seg;
+        };
+        struct Ahead {
+          int id;       // page id, -1: no key, -2: outside the cache
+          int h;
+          Tile tile;    // length -1: none
+        };
+        bool more = true;
+        auto next_tile = [&]() {  // of the run, and on; its segment is published first
+          Ahead a{-1, 0, {0, -1, 0, 0}};
+          if (!more) return a;
+          if (j == 0) publish_segment(false);
+          if (!ok) return a;
           a.h = w.s.h;
-          const int key = (w.s.t0 + j) * kTileKeys + lane * 16;
-          if (lane < kGroups && key < w.e.length) {
+          a.tile = Tile{(w.s.t0 + j) * kTileKeys, w.s.length, w.s.safe, seg - 1};
+          const int key = a.tile.key0 + lane * 16;
+          if (lane < kGroups && key < w.s.length) {
             a.id = p.table[w.s.b * p.table_stride + (key >> p.page_shift)];
             if (static_cast<unsigned>(a.id) >= static_cast<unsigned>(p.num_pages)) a.id = -2;
           }
-          first = ++j == w.s.n;
-          if (first) {
+          if (++j == w.s.n) {
             j = 0;
-            ++seg;
-            w.next();
+            more = w.next();
           }
-          return true;
+          return a;
         };
-        Ahead a0, a1;
         float ks = 1.f, vs = 1.f;
         auto fetch_scales = [&](const Ahead& a) {
           if (a.id >= 0) {
@@ -363,10 +409,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             vs = p.scale[1][plane];
           }
         };
-        bool have0 = next_ids(a0), have1 = next_ids(a1);
+        Ahead a0 = next_tile();
+        Ahead a1 = next_tile();
         fetch_scales(a0);
-        bool ok = true;
-        for (int n = 0; ok && have0; ++n) {
+        for (int n = 0; ok; ++n) {
           Meta m{-1, 1.f, -INFINITY, 0.f};
           if (a0.id >= 0) {
             const int ev = stored_exponent(__float_as_uint(vs));
@@ -374,21 +420,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           } else if (a0.id == -2 && p.status) {
             atomicOr(p.status, TA_DEVSTAT_BAD_PAGE);
           }
-          const Ahead now = a0;
+          const Tile now = a0.tile;
           a0 = a1;
-          have0 = have1;
-          have1 = next_ids(a1);
+          if (ok && now.length >= 0) a1 = next_tile();
           fetch_scales(a0);
-          ok = mbar_wait_bounded(&bars->meta_empty[n % kMeta], ((n / kMeta) & 1) ^ 1, abort_flag, kTimeoutNs);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (now.first) {  // a segment's first tile: no NaN noted yet
-            for (int d = lane; d < D; d += 32) nan_key[(now.seg % kNan) * D + d] = 0x7fffffff;
-            if (lane == 0) bars->any_nan[now.seg % kNan] = 0;
-          }
+          if (!ok || !wait(&bars->meta_empty[n % kMeta], (n / kMeta) ^ 1)) break;
           if (lane < kGroups) meta[(n % kMeta) * kGroups + lane] = m;
+          if (lane == 0) bars->tiles[n % kMeta] = now;
           mbar_arrive(&bars->meta_full[n % kMeta]);
+          if (now.length < 0) break;
         }
+        if (ok) publish_segment(true);
         if (!ok && lane == 0 && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_LOAD, abort_flag);
       }
     } else {
@@ -430,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       const bool real = c * 16 < p.D;
       uint8_t* const store = kv_smem + (c >> 2) * (kTileKeys * 128);  // 64 dims: 128 bytes a key
       bool ok = true;
-      int it = 0, tile_no = 0, seg = 0;
+      int st = 0, phase = 0;  // of the next unit
 
       // Codes of pass i of a unit: kind 0 K, 1 V, of the tile in meta slot `slot` whose first key is
       // key0, of a sequence of `length` keys. Rows without a key read as zeros.
@@ -448,48 +490,32 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         return mbar_wait_bounded(&bars->meta_full[n % kMeta], (n / kMeta) & 1, abort_flag, kTimeoutNs);
       };
 
-      Walk<D> w(p, w0, w1, start_b, start_w);
       uint4 held[kHeld];
       ok = wait_meta(0);
+      Tile now{0, -1, 0, 0};
       if (ok) {
+        now = bars->tiles[0];
 #pragma unroll
         for (int i = 0; i < kHeld; ++i)
-          held[i] = fetch(i % C::kChunks, i / C::kChunks, 0, w.s.t0 * kTileKeys, w.e.length);
+          held[i] = fetch(i % C::kChunks, i / C::kChunks, 0, now.key0, now.length);
       }
-      while (ok && w.valid()) {
-        const Segment s = w.s;
-        const int length = w.e.length;
-        // Keys that every row of the block with any keys sees: values beyond need care with NaN.
-        const int rows = min(p.group * p.T, (s.rb + 1) * C::kRows);
-        int safe = length;
-        if (p.causal) {
-          for (int tok = s.rb * C::kRows / p.group; tok <= (rows - 1) / p.group; ++tok) {
-            const int lim = row_limit(length, w.e.count, tok, 1);
-            if (lim > 0) {
-              safe = lim;
-              break;
-            }
-          }
-        }
-        w.next();
-        int* const nan_here = nan_key + (seg % kNan) * D;
-        int* const any_nan = &bars->any_nan[seg % kNan];
-        ++seg;
-        for (int j = 0; ok && j < s.n; ++j, ++tile_no) {
-          const int key0 = (s.t0 + j) * kTileKeys;
-          const bool edge = key0 + kTileKeys > safe;
-          const bool last_tile = j + 1 == s.n;
+      {
+        int tile_no = 0;
+        while (ok && now.length >= 0) {
+          const int key0 = now.key0, length = now.length;
+          const bool edge = key0 + kTileKeys > now.safe;  // values that some row does not see
+          int* const nan_here = nan_key + now.seg % kSegs * D;
+          int* const any_nan = &bars->any_nan[now.seg % kSegs];
           const int slot = tile_no % kMeta, next_slot = (tile_no + 1) % kMeta;
-          const int next_key0 = last_tile ? w.s.t0 * kTileKeys : key0 + kTileKeys;
-          const int next_length = last_tile ? (w.valid() ? w.e.length : 0) : length;
-          if (next_length > 0) ok = wait_meta(tile_no + 1);
+          ok = wait_meta(tile_no + 1);
+          if (!ok) break;
+          now = bars->tiles[next_slot];
+          const int next_key0 = now.key0, next_length = now.length;
+          ++tile_no;
 #pragma unroll
           for (int kind = 0; kind < 2; ++kind) {
-            const int st = it % C::kStages;
-            ok = ok && mbar_wait_bounded(&bars->kv_empty[st], ((it / C::kStages) & 1) ^ 1, abort_flag,
-                                         kTimeoutNs);
+            ok = ok && mbar_wait_bounded(&bars->kv_empty[st], phase ^ 1, abort_flag, kTimeoutNs);
             if (!ok) break;
-            ++it;
             uint8_t* const dst = store + st * C::kTileBytes;
 #pragma unroll
             for (int i = 0; i < C::kChunks; ++i) {
@@ -529,6 +555,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             }
             fence_proxy_async_shared();
             mbar_arrive(&bars->kv_full[st]);
+            if (++st == C::kStages) {
+              st = 0;
+              phase ^= 1;
+            }
           }
         }
       }
@@ -546,18 +576,27 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       const uint32_t t_o = tmem + lane_bits + 256 + t * D;
       const int rows = p.group * p.T;
       bool ok = true;
-      int tile_no = 0, seen = 0, segs = 0, seg = 0;
-      for (Walk<D> w(p, w0, w1, start_b, start_w); ok && w.valid(); w.next()) {
-        const Segment s = w.s;
-        const int nan_slot = seg++ % kNan;
-        if (t == 1 && !w.two()) {
+      int tile_no = 0, seen = 0, segs = 0;
+      for (int seg = 0; ok; ++seg) {
+        const int seg_slot = seg % kSegs;
+        ok = mbar_wait_bounded(&bars->seg_full[seg_slot], (seg / kSegs) & 1, abort_flag, kTimeoutNs);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          if (lane == 0 && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_SOFTMAX, abort_flag);
+          break;
+        }
+        const Segment s = bars->segs[seg_slot];
+        if (s.n == 0) break;
+        if (t == 1 && !has_two<D>(p, s.rb)) {
           tile_no += s.n;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->seg_empty[seg_slot]);
           continue;
         }
         const int row = s.rb * C::kRows + t * kTileRows + r_in_tile;
         const int tok = row / p.group, hd = s.h * p.group + (row - tok * p.group);
-        const bool real = row < rows && tok < w.e.count;
-        const int lim = real ? row_limit(w.e.length, w.e.count, tok, p.causal) : 0;
+        const bool real = row < rows && tok < s.count;
+        const int lim = real ? row_limit(s.length, s.count, tok, p.causal) : 0;
         const int safe = __reduce_min_sync(0xffffffffu, lim > 0 ? lim : 0x7fffffff);
 
         // The row of q times a power of two, with its largest value in [2^14, 2^15), as fp16.
@@ -733,8 +772,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
                              t * kTileRows + r_in_tile;
         uint16_t* out = static_cast<uint16_t*>(p.o) + s.b * p.o_sb + static_cast<int64_t>(hd) * p.o_sh +
                         static_cast<int64_t>(tok) * p.o_ss;
-        const bool any_nan = *static_cast<volatile int*>(&bars->any_nan[nan_slot]) != 0;
-        const int* nan_here = nan_key + nan_slot * D;
+        const bool any_nan = *static_cast<volatile int*>(&bars->any_nan[seg_slot]) != 0;
+        const int* nan_here = nan_key + seg_slot * D;
 #pragma unroll
         for (int cc = 0; cc < D / 32; ++cc) {
           uint32_t o[32];
@@ -778,11 +817,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         }
         // The run that ends a cut block leaves its merge's address.
         if (t == 0 && threadIdx.x == 0 && s.t0 > 0 && s.t0 + s.n == s.tiles) {
-          p.cuts[blockIdx.x] =
-              Cut{s.b, s.h, s.rb, static_cast<int>(run_of(w.at - s.t0, sc.total, parts))};
+          p.cuts[blockIdx.x] = Cut{s.b, s.h, s.rb, s.first_run};
         }
         // The next block's MMAs write the accumulator that was just read.
         tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->seg_empty[seg_slot]);
       }
     }
   }
