@@ -38,6 +38,7 @@ namespace chunk {
 namespace {
 
 constexpr int kTileRows = 128, kTileKeys = 128;
+constexpr int kHalfKeys = kTileKeys / 2;  // keys of a score half
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 // Register split of the launch's 512 x 128 registers: softmax, converters, MMA and idle.
@@ -62,16 +63,16 @@ struct Cfg {
   static constexpr int kQOff = 0;
   static constexpr int kKvOff = kTiles * kTileBytes;
   static constexpr int kMetaOff = kKvOff + kStages * kTileBytes;
-  static constexpr int kNanOff = kMetaOff + kMeta * kGroups * 16;
+  static constexpr int kNanOff = kMetaOff + kMeta * kGroups * (16 + 8);
   static constexpr int kBarOff = kNanOff + kSegs * D * 4;
   static constexpr int kBytes = kBarOff + 1024 + 1024;  // slack: 1024-byte alignment
 };
 
-struct Meta {  // of 16 keys: where they are, and their scales in softmax's terms
-  int plane;   // page * Hkv + head, or -1: no key here, or a page outside the cache
-  float ks;    // scale of K
-  float e;     // exponent of V's scale; -inf where plane is -1: such keys have no weight
-  float back;  // 2^-e
+struct Meta {   // of 16 keys: their scales in softmax's terms
+  float ks;     // scale of K
+  float e;      // exponent of V's scale; -inf where there is no key: such keys have no weight
+  float back;   // 2^-e
+  int unused;
 };
 
 // A key tile on the line, as the converters need it; length -1: the run is over.
@@ -90,7 +91,7 @@ struct Segment {
 };
 
 struct Barriers {
-  uint64_t q_full[2], s_full[2], p_full[2], o_final[2];
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2];  // [row tile][half]
   uint64_t drain;
   uint64_t kv_full[6], kv_empty[6], meta_full[kMeta], meta_empty[kMeta], seg_full[kSegs], seg_empty[kSegs];
   Segment segs[kSegs];
@@ -175,6 +176,10 @@ __device__ __forceinline__ void report(const AttendParams& p, uint32_t code, vol
   if (p.status) atomicOr(p.status, code);
 }
 
+__device__ __forceinline__ void st_shared128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w));
+}
+
 __device__ __forceinline__ void sts128(void* a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   *reinterpret_cast<uint4*>(a) = make_uint4(x, y, z, w);
 }
@@ -197,6 +202,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
   uint8_t* q_smem = smem + C::kQOff;
   uint8_t* kv_smem = smem + C::kKvOff;
   Meta* meta = reinterpret_cast<Meta*>(smem + C::kMetaOff);
+  // Where 16 keys are: byte offset of the first one's codes * 32 + how many there are.
+  int64_t* place = reinterpret_cast<int64_t*>(meta + kMeta * kGroups);
   int* nan_key = reinterpret_cast<int*>(smem + C::kNanOff);  // [kSegs][D]
   Start* start = reinterpret_cast<Start*>(nan_key);
   Barriers* bars = reinterpret_cast<Barriers*>(smem + C::kBarOff);
@@ -206,9 +213,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(&bars->q_full[t], kTileRows);
-      mbar_init(&bars->s_full[t], 1);
-      mbar_init(&bars->p_full[t], kTileRows);
-      mbar_init(&bars->o_final[t], 1);
+      for (int half = 0; half < 2; ++half) {
+        mbar_init(&bars->s_full[t][half], 1);
+        mbar_init(&bars->p_full[t][half], kTileRows);
+      }
+      mbar_init(&bars->pv_done[t], 1);
     }
     mbar_init(&bars->drain, 1);
     for (int s = 0; s < C::kStages; ++s) {
@@ -264,32 +273,38 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
     if (warp == 12) {
       // ------------------------------------------------------------ MMA issuer
       if (lane == 0 && has_run) {
-        constexpr uint32_t kIdescQK = idesc_f16(kTileRows, kTileKeys, false, false, false);
+        constexpr uint32_t kIdescQK = idesc_f16(kTileRows, kHalfKeys, false, false, false);
         constexpr uint32_t kIdescPV = idesc_f16(kTileRows, D, false, false, true);
         const uint64_t q_desc = sdesc_sw128(smem_u32(q_smem), 16, 1024);
         const uint64_t kv_desc_k = sdesc_sw128(smem_u32(kv_smem), 16, 1024);
         const uint64_t kv_desc_v = sdesc_sw128(smem_u32(kv_smem), kTileKeys * 128, 1024);
-        auto issue_qk = [&](int t, int st) {
+        // Scores of one half of a tile's keys for row tile t. Halves: a tile's columns of tensor
+        // memory hold two of 64, so the next tile's first half is computed while softmax works on
+        // this one's second, where a whole tile would leave one of the two idle in turn.
+        auto issue_qk = [&](int t, int st, int half) {
           const uint64_t qd = q_desc + static_cast<uint64_t>((t * C::kTileBytes) >> 4);
-          const uint64_t kd = kv_desc_k + static_cast<uint64_t>((st * C::kTileBytes) >> 4);
+          const uint64_t kd =
+              kv_desc_k + static_cast<uint64_t>((st * C::kTileBytes + half * (kHalfKeys * 128)) >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint64_t off =
                 static_cast<uint64_t>(((kk >> 2) * (kTileRows * 128) + (kk & 3) * 32) >> 4);
-            mma_ss(tmem + t * 128, qd + off, kd + off, kIdescQK, kk > 0 ? 1u : 0u);
+            mma_ss(tmem + t * 128 + half * kHalfKeys, qd + off, kd + off, kIdescQK, kk > 0 ? 1u : 0u);
           }
-          mma_commit(&bars->s_full[t]);
+          mma_commit(&bars->s_full[t][half]);
         };
-        auto issue_pv = [&](int t, int st, bool acc) {
-          const uint64_t vd = kv_desc_v + static_cast<uint64_t>((st * C::kTileBytes) >> 4);
+        auto issue_pv = [&](int t, int st, int half, bool acc) {
+          const uint64_t vd =
+              kv_desc_v + static_cast<uint64_t>((st * C::kTileBytes + half * (kHalfKeys * 128)) >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kTileKeys / 16; ++kk)
-            mma_ts(tmem + 256 + t * D, tmem + t * 128 + kk * 8,
+          for (int kk = 0; kk < kHalfKeys / 16; ++kk)
+            mma_ts(tmem + 256 + t * D, tmem + t * 128 + half * kHalfKeys + kk * 8,
                    vd + static_cast<uint64_t>((kk * 16 * 128) >> 4), kIdescPV,
                    (acc || kk > 0) ? 1u : 0u);
+          mma_commit(&bars->pv_done[t]);
         };
         int st = 0, phase = 0;     // of the next unit
-        int seen[2] = {0, 0};      // tiles of each row tile
+        int seen[2] = {0, 0};      // halves of each row tile
         int segs[2] = {0, 0};
         int tile_no = 0;
         bool ok = true;
@@ -312,7 +327,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           for (int t = 0; t < nt; ++t) wait(&bars->q_full[t], segs[t]++);
           if (!wait(&bars->kv_full[st], phase)) break;
           tc_fence_after();
-          for (int t = 0; t < nt; ++t) issue_qk(t, st);
+          for (int half = 0; half < 2; ++half)
+            for (int t = 0; t < nt; ++t) issue_qk(t, st, half);
           mma_commit(&bars->kv_empty[st]);
           next_unit();
           for (int j = 0; j < n; ++j) {
@@ -320,20 +336,21 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             const int st_v = st;
             next_unit();
             const bool more = j + 1 < n;
-            for (int t = 0; t < nt; ++t) {
-              if (!wait(&bars->p_full[t], seen[t]++)) break;
-              tc_fence_after();
-              issue_pv(t, st_v, j > 0);
-              if (t == nt - 1) mma_commit(&bars->kv_empty[st_v]);
-              if (more) {
-                if (t == 0 && !wait(&bars->kv_full[st], phase)) break;
+            for (int half = 0; ok && half < 2; ++half)
+              for (int t = 0; t < nt; ++t) {
+                if (!wait(&bars->p_full[t][half], seen[t] >> 1)) break;
+                ++seen[t];
                 tc_fence_after();
-                issue_qk(t, st);
-                if (t == nt - 1) mma_commit(&bars->kv_empty[st]);
-              } else {
-                mma_commit(&bars->o_final[t]);
+                issue_pv(t, st_v, half, j > 0 || half > 0);
+                const bool last = half == 1 && t == nt - 1;
+                if (last) mma_commit(&bars->kv_empty[st_v]);
+                if (more) {
+                  if (half == 0 && t == 0 && !wait(&bars->kv_full[st], phase)) break;
+                  tc_fence_after();
+                  issue_qk(t, st, half);
+                  if (last) mma_commit(&bars->kv_empty[st]);
+                }
               }
-            }
             if (!ok) break;
             // Softmax has taken this tile's scales and the converters its pages.
             mbar_arrive(&bars->meta_empty[tile_no++ % kMeta]);
@@ -413,10 +430,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         Ahead a1 = next_tile();
         fetch_scales(a0);
         for (int n = 0; ok; ++n) {
-          Meta m{-1, 1.f, -INFINITY, 0.f};
+          Meta m{1.f, -INFINITY, 0.f, 0};
+          int64_t at = 0;
           if (a0.id >= 0) {
             const int ev = stored_exponent(__float_as_uint(vs));
-            m = Meta{a0.id * p.Hkv + a0.h, ks, static_cast<float>(ev), pow2f(-ev)};
+            m = Meta{ks, static_cast<float>(ev), pow2f(-ev), 0};
+            const int key = a0.tile.key0 + lane * 16;
+            const int64_t row = (static_cast<int64_t>(a0.id) * p.Hkv + a0.h) * p.page + (key & (p.page - 1));
+            at = row * p.D * 32 + min(16, a0.tile.length - key);
           } else if (a0.id == -2 && p.status) {
             atomicOr(p.status, TA_DEVSTAT_BAD_PAGE);
           }
@@ -425,7 +446,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           if (ok && now.length >= 0) a1 = next_tile();
           fetch_scales(a0);
           if (!ok || !wait(&bars->meta_empty[n % kMeta], (n / kMeta) ^ 1)) break;
-          if (lane < kGroups) meta[(n % kMeta) * kGroups + lane] = m;
+          if (lane < kGroups) {
+            meta[(n % kMeta) * kGroups + lane] = m;
+            place[(n % kMeta) * kGroups + lane] = at;
+          }
           if (lane == 0) bars->tiles[n % kMeta] = now;
           mbar_arrive(&bars->meta_full[n % kMeta]);
           if (now.length < 0) break;
@@ -470,20 +494,34 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
                                                 : (lane >> 2) & 1;
       const int row0 = (warp - 8) * (kRowsPerPass / 4) + row_in_warp;
       const bool real = c * 16 < p.D;
-      uint8_t* const store = kv_smem + (c >> 2) * (kTileKeys * 128);  // 64 dims: 128 bytes a key
+      const uint32_t store = smem_u32(kv_smem) + (c >> 2) * (kTileKeys * 128);  // 64 dims: 128 bytes a key
+      // The thread's two 16-byte pieces of a row, swizzled; a pass's rows are 8 k apart or more.
+      const uint32_t piece0 = row0 * 128 + ((((2 * c) & 7) ^ (row0 & 7)) << 4);
+      const uint32_t piece1 = row0 * 128 + ((((2 * c + 1) & 7) ^ (row0 & 7)) << 4);
+      static_assert(kRowsPerPass % 8 == 0, "a pass keeps a row's swizzle");
+      constexpr int kPlaces = kRowsPerPass >= 16 ? C::kChunks : C::kChunks / 2;
+      const uint32_t places = smem_u32(place) + (kRowsPerPass > 16 ? row0 >> 4 : 0) * 8;
+      const int in_block = row0 & 15;
+      const uint8_t* const mine[2] = {p.pages[0] + in_block * p.D + c * 16,
+                                      p.pages[1] + in_block * p.D + c * 16};
       bool ok = true;
       int st = 0, phase = 0;  // of the next unit
 
-      // Codes of pass i of a unit: kind 0 K, 1 V, of the tile in meta slot `slot` whose first key is
-      // key0, of a sequence of `length` keys. Rows without a key read as zeros.
-      auto fetch = [&](int i, int kind, int slot, int key0, int length) {
-        const int row = i * kRowsPerPass + row0;
-        const int plane = meta[slot * kGroups + (row >> 4)].plane;
+      int64_t at[kPlaces];  // of the tile whose codes are loaded next
+      auto read_places = [&](int slot) {
+#pragma unroll
+        for (int i = 0; i < kPlaces; ++i)
+          asm volatile("ld.shared.b64 %0, [%1];"
+                       : "=l"(at[i])
+                       : "r"(places + (slot * kGroups + i * (kRowsPerPass > 16 ? kRowsPerPass / 16 : 1)) * 8));
+      };
+      // Codes of pass i of a unit (kind 0 K, 1 V) of that tile. Rows without a key read as zeros.
+      auto fetch = [&](int i, int kind) {
+        const int64_t where = at[kRowsPerPass >= 16 ? i : i / 2];
+        const int row = in_block + (kRowsPerPass < 16 ? (i & 1) * kRowsPerPass : 0);
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (real && plane >= 0 && key0 + row < length)
-          v = __ldg(reinterpret_cast<const uint4*>(
-              p.pages[kind] +
-              (static_cast<int64_t>(plane) * p.page + ((key0 + row) & (p.page - 1))) * p.D + c * 16));
+        if (real && row < static_cast<int>(where & 31))
+          v = __ldg(reinterpret_cast<const uint4*>(mine[kind] + (where >> 5) + (row - in_block) * p.D));
         return v;
       };
       auto wait_meta = [&](int n) {
@@ -495,70 +533,63 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       Tile now{0, -1, 0, 0};
       if (ok) {
         now = bars->tiles[0];
+        read_places(0);
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i)
-          held[i] = fetch(i % C::kChunks, i / C::kChunks, 0, now.key0, now.length);
+        for (int i = 0; i < kHeld; ++i) held[i] = fetch(i % C::kChunks, i / C::kChunks);
       }
-      {
-        int tile_no = 0;
-        while (ok && now.length >= 0) {
-          const int key0 = now.key0, length = now.length;
-          const bool edge = key0 + kTileKeys > now.safe;  // values that some row does not see
-          int* const nan_here = nan_key + now.seg % kSegs * D;
-          int* const any_nan = &bars->any_nan[now.seg % kSegs];
-          const int slot = tile_no % kMeta, next_slot = (tile_no + 1) % kMeta;
-          ok = wait_meta(tile_no + 1);
+      for (int tile_no = 1; ok && now.length >= 0; ++tile_no) {
+        const int key0 = now.key0;
+        const bool edge = key0 + kTileKeys > now.safe;  // values that some row does not see
+        int* const nan_here = nan_key + now.seg % kSegs * D;
+        int* const any_nan = &bars->any_nan[now.seg % kSegs];
+        ok = wait_meta(tile_no);  // the next tile's pages
+        if (!ok) break;
+        now = bars->tiles[tile_no % kMeta];
+        if (kWholeTile) read_places(tile_no % kMeta);
+#pragma unroll
+        for (int kind = 0; kind < 2; ++kind) {
+          if (!kWholeTile && kind == 1) read_places(tile_no % kMeta);
+          ok = ok && mbar_wait_bounded(&bars->kv_empty[st], phase ^ 1, abort_flag, kTimeoutNs);
           if (!ok) break;
-          now = bars->tiles[next_slot];
-          const int next_key0 = now.key0, next_length = now.length;
-          ++tile_no;
+          const uint32_t dst = store + st * C::kTileBytes;
 #pragma unroll
-          for (int kind = 0; kind < 2; ++kind) {
-            ok = ok && mbar_wait_bounded(&bars->kv_empty[st], phase ^ 1, abort_flag, kTimeoutNs);
-            if (!ok) break;
-            uint8_t* const dst = store + st * C::kTileBytes;
-#pragma unroll
-            for (int i = 0; i < C::kChunks; ++i) {
-              const int row = i * kRowsPerPass + row0;
-              uint4& h = held[kWholeTile ? kind * C::kChunks + i : i];
-              uint4 v = h;
-              // the register's next load
-              if (kWholeTile) h = fetch(i, kind, next_slot, next_key0, next_length);
-              else if (kind == 0) h = fetch(i, 1, slot, key0, length);
-              else h = fetch(i, 0, next_slot, next_key0, next_length);
-              if (edge && kind == 1) {
-                uint32_t x[4] = {v.x, v.y, v.z, v.w};
-                if ((nan_bits(x[0]) | nan_bits(x[1]) | nan_bits(x[2]) | nan_bits(x[3])) != 0) {
-                  *any_nan = 1;
+          for (int i = 0; i < C::kChunks; ++i) {
+            uint4 v = held[kWholeTile ? kind * C::kChunks + i : i];
+            if (edge && kind == 1) {
+              if ((nan_bits(v.x) | nan_bits(v.y) | nan_bits(v.z) | nan_bits(v.w)) != 0) {
+                *any_nan = 1;
 #pragma unroll 1
-                  for (int k = 0; k < 4; ++k) {
-                    uint32_t y = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w;
-                    for (int b = 0; b < 4; ++b)
-                      if ((y >> (8 * b) & 0x7fu) == 0x7fu)
-                        atomicMin(nan_here + c * 16 + k * 4 + b, key0 + row);
-                    y &= ~((nan_bits(y) >> 7) * 0xffu);
-                    if (k == 0) v.x = y;
-                    else if (k == 1) v.y = y;
-                    else if (k == 2) v.z = y;
-                    else v.w = y;
-                  }
+                for (int k = 0; k < 4; ++k) {
+                  uint32_t y = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w;
+                  for (int b = 0; b < 4; ++b)
+                    if ((y >> (8 * b) & 0x7fu) == 0x7fu)
+                      atomicMin(nan_here + c * 16 + k * 4 + b, key0 + i * kRowsPerPass + row0);
+                  y &= ~((nan_bits(y) >> 7) * 0xffu);
+                  if (k == 0) v.x = y;
+                  else if (k == 1) v.y = y;
+                  else if (k == 2) v.z = y;
+                  else v.w = y;
                 }
               }
-              uint32_t f[8];
-              codes_to_f16(v.x, f[0], f[1]);
-              codes_to_f16(v.y, f[2], f[3]);
-              codes_to_f16(v.z, f[4], f[5]);
-              codes_to_f16(v.w, f[6], f[7]);
-              uint8_t* const at = dst + row * 128;
-              sts128(at + (((2 * c) & 7) ^ (row & 7)) * 16, f[0], f[1], f[2], f[3]);
-              sts128(at + (((2 * c + 1) & 7) ^ (row & 7)) * 16, f[4], f[5], f[6], f[7]);
             }
-            fence_proxy_async_shared();
-            mbar_arrive(&bars->kv_full[st]);
-            if (++st == C::kStages) {
-              st = 0;
-              phase ^= 1;
-            }
+            uint32_t f[8];
+            codes_to_f16(v.x, f[0], f[1]);
+            codes_to_f16(v.y, f[2], f[3]);
+            codes_to_f16(v.z, f[4], f[5]);
+            codes_to_f16(v.w, f[6], f[7]);
+            st_shared128(dst + i * (kRowsPerPass * 128) + piece0, f[0], f[1], f[2], f[3]);
+            st_shared128(dst + i * (kRowsPerPass * 128) + piece1, f[4], f[5], f[6], f[7]);
+          }
+          fence_proxy_async_shared();
+          mbar_arrive(&bars->kv_full[st]);
+          // The registers' next loads: the next tile's, or at head dim 256 the next unit's. All in one
+          // burst: a load issued between the uses of others makes those uses wait for it too.
+#pragma unroll
+          for (int i = 0; i < C::kChunks; ++i)
+            held[kWholeTile ? kind * C::kChunks + i : i] = fetch(i, kWholeTile ? kind : kind ^ 1);
+          if (++st == C::kStages) {
+            st = 0;
+            phase ^= 1;
           }
         }
       }
@@ -576,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       const uint32_t t_o = tmem + lane_bits + 256 + t * D;
       const int rows = p.group * p.T;
       bool ok = true;
-      int tile_no = 0, seen = 0, segs = 0;
+      int tile_no = 0, seen = 0;  // tiles of the run, halves of this row tile
       for (int seg = 0; ok; ++seg) {
         const int seg_slot = seg % kSegs;
         ok = mbar_wait_bounded(&bars->seg_full[seg_slot], (seg / kSegs) & 1, abort_flag, kTimeoutNs);
@@ -640,44 +671,39 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         }
 
         float ref = -INFINITY, l_run = 0.f;
-        for (int j = 0; j < s.n; ++j, ++tile_no, ++seen) {
+        for (int j2 = 0; j2 < 2 * s.n; ++j2, ++seen) {
+          const int half = j2 & 1;
           const int slot = tile_no % kMeta;
-          ok = mbar_wait_bounded(&bars->meta_full[slot], (tile_no / kMeta) & 1, abort_flag, kTimeoutNs) &&
-               mbar_wait_bounded(&bars->s_full[t], seen & 1, abort_flag, kTimeoutNs);
+          if (half == 0)
+            ok = mbar_wait_bounded(&bars->meta_full[slot], (tile_no / kMeta) & 1, abort_flag, kTimeoutNs);
+          ok = ok && mbar_wait_bounded(&bars->s_full[t][half], (seen >> 1) & 1, abort_flag, kTimeoutNs);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
-          // Two passes over the scores, 32 columns in registers at a time (reading tensor memory
-          // twice costs less than holding 128 scores).
-          const int key0 = (s.t0 + j) * kTileKeys;
-          const int visible = key0 + kTileKeys > safe ? lim - key0 : kTileKeys;  // of this tile's
-          const bool edge = key0 + kTileKeys > safe;
-          const Meta* m = meta + slot * kGroups;
+          uint32_t x[64];
+          tmem_ld64(t_s + half * kHalfKeys, *reinterpret_cast<uint32_t(*)[32]>(x),
+                    *reinterpret_cast<uint32_t(*)[32]>(x + 32));
+          tmem_wait_ld();
+          const int key0 = (s.t0 + (j2 >> 1)) * kTileKeys + half * kHalfKeys;
+          if (key0 + kHalfKeys > safe) {
+            const int visible = lim - key0;
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (i >= visible) x[i] = 0xff800000u;
+          }
+          const Meta* m = meta + slot * kGroups + half * (kGroups / 2);
           // t = score * c + e, c held above zero so that a masked score stays -inf
           float cand = -INFINITY;
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            uint32_t y[32];
-            tmem_ld32(t_s + 32 * q4, y);
-            tmem_wait_ld();
-            if (edge) {
+          for (int g = 0; g < 4; ++g) {
+            float a = fmaxf(__uint_as_float(x[16 * g]), __uint_as_float(x[16 * g + 1]));
+            float b = fmaxf(__uint_as_float(x[16 * g + 2]), __uint_as_float(x[16 * g + 3]));
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (q4 * 32 + i >= visible) y[i] = 0xff800000u;
+            for (int i = 4; i < 16; i += 4) {
+              a = fmax3(a, __uint_as_float(x[16 * g + i]), __uint_as_float(x[16 * g + i + 1]));
+              b = fmax3(b, __uint_as_float(x[16 * g + i + 2]), __uint_as_float(x[16 * g + i + 3]));
             }
-#pragma unroll
-            for (int gg = 0; gg < 2; ++gg) {
-              const uint32_t* x = y + 16 * gg;
-              float a = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-              float b = fmaxf(__uint_as_float(x[2]), __uint_as_float(x[3]));
-#pragma unroll
-              for (int i = 4; i < 16; i += 4) {
-                a = fmax3(a, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-                b = fmax3(b, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
-              }
-              const int g = q4 * 2 + gg;
-              cand = fmaxf(cand, fmaf(fmaxf(a, b), fmaxf(mul * m[g].ks, 1e-37f), m[g].e));
-            }
+            cand = fmaxf(cand, fmaf(fmaxf(a, b), fmaxf(mul * m[g].ks, 1e-37f), m[g].e));
           }
           const bool grow = cand > ref + kGrowth;
           if (__any_sync(0xffffffffu, grow)) {
@@ -687,7 +713,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
               ref = cand - kBelow;
               l_run *= alpha;
             }
-            if (j > 0) {
+            if (j2 > 0) {
+              // The product of the half before may still be adding to the output (that of the half
+              // before it cannot: these scores were issued behind it, or are a block's first).
+              ok = mbar_wait_bounded(&bars->pv_done[t], (seen - 1) & 1, abort_flag, kTimeoutNs);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              tc_fence_after();
               const uint64_t alpha2 = f2_pack(alpha, alpha);
 #pragma unroll
               for (int cc = 0; cc < D / 32; ++cc) {
@@ -706,58 +738,41 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
               }
             }
           }
-          // The weights (16-bit, two a column) go over the first 64 columns: the second pass reads
-          // ahead of them.
+          // The weights (16-bit, two a column) go over the first 32 of the half's columns.
           const float r = ref == -INFINITY ? 0.f : ref;
-          uint32_t pk[32], y[32];
-          tmem_ld32(t_s, y);
+          uint32_t pk[32];
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            tmem_wait_ld();
-            reg_fence32(y);
-            if (edge) {
+          for (int g = 0; g < 4; ++g) {
+            const float cs = fmaxf(mul * m[g].ks, 1e-37f), sh = m[g].e - r;
+            const uint64_t c2 = f2_pack(cs, cs), s2 = f2_pack(sh, sh);
+            uint64_t sum = f2_pack(0.f, 0.f);
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (q4 * 32 + i >= visible) y[i] = 0xff800000u;
+            for (int i = 0; i < 8; ++i) {
+              float a0, a1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(x[16 * g + 2 * i]),
+                                       __uint_as_float(x[16 * g + 2 * i + 1])), c2, s2), a0, a1);
+              a0 = ex2_approx(a0);
+              a1 = ex2_approx(a1);
+              pk[g * 8 + i] = pack_f16(a0, a1);
+              sum = f2_add(sum, f2_pack(a0, a1));
             }
-#pragma unroll
-            for (int gg = 0; gg < 2; ++gg) {
-              const int g = q4 * 2 + gg;
-              const float cs = fmaxf(mul * m[g].ks, 1e-37f), sh = m[g].e - r;
-              const uint64_t c2 = f2_pack(cs, cs), s2 = f2_pack(sh, sh);
-              uint64_t sum = f2_pack(0.f, 0.f);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                float a0, a1;
-                f2_unpack(f2_fma(f2_pack(__uint_as_float(y[16 * gg + 2 * i]),
-                                         __uint_as_float(y[16 * gg + 2 * i + 1])), c2, s2), a0, a1);
-                a0 = ex2_approx(a0);
-                a1 = ex2_approx(a1);
-                pk[(q4 & 1) * 16 + gg * 8 + i] = pack_f16(a0, a1);
-                sum = f2_add(sum, f2_pack(a0, a1));
-              }
-              float s0, s1;
-              f2_unpack(sum, s0, s1);
-              l_run = fmaf(s0 + s1, m[g].back, l_run);
-            }
-            if (q4 < 3) tmem_ld32(t_s + 32 * (q4 + 1), y);
-            // columns 0-31 are written once 0-63 have been read, 32-63 at the end
-            if (q4 == 1) tmem_st32(t_s, pk);
-            if (q4 == 3) tmem_st32(t_s + 32, pk);
+            float s0, s1;
+            f2_unpack(sum, s0, s1);
+            l_run = fmaf(s0 + s1, m[g].back, l_run);
           }
+          tmem_st32(t_s + half * kHalfKeys, pk);
           tmem_wait_st();
           tc_fence_before();
-          mbar_arrive(&bars->p_full[t]);
+          mbar_arrive(&bars->p_full[t][half]);
+          tile_no += half;
+        }
+        if (ok) {  // the last two products, one by one: a parity tells neighbouring phases apart only
+          ok = mbar_wait_bounded(&bars->pv_done[t], seen & 1, abort_flag, kTimeoutNs) &&
+               mbar_wait_bounded(&bars->pv_done[t], (seen - 1) & 1, abort_flag, kTimeoutNs);
+          ok = __all_sync(0xffffffffu, ok);
         }
         if (!ok) {
           if (lane == 0 && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_SOFTMAX, abort_flag);
-          break;
-        }
-        ok = mbar_wait_bounded(&bars->o_final[t], segs & 1, abort_flag, kTimeoutNs);
-        ++segs;
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) {
-          if (lane == 0 && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_EPILOG, abort_flag);
           break;
         }
         tc_fence_after();
