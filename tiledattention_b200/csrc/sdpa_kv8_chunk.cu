@@ -30,6 +30,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <utility>
+
 #include "kv8_device.cuh"
 
 namespace ta {
@@ -91,7 +93,7 @@ struct Segment {
 };
 
 struct Barriers {
-  uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2];  // [row tile][half]
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], o_final[2][2];  // [row tile][half]
   uint64_t drain;
   uint64_t kv_full[6], kv_empty[6], meta_full[kMeta], meta_empty[kMeta], seg_full[kSegs], seg_empty[kSegs];
   Segment segs[kSegs];
@@ -176,6 +178,23 @@ __device__ __forceinline__ void report(const AttendParams& p, uint32_t code, vol
   if (p.status) atomicOr(p.status, code);
 }
 
+// The MMAs of a product, descriptor steps as immediates: scores over D dims, 16 at a time (64 dims
+// are one 128-byte-wide part of a tile) ...
+template <int A, int B, int... kk>
+__device__ __forceinline__ void issue_qk_seq(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                             std::integer_sequence<int, kk...>) {
+  (mma_ss_imm<((A + (kk >> 2) * (kTileRows * 128) + (kk & 3) * 32) >> 4),
+              ((B + (kk >> 2) * (kTileKeys * 128) + (kk & 3) * 32) >> 4), (kk > 0 ? 1 : 0)>(d, a, b,
+                                                                                           idesc),
+   ...);
+}
+// ... and the output over keys, 16 at a time.
+template <int B, int... kk>
+__device__ __forceinline__ void issue_pv_seq(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                             uint32_t acc, std::integer_sequence<int, kk...>) {
+  (mma_ts_imm_acc<kk * 8, ((B + kk * 16 * 128) >> 4)>(d, a, b, idesc, kk == 0 ? acc : 1u), ...);
+}
+
 __device__ __forceinline__ void st_shared128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w));
 }
@@ -216,8 +235,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       for (int half = 0; half < 2; ++half) {
         mbar_init(&bars->s_full[t][half], 1);
         mbar_init(&bars->p_full[t][half], kTileRows);
+        mbar_init(&bars->o_final[t][half], 1);
       }
-      mbar_init(&bars->pv_done[t], 1);
     }
     mbar_init(&bars->drain, 1);
     for (int s = 0; s < C::kStages; ++s) {
@@ -278,40 +297,37 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         const uint64_t q_desc = sdesc_sw128(smem_u32(q_smem), 16, 1024);
         const uint64_t kv_desc_k = sdesc_sw128(smem_u32(kv_smem), 16, 1024);
         const uint64_t kv_desc_v = sdesc_sw128(smem_u32(kv_smem), kTileKeys * 128, 1024);
-        // Scores of one half of a tile's keys for row tile t. Halves: a tile's columns of tensor
-        // memory hold two of 64, so the next tile's first half is computed while softmax works on
-        // this one's second, where a whole tile would leave one of the two idle in turn.
-        auto issue_qk = [&](int t, int st, int half) {
-          const uint64_t qd = q_desc + static_cast<uint64_t>((t * C::kTileBytes) >> 4);
-          const uint64_t kd =
-              kv_desc_k + static_cast<uint64_t>((st * C::kTileBytes + half * (kHalfKeys * 128)) >> 4);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint64_t off =
-                static_cast<uint64_t>(((kk >> 2) * (kTileRows * 128) + (kk & 3) * 32) >> 4);
-            mma_ss(tmem + t * 128 + half * kHalfKeys, qd + off, kd + off, kIdescQK, kk > 0 ? 1u : 0u);
-          }
-          mma_commit(&bars->s_full[t][half]);
-        };
-        auto issue_pv = [&](int t, int st, int half, bool acc) {
-          const uint64_t vd =
-              kv_desc_v + static_cast<uint64_t>((st * C::kTileBytes + half * (kHalfKeys * 128)) >> 4);
-#pragma unroll
-          for (int kk = 0; kk < kHalfKeys / 16; ++kk)
-            mma_ts(tmem + 256 + t * D, tmem + t * 128 + half * kHalfKeys + kk * 8,
-                   vd + static_cast<uint64_t>((kk * 16 * 128) >> 4), kIdescPV,
-                   (acc || kk > 0) ? 1u : 0u);
-          mma_commit(&bars->pv_done[t]);
-        };
-        int st = 0, phase = 0;     // of the next unit
-        int seen[2] = {0, 0};      // halves of each row tile
-        int segs[2] = {0, 0};
-        int tile_no = 0;
+        const uint32_t unit = C::kTileBytes >> 4;  // in a descriptor's 16-byte steps
         bool ok = true;
-        auto wait = [&](uint64_t* bar, int parity) {
-          ok = ok && mbar_wait_bounded(bar, parity & 1, abort_flag, kTimeoutNs);
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+          if (!mbar_try_wait(smem_u32(bar), parity))
+            ok = ok && mbar_wait_bounded(bar, parity, abort_flag, kTimeoutNs);
+          tc_fence_after();
           return ok;
         };
+        // Scores of one half of a tile's keys for row tile t. Halves: a tile's columns of tensor
+        // memory hold two of 64, so the next tile's first half is computed while softmax works on
+        // this one's second, where a whole tile would leave one of the two idle in turn. This one
+        // thread issues everything, so its instructions count: descriptor steps are immediates
+        // and the halves and row tiles unrolled.
+        auto issue_qk = [&](auto t_, auto half_, uint32_t st) {
+          constexpr int t = decltype(t_)::value, half = decltype(half_)::value;
+          issue_qk_seq<t * C::kTileBytes, half * kHalfKeys * 128>(
+              tmem + t * 128 + half * kHalfKeys, q_desc, kv_desc_k + st * unit, kIdescQK,
+              std::make_integer_sequence<int, D / 16>());
+          mma_commit(&bars->s_full[t][half]);
+        };
+        auto issue_pv = [&](auto t_, auto half_, uint32_t st, uint32_t acc) {
+          constexpr int t = decltype(t_)::value, half = decltype(half_)::value;
+          issue_pv_seq<half * kHalfKeys * 128>(tmem + 256 + t * D, tmem + t * 128 + half * kHalfKeys,
+                                               kv_desc_v + st * unit, kIdescPV, acc,
+                                               std::make_integer_sequence<int, kHalfKeys / 16>());
+        };
+        constexpr std::integral_constant<int, 0> k0{};
+        constexpr std::integral_constant<int, 1> k1{};
+        uint32_t st = 0, phase = 0;  // of the next unit
+        uint32_t q_par[2] = {0, 0}, p_par[2] = {0, 0};  // parities of row tiles' segments, tiles
+        int tile_no = 0;
         auto next_unit = [&]() {
           if (++st == C::kStages) {
             st = 0;
@@ -319,38 +335,53 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           }
         };
         for (int seg = 0; ok; ++seg) {
-          if (!wait(&bars->seg_full[seg % kSegs], seg / kSegs)) break;
+          if (!wait(&bars->seg_full[seg % kSegs], (seg / kSegs) & 1)) break;
           const int n = bars->segs[seg % kSegs].n;
-          const int nt = has_two<D>(p, bars->segs[seg % kSegs].rb) ? 2 : 1;
+          const bool two = has_two<D>(p, bars->segs[seg % kSegs].rb);
           mbar_arrive(&bars->seg_empty[seg % kSegs]);
           if (n == 0) break;
-          for (int t = 0; t < nt; ++t) wait(&bars->q_full[t], segs[t]++);
+          wait(&bars->q_full[0], q_par[0]);
+          q_par[0] ^= 1;
+          if (two) {
+            wait(&bars->q_full[1], q_par[1]);
+            q_par[1] ^= 1;
+          }
           if (!wait(&bars->kv_full[st], phase)) break;
-          tc_fence_after();
-          for (int half = 0; half < 2; ++half)
-            for (int t = 0; t < nt; ++t) issue_qk(t, st, half);
+          issue_qk(k0, k0, st);
+          if (two) issue_qk(k1, k0, st);
+          issue_qk(k0, k1, st);
+          if (two) issue_qk(k1, k1, st);
           mma_commit(&bars->kv_empty[st]);
           next_unit();
           for (int j = 0; j < n; ++j) {
-            if (!wait(&bars->kv_full[st], phase)) break;
-            const int st_v = st;
+            const uint32_t st_v = st;
+            wait(&bars->kv_full[st], phase);
             next_unit();
             const bool more = j + 1 < n;
-            for (int half = 0; ok && half < 2; ++half)
-              for (int t = 0; t < nt; ++t) {
-                if (!wait(&bars->p_full[t][half], seen[t] >> 1)) break;
-                ++seen[t];
-                tc_fence_after();
-                issue_pv(t, st_v, half, j > 0 || half > 0);
-                const bool last = half == 1 && t == nt - 1;
-                if (last) mma_commit(&bars->kv_empty[st_v]);
-                if (more) {
-                  if (half == 0 && t == 0 && !wait(&bars->kv_full[st], phase)) break;
-                  tc_fence_after();
-                  issue_qk(t, st, half);
-                  if (last) mma_commit(&bars->kv_empty[st]);
-                }
+            auto step = [&](auto t_, auto half_, bool last) {
+              constexpr int t = decltype(t_)::value, half = decltype(half_)::value;
+              if (!ok || !wait(&bars->p_full[t][half], p_par[t])) return;
+              issue_pv(t_, half_, st_v, half > 0 || j > 0 ? 1u : 0u);
+              if (last) mma_commit(&bars->kv_empty[st_v]);
+              if (more) {
+                if (t == 0 && half == 0 && !wait(&bars->kv_full[st], phase)) return;
+                issue_qk(t_, half_, st);
+                if (last) mma_commit(&bars->kv_empty[st]);
+              } else {
+                mma_commit(&bars->o_final[t][half]);
               }
+            };
+            if (two) {
+              step(k0, k0, false);
+              step(k1, k0, false);
+              step(k0, k1, false);
+              step(k1, k1, true);
+              p_par[1] ^= 1;
+            } else {
+              step(k0, k0, false);
+              step(k0, k1, true);
+            }
+            p_par[0] ^= 1;
             if (!ok) break;
             // Softmax has taken this tile's scales and the converters its pages.
             mbar_arrive(&bars->meta_empty[tile_no++ % kMeta]);
@@ -607,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       const uint32_t t_o = tmem + lane_bits + 256 + t * D;
       const int rows = p.group * p.T;
       bool ok = true;
-      int tile_no = 0, seen = 0;  // tiles of the run, halves of this row tile
+      int tile_no = 0, seen = 0, segs = 0;  // tiles of the run, halves and blocks of this row tile
       for (int seg = 0; ok; ++seg) {
         const int seg_slot = seg % kSegs;
         ok = mbar_wait_bounded(&bars->seg_full[seg_slot], (seg / kSegs) & 1, abort_flag, kTimeoutNs);
@@ -714,9 +745,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
               l_run *= alpha;
             }
             if (j2 > 0) {
-              // The product of the half before may still be adding to the output (that of the half
-              // before it cannot: these scores were issued behind it, or are a block's first).
-              ok = mbar_wait_bounded(&bars->pv_done[t], (seen - 1) & 1, abort_flag, kTimeoutNs);
+              // The product of the half before may still be adding to the output. Behind it come the
+              // scores of the half after this one, or in the last tile its own signal.
+              ok = j2 + 1 < 2 * s.n
+                       ? mbar_wait_bounded(&bars->s_full[t][half ^ 1], ((seen + 1) >> 1) & 1, abort_flag, kTimeoutNs)
+                       : mbar_wait_bounded(&bars->o_final[t][0], segs & 1, abort_flag, kTimeoutNs);
               ok = __all_sync(0xffffffffu, ok);
               if (!ok) break;
               tc_fence_after();
@@ -766,9 +799,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           mbar_arrive(&bars->p_full[t][half]);
           tile_no += half;
         }
-        if (ok) {  // the last two products, one by one: a parity tells neighbouring phases apart only
-          ok = mbar_wait_bounded(&bars->pv_done[t], seen & 1, abort_flag, kTimeoutNs) &&
-               mbar_wait_bounded(&bars->pv_done[t], (seen - 1) & 1, abort_flag, kTimeoutNs);
+        if (ok) {  // the last tile's products
+          ok = mbar_wait_bounded(&bars->o_final[t][0], segs & 1, abort_flag, kTimeoutNs) &&
+               mbar_wait_bounded(&bars->o_final[t][1], segs & 1, abort_flag, kTimeoutNs);
+          ++segs;
           ok = __all_sync(0xffffffffu, ok);
         }
         if (!ok) {
