@@ -105,6 +105,13 @@ int main() {
         }
     }
 
+  // division by the group: every group, at its multiples' borders up to 2^24
+  for (int g = 1; g <= kMaxGroup; ++g)
+    for (int n = 0; n < (1 << 24); n += n < 4096 ? 1 : 65521)
+      for (int m : {n, n / g * g, n / g * g + g - 1})
+        if (m < (1 << 24) && divide_by_group(m, group_reciprocal(g)) != m / g) CHECK(false);
+  CHECK(divide_by_group((1 << 24) - 1, group_reciprocal(256)) == ((1 << 24) - 1) / 256);
+
   // tiles of a block of rows: the last key that any of its rows sees, against a walk over rows
   for (int group : {1, 3, 4, 8})
     for (int T : {1, 5, 64, 100})
@@ -120,7 +127,7 @@ int main() {
                   const int l = row_limit(e.length, e.count, r / group, causal);
                   if (l > lim) lim = l;
                 }
-                CHECK(block_tiles(e, group, row0, n, T, causal, 128) == (lim + 127) / 128);
+                CHECK(block_tiles(e, group * T, group_reciprocal(group), row0, n, causal, 128) == (lim + 127) / 128);
               }
             }
 

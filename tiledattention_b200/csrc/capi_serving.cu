@@ -93,7 +93,7 @@ int make_pages_map(CUtensorMap* map, const void* pages, int D, int page, int64_t
 
 int64_t workspace_bytes_of(int B, int Hq, int Hkv, int T, int D, int sms) {
   const int64_t rows = static_cast<int64_t>(Hq / Hkv) * T;
-  if (rows > (1 << 24)) return 0;
+  if (rows >= (1 << 24) || Hq / Hkv > ta::kv8::kMaxGroup) return 0;
   return static_cast<int64_t>(ta::kv8::uses_chunk(static_cast<int>(rows), D)
                                   ? ta::kv8::chunk_workspace_bytes(D, sms)
                                   : ta::kv8::attend_workspace_bytes(B, Hq, Hkv, T, D, sms));
@@ -231,7 +231,9 @@ int ta_sdpa_kv8(const void* q, const int64_t* q_strides, void* o, const int64_t*
   if (rc) return rc;
   if (Hq <= 0 || Hq % Hkv != 0)
     return ta_capi_fail(TA_ERR_INVALID_ARGUMENT, "query heads must be a multiple of the cache's heads");
-  if (static_cast<int64_t>(Hq / Hkv) * T > (1 << 24))
+  if (Hq / Hkv > ta::kv8::kMaxGroup)
+    return ta_capi_fail(TA_ERR_INVALID_ARGUMENT, "at most 256 query heads per cache head");
+  if (static_cast<int64_t>(Hq / Hkv) * T >= (1 << 24))
     return ta_capi_fail(TA_ERR_INVALID_ARGUMENT, "too many query rows per cache head");
   if (!is_16bit(dtype)) return ta_capi_fail(TA_ERR_UNSUPPORTED_DTYPE, "q: fp16 or bf16");
   if (!(scale > 0.f) || !std::isfinite(scale))
@@ -277,6 +279,7 @@ int ta_sdpa_kv8(const void* q, const int64_t* q_strides, void* o, const int64_t*
   p.bf16 = dtype == TA_DTYPE_BF16;
   p.causal = causal != 0;
   p.group = Hq / Hkv;
+  p.group_recip = ta::kv8::group_reciprocal(p.group);
   p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
   if (ta::kv8::uses_chunk(p.group * T, D))
     return launched(ta::kv8::launch_chunk(p, sms, static_cast<cudaStream_t>(stream)),

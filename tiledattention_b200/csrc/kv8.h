@@ -93,10 +93,25 @@ struct AttendParams {
   float* part_ml;
   Cut* cuts;
   int B, Hq, Hkv, T, D, page, page_shift, width, num_pages, bf16, causal;
-  int group;                      // Hq / Hkv
+  int group;                      // Hq / Hkv, at most kMaxGroup
+  uint32_t group_recip;           // for group_of
   int row_blocks;                 // blocks of rows (token, head of the group) per kv head
   float scale_log2;               // softmax scale * log2(e)
 };
+
+// n / group for 0 <= n < 2^24 by a multiplication (a division costs some thirty instructions in
+// each of its many places): recip = ceil(2^32 / group), exact for group <= kMaxGroup = 2^8.
+constexpr int kMaxGroup = 256;
+__host__ __device__ __forceinline__ uint32_t group_reciprocal(int group) {
+  return group == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + group - 1) / group);
+}
+__host__ __device__ __forceinline__ int divide_by_group(int n, uint32_t recip) {
+  return recip == 0 ? n
+                    : static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * recip) >> 32);
+}
+__host__ __device__ __forceinline__ int group_of(const AttendParams& p, int n) {
+  return divide_by_group(n, p.group_recip);
+}
 
 // Keys of a sequence that its row of token t may see: [0, limit).
 __host__ __device__ __forceinline__ int row_limit(int length, int count, int t, int causal) {
@@ -120,13 +135,13 @@ __host__ __device__ __forceinline__ SeqExtent checked_extent(int length, int cou
   return e;
 }
 
-// Key tiles of rows [row0, row0 + n) of a sequence's T * group rows (token, head of the group):
+// Key tiles of rows [row0, row0 + n) of a sequence's `rows` rows (token, head of the group):
 // up to the last key that any of them sees.
-__host__ __device__ __forceinline__ int block_tiles(const SeqExtent& e, int group, int row0, int n,
-                                                    int T, int causal, int tile) {
-  const int end = row0 + n < group * T ? row0 + n : group * T;
+__host__ __device__ __forceinline__ int block_tiles(const SeqExtent& e, int rows, uint32_t recip, int row0,
+                                                    int n, int causal, int tile) {
+  const int end = row0 + n < rows ? row0 + n : rows;
   if (row0 >= end) return 0;
-  const int first = row0 / group, last = (end - 1) / group;
+  const int first = divide_by_group(row0, recip), last = divide_by_group(end - 1, recip);
   if (first >= e.count) return 0;
   const int lim = row_limit(e.length, e.count, last < e.count ? last : e.count - 1, causal);
   return (lim + tile - 1) / tile;

@@ -51,25 +51,20 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// A batch-wide exclusive sum by one block of WARPS warps. `work(b, extent)`: the work of sequence b. Every
-// thread gets the total and the work before its own share [b0, b1) of the batch; `report`:
-// record lengths and counts out of range.
+// An exclusive sum over n items by one block of WARPS warps; `work(i)`: item i's. Every thread gets
+// the total and the work before its own share [i0, i1) of the items.
 struct Scan {
   int64_t total, mine;
-  int b0, b1;
+  int i0, i1;
 };
 template <int WARPS, class F>
-__device__ __forceinline__ Scan scan_batch(const AttendParams& p, int64_t* s_warp, bool report, F work) {
+__device__ __forceinline__ Scan scan_items(int n, int64_t* s_warp, F work) {
   Scan r;
-  const int share = (p.B + WARPS * 32 - 1) / (WARPS * 32);
-  r.b0 = min(p.B, static_cast<int>(threadIdx.x) * share);
-  r.b1 = min(p.B, r.b0 + share);
+  const int share = (n + WARPS * 32 - 1) / (WARPS * 32);
+  r.i0 = min(n, static_cast<int>(threadIdx.x) * share);
+  r.i1 = min(n, r.i0 + share);
   int64_t sum = 0;
-  for (int b = r.b0; b < r.b1; ++b) {
-    const SeqExtent e = extent_of(p, b);
-    if (e.bad && report && p.status) atomicOr(p.status, TA_DEVSTAT_BAD_LENGTH);
-    sum += work(e);
-  }
+  for (int i = r.i0; i < r.i1; ++i) sum += work(i);
   int64_t incl = sum;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -87,6 +82,11 @@ __device__ __forceinline__ Scan scan_batch(const AttendParams& p, int64_t* s_war
   }
   r.mine = before + incl - sum;
   return r;
+}
+
+// Records a sequence whose length or count is out of range.
+__device__ __forceinline__ void report_extent(const AttendParams& p, const SeqExtent& e) {
+  if (e.bad && blockIdx.x == 0 && p.status) atomicOr(p.status, TA_DEVSTAT_BAD_LENGTH);
 }
 
 }  // namespace kv8

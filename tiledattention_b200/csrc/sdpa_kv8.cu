@@ -187,7 +187,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
 
   // This block's run of the line, and the sequence it begins in.
   const int hrs = p.Hkv * p.row_blocks;
-  const Scan sc = scan_batch<kWarps>(p, s_scan, blockIdx.x == 0, [&](const SeqExtent& e) {
+  const Scan sc = scan_items<kWarps>(p.B, s_scan, [&](int b) {
+    const SeqExtent e = extent_of(p, b);
+    report_extent(p, e);
     return static_cast<int64_t>(tiles_of(e, C::kTile)) * hrs;
   });
   const int64_t total = sc.total;
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
   const int steps = static_cast<int>(run_begin(blockIdx.x + 1, total, parts) - w0);
   {
     int64_t at = sc.mine;
-    for (int b = sc.b0; b < sc.b1; ++b) {
+    for (int b = sc.i0; b < sc.i1; ++b) {
       const int64_t n = static_cast<int64_t>(tiles_of(extent_of(p, b), C::kTile)) * hrs;
       if (at <= w0 && w0 < at + n) {
         s_start[0] = b;
@@ -356,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
 #pragma unroll
           for (int x = 0; x < 4; ++x) o[m][nt][x] = 0.f;
         const int r = cur.rb * C::kRows + nt * 8 + g;
-        const int tok = r / p.group, hd = cur.h * p.group + (r - tok * p.group);
+        const int tok = group_of(p, r), hd = cur.h * p.group + (r - tok * p.group);
         const bool real = r < rows && tok < e.count;
         const int limit = real ? row_limit(e.length, e.count, tok, p.causal) : 0;
         if (limit > 0) least = min(least, limit);
@@ -680,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
             l = fmaf(s_l[w * C::kRows + r], mw == -INFINITY ? 1.f : ex2_approx(mw - m), l);
           }
           if (whole) {
-            const int tok = row / p.group, hd = cur.h * p.group + (row - tok * p.group);
+            const int tok = group_of(p, row), hd = cur.h * p.group + (row - tok * p.group);
             const float inv = l == 0.f ? 0.f : 1.f / l;
             uint16_t* out = static_cast<uint16_t*>(p.o) + cur.b * p.o_sb + hd * p.o_sh + tok * p.o_ss + d;
             *reinterpret_cast<uint2*>(out) = make_uint2(pack16(a.x * inv, a.y * inv, p.bf16),
@@ -731,12 +733,12 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const AttendParams p, i
   const int h = (blockIdx.x / row_groups) % p.Hkv;
   const int b = blockIdx.x / row_groups / p.Hkv;
   const int hrs = p.Hkv * p.row_blocks;
-  const Scan sc = scan_batch<kWarps>(p, s_scan, false, [&](const SeqExtent& e) {
-    return static_cast<int64_t>(tiles_of(e, C::kTile)) * hrs;
+  const Scan sc = scan_items<kWarps>(p.B, s_scan, [&](int i) {
+    return static_cast<int64_t>(tiles_of(extent_of(p, i), C::kTile)) * hrs;
   });
   {
     int64_t at = sc.mine;
-    for (int i = sc.b0; i < sc.b1; ++i) {
+    for (int i = sc.i0; i < sc.i1; ++i) {
       const int n = tiles_of(extent_of(p, i), C::kTile);
       if (i == b) {
         s_at = at;
@@ -824,7 +826,7 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const AttendParams p, i
     }
   }
   if (!mine) return;
-  const int tok = row / p.group, hd = h * p.group + (row - tok * p.group);
+  const int tok = group_of(p, row), hd = h * p.group + (row - tok * p.group);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* out = static_cast<uint16_t*>(p.o) + b * p.o_sb + hd * p.o_sh + tok * p.o_ss;
 #pragma unroll

@@ -12,9 +12,10 @@
 //   warps 8-11      converters: codes from the pages straight into registers (up to a tile
 //                   ahead), fp16 (exact) into the 128-byte-swizzled tiles that tcgen05 reads, a
 //                   unit being one tile's K or V
-//   warp 12         tensor memory and MMA issue (kind::f16, fp16 operands)
-//   warp 13         walks ahead through page table and scales
-//   warps 14-15     zero the rows of blocks without keys
+//   warps 12, 15    MMA issue for row tile 0, 1 (kind::f16, fp16 operands): one thread for both took
+//                   longer to issue and wait than the tensor pipe to compute
+//   warp 13         walks ahead through line, page table and scales
+//   warp 14         zeroes the rows of blocks without keys
 // Converting once in shared memory costs 2 D x 128 conversions a tile for 256 rows; fp8
 // MMAs would take e4m3 as it is, but then the weights have to be cut into several fp8 parts,
 // which costs the softmax warps, the tightest role, about three operations more an element.
@@ -45,7 +46,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 // Register split of the launch's 512 x 128 registers: softmax, converters, MMA and idle.
 constexpr int kLaunchRegs = 128;
-constexpr int kSoftmaxRegs = 152, kConvertRegs = 128, kSideRegs = 80;
+constexpr int kSoftmaxRegs = 160, kConvertRegs = 128, kSideRegs = 64;
 static_assert(128 * (2 * kSoftmaxRegs + kConvertRegs + kSideRegs) == kThreads * kLaunchRegs,
               "register split must match the launch allocation");
 constexpr uint32_t kTmemCols = 512;
@@ -94,7 +95,7 @@ struct Segment {
 
 struct Barriers {
   uint64_t q_full[2], s_full[2][2], p_full[2][2], o_final[2][2];  // [row tile][half]
-  uint64_t drain;
+  uint64_t drain[2];
   uint64_t kv_full[6], kv_empty[6], meta_full[kMeta], meta_empty[kMeta], seg_full[kSegs], seg_empty[kSegs];
   Segment segs[kSegs];
   Tile tiles[kMeta];
@@ -109,7 +110,7 @@ struct Start {  // where the run begins; its memory is the accumulator's notes' 
 };
 static_assert(sizeof(Barriers) <= 1024 && sizeof(Start) <= kSegs * 64 * 4, "shared memory blocks");
 
-// The run's walk over the line (warp 13's).
+// The run's walk over the line, by all lanes of one warp.
 template <int D>
 struct Walk {
   const AttendParams& p;
@@ -117,23 +118,40 @@ struct Walk {
   Segment s;
   SeqExtent e;
   __device__ int block() const {
-    return block_tiles(e, p.group, s.rb * Cfg<D>::kRows, Cfg<D>::kRows, p.T, p.causal, kTileKeys);
+    return block_tiles(e, p.group * p.T, p.group_recip, s.rb * Cfg<D>::kRows, Cfg<D>::kRows, p.causal, kTileKeys);
   }
   __device__ Walk(const AttendParams& pp, int64_t w0, int64_t w1, int b, int64_t before)
       : p(pp), at(w0), end(w1) {
     s.b = b;
     e = extent_of(p, b);
-    int64_t head = 0;
-    for (s.rb = 0; s.rb < p.row_blocks; ++s.rb) head += block();
+    const int lane = threadIdx.x & 31;
+    auto tiles_at = [&](int rb) {
+      s.rb = rb;
+      return rb < p.row_blocks ? block() : 0;
+    };
+    int64_t head = 0;  // tiles of one head
+    for (int base = 0; base < p.row_blocks; base += 32)
+      head += __reduce_add_sync(0xffffffffu, tiles_at(base + lane));
     int64_t rem = w0 - before;
     s.h = static_cast<int>(rem / head);
     rem -= s.h * head;
-    s.rb = 0;
-    s.tiles = block();
-    while (rem >= s.tiles) {
-      rem -= s.tiles;
-      ++s.rb;
-      s.tiles = block();
+    for (int base = 0;; base += 32) {
+      const int mine = tiles_at(base + lane);
+      int incl = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += up;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, incl > rem);
+      if (past) {
+        const int at_lane = __ffs(past) - 1;
+        s.tiles = __shfl_sync(0xffffffffu, mine, at_lane);
+        rem -= __shfl_sync(0xffffffffu, incl, at_lane) - s.tiles;
+        s.rb = base + at_lane;
+        break;
+      }
+      rem -= __shfl_sync(0xffffffffu, incl, 31);
     }
     begin(static_cast<int>(rem));
   }
@@ -144,7 +162,7 @@ struct Walk {
     s.count = e.count;
     s.safe = e.length;
     if (p.causal) {  // the first token with any keys sees the fewest
-      const int tok = max(s.rb * Cfg<D>::kRows / p.group, e.count - e.length);
+      const int tok = max(group_of(p, s.rb * Cfg<D>::kRows), e.count - e.length);
       s.safe = row_limit(e.length, e.count, tok, 1);
     }
   }
@@ -180,19 +198,18 @@ __device__ __forceinline__ void report(const AttendParams& p, uint32_t code, vol
 
 // The MMAs of a product, descriptor steps as immediates: scores over D dims, 16 at a time (64 dims
 // are one 128-byte-wide part of a tile) ...
-template <int A, int B, int... kk>
+template <int... kk>
 __device__ __forceinline__ void issue_qk_seq(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                              std::integer_sequence<int, kk...>) {
-  (mma_ss_imm<((A + (kk >> 2) * (kTileRows * 128) + (kk & 3) * 32) >> 4),
-              ((B + (kk >> 2) * (kTileKeys * 128) + (kk & 3) * 32) >> 4), (kk > 0 ? 1 : 0)>(d, a, b,
-                                                                                           idesc),
+  (mma_ss_imm<(((kk >> 2) * (kTileRows * 128) + (kk & 3) * 32) >> 4),
+              (((kk >> 2) * (kTileKeys * 128) + (kk & 3) * 32) >> 4), (kk > 0 ? 1 : 0)>(d, a, b, idesc),
    ...);
 }
 // ... and the output over keys, 16 at a time.
-template <int B, int... kk>
+template <int... kk>
 __device__ __forceinline__ void issue_pv_seq(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
                                              uint32_t acc, std::integer_sequence<int, kk...>) {
-  (mma_ts_imm_acc<kk * 8, ((B + kk * 16 * 128) >> 4)>(d, a, b, idesc, kk == 0 ? acc : 1u), ...);
+  (mma_ts_imm_acc<kk * 8, ((kk * 16 * 128) >> 4)>(d, a, b, idesc, kk == 0 ? acc : 1u), ...);
 }
 
 __device__ __forceinline__ void st_shared128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
@@ -238,18 +255,20 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         mbar_init(&bars->o_final[t][half], 1);
       }
     }
-    mbar_init(&bars->drain, 1);
+    mbar_init(&bars->drain[0], 1);
+    mbar_init(&bars->drain[1], 1);
+    start->b = -1;
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&bars->kv_full[s], 128);
-      mbar_init(&bars->kv_empty[s], 1);
+      mbar_init(&bars->kv_empty[s], C::kTiles);
     }
     for (int i = 0; i < kMeta; ++i) {
       mbar_init(&bars->meta_full[i], 32);
-      mbar_init(&bars->meta_empty[i], 1);
+      mbar_init(&bars->meta_empty[i], C::kTiles);
     }
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(&bars->seg_full[i], 32);
-      mbar_init(&bars->seg_empty[i], 4 * C::kTiles + 1);  // softmax warps and the MMA warp
+      mbar_init(&bars->seg_empty[i], 5 * C::kTiles);  // a row tile's softmax and MMA warps
     }
     bars->abort_flag = 0;
     p.cuts[blockIdx.x] = Cut{0, 0, 0, -1};  // until this thread knows better
@@ -260,13 +279,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
     tmem_relinquish();
   }
   tc_fence_before();
-  const auto per_seq = [&](const SeqExtent& e) {
-    int64_t n = 0;
-    for (int rb = 0; rb < p.row_blocks; ++rb)
-      n += block_tiles(e, p.group, rb * C::kRows, C::kRows, p.T, p.causal, kTileKeys);
-    return n * p.Hkv;
+  // Items: blocks of rows of one head of each sequence.
+  const auto item_work = [&](int i) {
+    const int b = i / p.row_blocks, rb = i - b * p.row_blocks;
+    const SeqExtent e = extent_of(p, b);
+    if (rb == 0) report_extent(p, e);
+    return static_cast<int64_t>(block_tiles(e, p.group * p.T, p.group_recip, rb * C::kRows, C::kRows,
+                                            p.causal, kTileKeys)) * p.Hkv;
   };
-  const Scan sc = scan_batch<kWarps>(p, start->scan, blockIdx.x == 0, per_seq);  // has a barrier
+  const Scan sc = scan_items<kWarps>(p.B * p.row_blocks, start->scan, item_work);  // has a barrier
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = bars->tmem_base;
@@ -274,30 +295,37 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
   const bool has_run = blockIdx.x < parts;
   const int64_t w0 = has_run ? run_begin(blockIdx.x, sc.total, parts) : 0;
   const int64_t w1 = has_run ? run_begin(blockIdx.x + 1, sc.total, parts) : 0;
-  if (has_run) {
-    int64_t at = sc.mine;
-    for (int b = sc.b0; b < sc.b1; ++b) {
-      const int64_t n = per_seq(extent_of(p, b));
-      if (at <= w0 && w0 < at + n) {
-        start->b = b;
-        start->w = at;
+  // The run's first sequence: the last one whose work begins at or before it.
+  if (has_run)
+    for (int pass = 0; pass < 2; ++pass) {
+      int64_t at = sc.mine;
+      for (int i = sc.i0; i < sc.i1; ++i) {
+        if (i % p.row_blocks == 0 && at <= w0) {
+          if (pass == 0) atomicMax(&start->b, i / p.row_blocks);
+          else if (start->b == i / p.row_blocks) start->w = at;
+        }
+        if (at > w0) break;
+        if (pass == 0 || i + 1 < sc.i1) at += item_work(i);
       }
-      at += n;
+      __syncthreads();
     }
-  }
-  __syncthreads();
 
   if (warp >= 12) {
     regs_dec<kSideRegs>();
-    if (warp == 12) {
-      // ------------------------------------------------------------ MMA issuer
+    if (warp == 12 || (warp == 15 && C::kTiles == 2)) {
+      // ------------------------------------------------------------ MMA issuers
       if (lane == 0 && has_run) {
         constexpr uint32_t kIdescQK = idesc_f16(kTileRows, kHalfKeys, false, false, false);
         constexpr uint32_t kIdescPV = idesc_f16(kTileRows, D, false, false, true);
-        const uint64_t q_desc = sdesc_sw128(smem_u32(q_smem), 16, 1024);
+        constexpr uint32_t kUnit = C::kTileBytes >> 4;  // in a descriptor's 16-byte steps
+        constexpr uint32_t kHalfStep = kHalfKeys * 128 >> 4;
+        const int t = warp == 12 ? 0 : 1;
+        const uint64_t q_desc = sdesc_sw128(smem_u32(q_smem + t * C::kTileBytes), 16, 1024);
         const uint64_t kv_desc_k = sdesc_sw128(smem_u32(kv_smem), 16, 1024);
         const uint64_t kv_desc_v = sdesc_sw128(smem_u32(kv_smem), kTileKeys * 128, 1024);
-        const uint32_t unit = C::kTileBytes >> 4;  // in a descriptor's 16-byte steps
+        const uint32_t t_s = tmem + t * 128, t_o = tmem + 256 + t * D;
+        uint64_t* const s_full = bars->s_full[t];
+        uint64_t* const p_full = bars->p_full[t];
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
           if (!mbar_try_wait(smem_u32(bar), parity))
@@ -305,94 +333,79 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           tc_fence_after();
           return ok;
         };
-        // Scores of one half of a tile's keys for row tile t. Halves: a tile's columns of tensor
-        // memory hold two of 64, so the next tile's first half is computed while softmax works on
-        // this one's second, where a whole tile would leave one of the two idle in turn. This one
-        // thread issues everything, so its instructions count: descriptor steps are immediates
-        // and the halves and row tiles unrolled.
-        auto issue_qk = [&](auto t_, auto half_, uint32_t st) {
-          constexpr int t = decltype(t_)::value, half = decltype(half_)::value;
-          issue_qk_seq<t * C::kTileBytes, half * kHalfKeys * 128>(
-              tmem + t * 128 + half * kHalfKeys, q_desc, kv_desc_k + st * unit, kIdescQK,
-              std::make_integer_sequence<int, D / 16>());
-          mma_commit(&bars->s_full[t][half]);
-        };
-        auto issue_pv = [&](auto t_, auto half_, uint32_t st, uint32_t acc) {
-          constexpr int t = decltype(t_)::value, half = decltype(half_)::value;
-          issue_pv_seq<half * kHalfKeys * 128>(tmem + 256 + t * D, tmem + t * 128 + half * kHalfKeys,
-                                               kv_desc_v + st * unit, kIdescPV, acc,
-                                               std::make_integer_sequence<int, kHalfKeys / 16>());
-        };
-        constexpr std::integral_constant<int, 0> k0{};
-        constexpr std::integral_constant<int, 1> k1{};
         uint32_t st = 0, phase = 0;  // of the next unit
-        uint32_t q_par[2] = {0, 0}, p_par[2] = {0, 0};  // parities of row tiles' segments, tiles
-        int tile_no = 0;
         auto next_unit = [&]() {
           if (++st == C::kStages) {
             st = 0;
             phase ^= 1;
           }
         };
+        // Halves: a row tile's columns of tensor memory hold the scores of two times 64 keys, so the
+        // next tile's first half is computed while softmax works on this one's second.
+        auto issue_qk = [&](int half, uint64_t kd) {
+          issue_qk_seq(t_s + half * kHalfKeys, q_desc, kd + half * kHalfStep, kIdescQK,
+                       std::make_integer_sequence<int, D / 16>());
+          mma_commit(&s_full[half]);
+        };
+        uint32_t q_par = 0, p_par = 0;
+        int tile_no = 0;
         for (int seg = 0; ok; ++seg) {
           if (!wait(&bars->seg_full[seg % kSegs], (seg / kSegs) & 1)) break;
           const int n = bars->segs[seg % kSegs].n;
-          const bool two = has_two<D>(p, bars->segs[seg % kSegs].rb);
+          const bool mine = t == 0 || has_two<D>(p, bars->segs[seg % kSegs].rb);
           mbar_arrive(&bars->seg_empty[seg % kSegs]);
           if (n == 0) break;
-          wait(&bars->q_full[0], q_par[0]);
-          q_par[0] ^= 1;
-          if (two) {
-            wait(&bars->q_full[1], q_par[1]);
-            q_par[1] ^= 1;
+          if (!mine) {  // no rows: the units pass
+            for (int u = 0; ok && u < 2 * n; ++u) {
+              if (!wait(&bars->kv_full[st], phase)) break;
+              mbar_arrive(&bars->kv_empty[st]);
+              next_unit();
+              if (u & 1) mbar_arrive(&bars->meta_empty[tile_no++ % kMeta]);
+            }
+            continue;
           }
+          wait(&bars->q_full[t], q_par);
+          q_par ^= 1;
           if (!wait(&bars->kv_full[st], phase)) break;
-          issue_qk(k0, k0, st);
-          if (two) issue_qk(k1, k0, st);
-          issue_qk(k0, k1, st);
-          if (two) issue_qk(k1, k1, st);
+          issue_qk(0, kv_desc_k + st * kUnit);
+          issue_qk(1, kv_desc_k + st * kUnit);
           mma_commit(&bars->kv_empty[st]);
           next_unit();
           for (int j = 0; j < n; ++j) {
             const uint32_t st_v = st;
+            const uint64_t vd = kv_desc_v + st * kUnit;
             wait(&bars->kv_full[st], phase);
             next_unit();
             const bool more = j + 1 < n;
-            auto step = [&](auto t_, auto half_, bool last) {
-              constexpr int t = decltype(t_)::value, half = decltype(half_)::value;
-              if (!ok || !wait(&bars->p_full[t][half], p_par[t])) return;
-              issue_pv(t_, half_, st_v, half > 0 || j > 0 ? 1u : 0u);
-              if (last) mma_commit(&bars->kv_empty[st_v]);
+            const uint64_t kd = kv_desc_k + st * kUnit;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (!wait(&p_full[half], p_par)) break;
+              issue_pv_seq(t_o, t_s + half * kHalfKeys, vd + half * kHalfStep, kIdescPV,
+                           half > 0 || j > 0 ? 1u : 0u, std::make_integer_sequence<int, kHalfKeys / 16>());
               if (more) {
-                if (t == 0 && half == 0 && !wait(&bars->kv_full[st], phase)) return;
-                issue_qk(t_, half_, st);
-                if (last) mma_commit(&bars->kv_empty[st]);
+                if (half == 0 && !wait(&bars->kv_full[st], phase)) break;
+                issue_qk(half, kd);
               } else {
                 mma_commit(&bars->o_final[t][half]);
               }
-            };
-            if (two) {
-              step(k0, k0, false);
-              step(k1, k0, false);
-              step(k0, k1, false);
-              step(k1, k1, true);
-              p_par[1] ^= 1;
-            } else {
-              step(k0, k0, false);
-              step(k0, k1, true);
             }
-            p_par[0] ^= 1;
             if (!ok) break;
+            mma_commit(&bars->kv_empty[st_v]);
+            if (more) {
+              mma_commit(&bars->kv_empty[st]);
+              next_unit();
+            }
+            p_par ^= 1;
             // Softmax has taken this tile's scales and the converters its pages.
             mbar_arrive(&bars->meta_empty[tile_no++ % kMeta]);
-            if (more) next_unit();
           }
         }
         if (!ok && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_MMA, abort_flag);
         // All MMAs this thread issued complete before tensor memory is freed.
-        mma_commit(&bars->drain);
+        mma_commit(&bars->drain[t]);
         volatile int no_abort = 0;
-        if (!mbar_wait_bounded(&bars->drain, 0, &no_abort, kTimeoutNs) && p.status)
+        if (!mbar_wait_bounded(&bars->drain[t], 0, &no_abort, kTimeoutNs) && p.status)
           atomicOr(p.status, TA_DEVSTAT_TIMEOUT_DRAIN);
       }
       __syncwarp();
@@ -488,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         if (ok) publish_segment(true);
         if (!ok && lane == 0 && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_LOAD, abort_flag);
       }
-    } else {
+    } else if (warp == 14) {
       // ------------------------------------------------------------ rows of blocks without keys
       const int rows = p.group * p.T;
       const int64_t blocks = static_cast<int64_t>(p.B) * p.Hkv * p.row_blocks;
@@ -496,11 +509,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         const int rb = static_cast<int>(i % p.row_blocks);
         const int h = static_cast<int>(i / p.row_blocks % p.Hkv);
         const int b = static_cast<int>(i / p.row_blocks / p.Hkv);
-        if (block_tiles(extent_of(p, b), p.group, rb * C::kRows, C::kRows, p.T, p.causal, kTileKeys))
+        if (block_tiles(extent_of(p, b), rows, p.group_recip, rb * C::kRows, C::kRows, p.causal, kTileKeys))
           continue;
         const int r1 = min(rows, (rb + 1) * C::kRows);
-        for (int r = rb * C::kRows + warp - 14; r < r1; r += 2) {
-          const int tok = r / p.group, hd = h * p.group + (r - tok * p.group);
+        for (int r = rb * C::kRows; r < r1; ++r) {
+          const int tok = group_of(p, r), hd = h * p.group + (r - tok * p.group);
           uint16_t* out = static_cast<uint16_t*>(p.o) + b * p.o_sb + hd * p.o_sh + tok * p.o_ss;
           for (int d = lane * 8; d < p.D; d += 256) sts128(out + d, 0, 0, 0, 0);
           if (p.lse && lane == 0)
@@ -583,26 +596,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           ok = ok && mbar_wait_bounded(&bars->kv_empty[st], phase ^ 1, abort_flag, kTimeoutNs);
           if (!ok) break;
           const uint32_t dst = store + st * C::kTileBytes;
+          uint32_t nans = 0;
 #pragma unroll
           for (int i = 0; i < C::kChunks; ++i) {
-            uint4 v = held[kWholeTile ? kind * C::kChunks + i : i];
-            if (edge && kind == 1) {
-              if ((nan_bits(v.x) | nan_bits(v.y) | nan_bits(v.z) | nan_bits(v.w)) != 0) {
-                *any_nan = 1;
-#pragma unroll 1
-                for (int k = 0; k < 4; ++k) {
-                  uint32_t y = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w;
-                  for (int b = 0; b < 4; ++b)
-                    if ((y >> (8 * b) & 0x7fu) == 0x7fu)
-                      atomicMin(nan_here + c * 16 + k * 4 + b, key0 + i * kRowsPerPass + row0);
-                  y &= ~((nan_bits(y) >> 7) * 0xffu);
-                  if (k == 0) v.x = y;
-                  else if (k == 1) v.y = y;
-                  else if (k == 2) v.z = y;
-                  else v.w = y;
-                }
-              }
-            }
+            const uint4 v = held[kWholeTile ? kind * C::kChunks + i : i];
+            if (kind == 1) nans |= nan_bits(v.x) | nan_bits(v.y) | nan_bits(v.z) | nan_bits(v.w);
             uint32_t f[8];
             codes_to_f16(v.x, f[0], f[1]);
             codes_to_f16(v.y, f[2], f[3]);
@@ -610,6 +608,19 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             codes_to_f16(v.w, f[6], f[7]);
             st_shared128(dst + i * (kRowsPerPass * 128) + piece0, f[0], f[1], f[2], f[3]);
             st_shared128(dst + i * (kRowsPerPass * 128) + piece1, f[4], f[5], f[6], f[7]);
+          }
+          if (kind == 1 && edge && nans) {  // rare: over the thread's own values once more
+#pragma unroll 1
+            for (int i = 0; i < C::kChunks * 16; ++i) {
+              const int pass = i >> 4, k = i & 15;
+              const uint32_t a = dst + pass * (kRowsPerPass * 128) + (k < 8 ? piece0 : piece1) + (k & 7) * 2;
+              uint16_t h;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(a));
+              if ((h & 0x7fff) <= 0x7c00) continue;
+              *any_nan = 1;
+              atomicMin(nan_here + c * 16 + k, key0 + pass * kRowsPerPass + row0);
+              asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(static_cast<uint16_t>(0)));
+            }
           }
           fence_proxy_async_shared();
           mbar_arrive(&bars->kv_full[st]);
@@ -656,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           continue;
         }
         const int row = s.rb * C::kRows + t * kTileRows + r_in_tile;
-        const int tok = row / p.group, hd = s.h * p.group + (row - tok * p.group);
+        const int tok = group_of(p, row), hd = s.h * p.group + (row - tok * p.group);
         const bool real = row < rows && tok < s.count;
         const int lim = real ? row_limit(s.length, s.count, tok, p.causal) : 0;
         const int safe = __reduce_min_sync(0xffffffffu, lim > 0 ? lim : 0x7fffffff);
@@ -667,35 +678,48 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           const uint4* q = reinterpret_cast<const uint4*>(
               static_cast<const uint16_t*>(p.q) + s.b * p.q_sb + static_cast<int64_t>(hd) * p.q_sh +
               static_cast<int64_t>(tok) * p.q_ss);
+          constexpr int kOnce = D <= 128 ? D / 8 : 16;  // vectors held at a time
+          uint4 v[kOnce];
           float amax = 0.f;
-          if (real)
-#pragma unroll 8
-            for (int i = 0; i < p.D / 8; ++i) {
-              const uint4 v = q[i];
-              const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+          auto load = [&](int base) {
+#pragma unroll
+            for (int i = 0; i < kOnce; ++i) {
+              v[i] = make_uint4(0, 0, 0, 0);
+              if (real && (base + i) * 8 < p.D) v[i] = q[base + i];
+            }
+          };
+#pragma unroll 1
+          for (int base = 0; base < D / 8; base += kOnce) {
+            load(base);
+#pragma unroll
+            for (int i = 0; i < kOnce; ++i) {
+              const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const float2 a = unpack16(x[k], p.bf16);
                 amax = fmaxf(amax, fmaxf(fabsf(a.x), fabsf(a.y)));
               }
             }
+          }
           const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 14, -126), 113);
           const float up = pow2f(-ex);
           mul = p.scale_log2 * pow2f(ex);
           uint8_t* dst = q_smem + t * C::kTileBytes + r_in_tile * 128;
-#pragma unroll 4
-          for (int i = 0; i < D / 8; ++i) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (real && i * 8 < p.D) v = q[i];
-            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-            uint32_t y[4];
+#pragma unroll 1
+          for (int base = 0; base < D / 8; base += kOnce) {
+            if (D / 8 > kOnce) load(base);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 a = unpack16(x[k], p.bf16);
-              y[k] = pack_f16(a.x * up, a.y * up);
+            for (int i = 0; i < kOnce; ++i) {
+              const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+              uint32_t y[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 a = unpack16(x[k], p.bf16);
+                y[k] = pack_f16(a.x * up, a.y * up);
+              }
+              sts128(dst + ((base + i) >> 3) * (kTileRows * 128) + ((i & 7) ^ (r_in_tile & 7)) * 16, y[0],
+                     y[1], y[2], y[3]);
             }
-            sts128(dst + (i >> 3) * (kTileRows * 128) + ((i & 7) ^ (r_in_tile & 7)) * 16, y[0], y[1],
-                   y[2], y[3]);
           }
           fence_proxy_async_shared();
           mbar_arrive(&bars->q_full[t]);
@@ -754,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
               if (!ok) break;
               tc_fence_after();
               const uint64_t alpha2 = f2_pack(alpha, alpha);
-#pragma unroll
+#pragma unroll 1
               for (int cc = 0; cc < D / 32; ++cc) {
                 uint32_t o[32];
                 tmem_ld32(t_o + cc * 32, o);
@@ -817,13 +841,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         }
         const bool has = ref != -INFINITY;
         const float inv = !whole ? 1.f : l_run == 0.f ? 0.f : 1.f / l_run;
-        const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + (s.t0 == 0 ? 1 : 0)) * C::kRows +
-                             t * kTileRows + r_in_tile;
+        // Partial results: [run][first or last block][4 dims][row][4], so that a warp's rows are
+        // written and read side by side.
+        const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + (s.t0 == 0 ? 1 : 0)) * C::kRows;
         uint16_t* out = static_cast<uint16_t*>(p.o) + s.b * p.o_sb + static_cast<int64_t>(hd) * p.o_sh +
                         static_cast<int64_t>(tok) * p.o_ss;
         const bool any_nan = *static_cast<volatile int*>(&bars->any_nan[seg_slot]) != 0;
         const int* nan_here = nan_key + seg_slot * D;
-#pragma unroll
+#pragma unroll 1
         for (int cc = 0; cc < D / 32; ++cc) {
           uint32_t o[32];
           tmem_ld32(t_o + cc * 32, o);
@@ -838,7 +863,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
 #pragma unroll
               for (int i = 0; i < 32; i += 4)
                 if (cc * 32 + i < p.D)
-                  *reinterpret_cast<float4*>(p.part_o + part * D + cc * 32 + i) =
+                  *reinterpret_cast<float4*>(p.part_o + part * D +
+                                             ((cc * 8 + i / 4) * C::kRows + t * kTileRows + r_in_tile) * 4) =
                       has ? make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
                                         __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]))
                           : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -860,7 +886,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         }
         if (row < rows) {
           if (!whole)
-            *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(ref, l_run);
+            *reinterpret_cast<float2*>(p.part_ml + (part + t * kTileRows + r_in_tile) * 2) =
+                make_float2(ref, l_run);
           else if (p.lse)
             p.lse[(static_cast<int64_t>(s.b) * p.Hq + hd) * p.T + tok] = lse_of(ref, l_run);
         }
@@ -883,73 +910,72 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
 }
 
 // Merges the blocks that several runs share: blockIdx.x = the run that ends the block,
-// blockIdx.y = 32 of its rows, four a warp.
+// blockIdx.y = 32 of its rows, a lane each; a warp has every eighth group of 4 dims.
 template <int D>
 __global__ void __launch_bounds__(256) merge_kernel(const AttendParams p) {
   using C = Cfg<D>;
-  constexpr int kVec = D <= 128 ? 1 : 2;  // float4 a lane
-  constexpr int kPer = 4;
+  constexpr int kVec = D / 32;
+  constexpr int kStride = D + 8;  // of a row of the 16-bit tile, values
+  __shared__ __align__(16) uint16_t tile[32 * kStride];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Cut cut = p.cuts[blockIdx.x];
   if (cut.first < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows = min(p.group * p.T - cut.rb * C::kRows, C::kRows);
-  const int r0 = blockIdx.y * 32 + warp * kPer;
+  const int r0 = blockIdx.y * 32;
   if (r0 >= rows) return;
-  float m[kPer], l[kPer];
-  float4 a[kPer][kVec];
+  const int r = min(r0 + lane, rows - 1);
+  float m = -INFINITY, l = 0.f;
+  float4 a[kVec];
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    m[k] = -INFINITY;
-    l[k] = 0.f;
-#pragma unroll
-    for (int v = 0; v < kVec; ++v) a[k][v] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
+  for (int v = 0; v < kVec; ++v) a[v] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
   for (int i = cut.first; i <= static_cast<int>(blockIdx.x); ++i) {
     // the block's first run has it in its second slot, the others in their first
-    const int64_t at = (static_cast<int64_t>(i) * 2 + (i == cut.first ? 1 : 0)) * C::kRows + r0;
+    const int64_t part = (static_cast<int64_t>(i) * 2 + (i == cut.first ? 1 : 0)) * C::kRows;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (part + r) * 2);
+    // without a reference: sums of 0 or NaN and outputs of 0, kept as they are
+    const float mn = fmaxf(m, ml.x);
+    const float fa = m == -INFINITY ? 1.f : exp2f(m - mn);
+    const float fb = ml.x == -INFINITY ? 1.f : exp2f(ml.x - mn);
+    l = l * fa + ml.y * fb;
+    m = mn;
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      if (r0 + k >= rows) break;
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (at + k) * 2);
-      // without a reference: sums of 0 or NaN and outputs of 0, kept as they are
-      const float mn = fmaxf(m[k], ml.x);
-      const float fa = m[k] == -INFINITY ? 1.f : exp2f(m[k] - mn);
-      const float fb = ml.x == -INFINITY ? 1.f : exp2f(ml.x - mn);
-      l[k] = l[k] * fa + ml.y * fb;
-      m[k] = mn;
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) {
-        const int d = (v * 32 + lane) * 4;
-        if (d < p.D) {
-          const float4 x = *reinterpret_cast<const float4*>(p.part_o + (at + k) * D + d);
-          a[k][v].x = a[k][v].x * fa + x.x * fb;
-          a[k][v].y = a[k][v].y * fa + x.y * fb;
-          a[k][v].z = a[k][v].z * fa + x.z * fb;
-          a[k][v].w = a[k][v].w * fa + x.w * fb;
-        }
+    for (int v = 0; v < kVec; ++v) {
+      const int d4 = v * 8 + warp;
+      if (d4 * 4 < p.D) {
+        const float4 x = *reinterpret_cast<const float4*>(p.part_o + part * D + (d4 * C::kRows + r) * 4);
+        a[v].x = a[v].x * fa + x.x * fb;
+        a[v].y = a[v].y * fa + x.y * fb;
+        a[v].z = a[v].z * fa + x.z * fb;
+        a[v].w = a[v].w * fa + x.w * fb;
       }
     }
   }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    if (r0 + k >= rows) break;
-    const int row = cut.rb * C::kRows + r0 + k;
-    const int tok = row / p.group, hd = cut.h * p.group + (row - tok * p.group);
-    const float inv = l[k] == 0.f ? 0.f : 1.f / l[k];
-    uint16_t* out = static_cast<uint16_t*>(p.o) + cut.b * p.o_sb + static_cast<int64_t>(hd) * p.o_sh +
-                    static_cast<int64_t>(tok) * p.o_ss;
-#pragma unroll
-    for (int v = 0; v < kVec; ++v) {
-      const int d = (v * 32 + lane) * 4;
-      if (d < p.D)
-        *reinterpret_cast<uint2*>(out + d) =
-            make_uint2(pack16(a[k][v].x * inv, a[k][v].y * inv, p.bf16),
-                       pack16(a[k][v].z * inv, a[k][v].w * inv, p.bf16));
-    }
-    if (p.lse && lane == 0)
-      p.lse[(static_cast<int64_t>(cut.b) * p.Hq + hd) * p.T + tok] = lse_of(m[k], l[k]);
+  for (int v = 0; v < kVec; ++v)
+    *reinterpret_cast<uint2*>(tile + lane * kStride + (v * 8 + warp) * 4) =
+        make_uint2(pack16(a[v].x * inv, a[v].y * inv, p.bf16), pack16(a[v].z * inv, a[v].w * inv, p.bf16));
+  const int n = min(32, rows - r0);
+  auto place = [&](int row, int64_t& o, int64_t& at_lse) {
+    const int g = cut.rb * C::kRows + r0 + row;
+    const int tok = group_of(p, g), hd = cut.h * p.group + (g - tok * p.group);
+    o = cut.b * p.o_sb + static_cast<int64_t>(hd) * p.o_sh + static_cast<int64_t>(tok) * p.o_ss;
+    at_lse = (static_cast<int64_t>(cut.b) * p.Hq + hd) * p.T + tok;
+  };
+  int64_t o, at;
+  if (p.lse && warp == 0 && lane < n) {
+    place(lane, o, at);
+    p.lse[at] = lse_of(m, l);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n * (D / 8); i += 256) {
+    const int row = i / (D / 8), c = i % (D / 8);
+    if (c * 8 >= p.D) continue;
+    place(row, o, at);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.o) + o + c * 8) =
+        *reinterpret_cast<const uint4*>(tile + row * kStride + c * 8);
   }
 }
 
@@ -978,6 +1004,7 @@ cudaError_t launch(AttendParams p, int sm_count, cudaStream_t stream) {
   }
   const int64_t rows = static_cast<int64_t>(p.group) * p.T;
   p.row_blocks = static_cast<int>((rows + C::kRows - 1) / C::kRows);
+  if (static_cast<int64_t>(p.B) * p.row_blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   const int64_t seq_tiles = (static_cast<int64_t>(p.width) * p.page + kTileKeys - 1) / kTileKeys;
   const int64_t most = seq_tiles * p.Hkv * p.row_blocks * p.B;
   const int parts = static_cast<int>(most < sm_count ? most : sm_count);
