@@ -649,7 +649,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       const uint32_t t_o = tmem + lane_bits + 256 + t * D;
       const int rows = p.group * p.T;
       bool ok = true;
-      const uint32_t metas = smem_u32(meta);
       int tile_no = 0, seen = 0, segs = 0;  // tiles of the run, halves and blocks of this row tile
       for (int seg = 0; ok; ++seg) {
         const int seg_slot = seg % kSegs;
@@ -727,41 +726,19 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         }
 
         float ref = -INFINITY, l_run = 0.f;
-        // Scores of a half are loaded while the half before is stored: `ready` says so.
-        uint32_t x[64];
-        auto load_scores = [&](int half) {
-          tc_fence_after();
-          tmem_ld64(t_s + half * kHalfKeys, *reinterpret_cast<uint32_t(*)[32]>(x),
-                    *reinterpret_cast<uint32_t(*)[32]>(x + 32));
-        };
-        bool ready = false;
-#pragma unroll 1
         for (int j2 = 0; j2 < 2 * s.n; ++j2, ++seen) {
           const int half = j2 & 1;
           const int slot = tile_no % kMeta;
-          if (half == 0 && !mbar_try_wait(smem_u32(&bars->meta_full[slot]), (tile_no / kMeta) & 1))
+          if (half == 0)
             ok = mbar_wait_bounded(&bars->meta_full[slot], (tile_no / kMeta) & 1, abort_flag, kTimeoutNs);
-          if (!ready) {
-            if (!mbar_try_wait(smem_u32(&bars->s_full[t][half]), (seen >> 1) & 1))
-              ok = ok && mbar_wait_bounded(&bars->s_full[t][half], (seen >> 1) & 1, abort_flag, kTimeoutNs);
-            if (!__all_sync(0xffffffffu, ok)) {
-              ok = false;
-              break;
-            }
-            load_scores(half);
-          }
-          float c[4], e[4], back[4];  // of the half's four pages, or parts of pages
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            float ks;
-            asm volatile("ld.shared.v4.f32 {%0, %1, %2, _}, [%3];"
-                         : "=f"(ks), "=f"(e[g]), "=f"(back[g])
-                         : "r"(metas + ((slot * kGroups) + half * (kGroups / 2) + g) * 16));
-            c[g] = fmaxf(mul * ks, 1e-37f);  // above zero, so that a masked score stays -inf
-          }
+          ok = ok && mbar_wait_bounded(&bars->s_full[t][half], (seen >> 1) & 1, abort_flag, kTimeoutNs);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          uint32_t x[64];
+          tmem_ld64(t_s + half * kHalfKeys, *reinterpret_cast<uint32_t(*)[32]>(x),
+                    *reinterpret_cast<uint32_t(*)[32]>(x + 32));
           tmem_wait_ld();
-          reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(x));
-          reg_fence32(*reinterpret_cast<uint32_t(*)[32]>(x + 32));
           const int key0 = (s.t0 + (j2 >> 1)) * kTileKeys + half * kHalfKeys;
           if (key0 + kHalfKeys > safe) {
             const int visible = lim - key0;
@@ -769,7 +746,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             for (int i = 0; i < 64; ++i)
               if (i >= visible) x[i] = 0xff800000u;
           }
-          // t = score * c + e
+          const Meta* m = meta + slot * kGroups + half * (kGroups / 2);
+          // t = score * c + e, c held above zero so that a masked score stays -inf
           float cand = -INFINITY;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
@@ -780,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
               a = fmax3(a, __uint_as_float(x[16 * g + i]), __uint_as_float(x[16 * g + i + 1]));
               b = fmax3(b, __uint_as_float(x[16 * g + i + 2]), __uint_as_float(x[16 * g + i + 3]));
             }
-            cand = fmaxf(cand, fmaf(fmaxf(a, b), c[g], e[g]));
+            cand = fmaxf(cand, fmaf(fmaxf(a, b), fmaxf(mul * m[g].ks, 1e-37f), m[g].e));
           }
           const bool grow = cand > ref + kGrowth;
           if (__any_sync(0xffffffffu, grow)) {
@@ -822,8 +800,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           uint32_t pk[32];
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const float sh = e[g] - r;
-            const uint64_t c2 = f2_pack(c[g], c[g]), s2 = f2_pack(sh, sh);
+            const float cs = fmaxf(mul * m[g].ks, 1e-37f), sh = m[g].e - r;
+            const uint64_t c2 = f2_pack(cs, cs), s2 = f2_pack(sh, sh);
             uint64_t sum = f2_pack(0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -837,14 +815,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             }
             float s0, s1;
             f2_unpack(sum, s0, s1);
-            l_run = fmaf(s0 + s1, back[g], l_run);
+            l_run = fmaf(s0 + s1, m[g].back, l_run);
           }
           tmem_st32(t_s + half * kHalfKeys, pk);
-          // The next half's scores, where they are there already (they never wait for these weights).
-          ready = j2 + 1 < 2 * s.n &&
-                  __all_sync(0xffffffffu, mbar_try_wait(smem_u32(&bars->s_full[t][half ^ 1]),
-                                                        ((seen + 1) >> 1) & 1));
-          if (ready) load_scores(half ^ 1);
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(&bars->p_full[t][half]);
