@@ -91,6 +91,7 @@ struct AttendParams {
   unsigned int* status;
   float* part_o;                  // partial outputs, maxima and sums (see sdpa_kv8.cu)
   float* part_ml;
+  int2* spans;                    // first and last run of a block of rows (see sdpa_kv8.cu)
   Cut* cuts;
   int B, Hq, Hkv, T, D, page, page_shift, width, num_pages, bf16, causal;
   int group;                      // Hq / Hkv, at most kMaxGroup
@@ -150,7 +151,11 @@ __host__ __device__ __forceinline__ int block_tiles(const SeqExtent& e, int rows
 // Work of the split kernel is a line of `total` tiles (sequence, then head and row block, then
 // keys), cut into `parts` equal runs: run i is [i * total / parts, (i + 1) * total / parts).
 __host__ __device__ __forceinline__ int64_t run_begin(int64_t i, int64_t total, int64_t parts) {
-  return i * total / parts;
+  // i total / parts without the 64-bit division where 32 bits do (parts < 2^16)
+  const int64_t each = total <= 0xffffffffll ? static_cast<uint32_t>(total) / static_cast<uint32_t>(parts)
+                                             : total / parts;
+  const uint32_t rest = static_cast<uint32_t>(total - each * parts);
+  return i * each + static_cast<uint32_t>(i) * rest / static_cast<uint32_t>(parts);
 }
 // The run that holds tile w.
 __host__ __device__ __forceinline__ int64_t run_of(int64_t w, int64_t total, int64_t parts) {

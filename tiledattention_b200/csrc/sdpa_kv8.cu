@@ -222,10 +222,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
     cur.h = hr / p.row_blocks;
     cur.rb = hr - cur.h * p.row_blocks;
   }
-  Cursor ahead = cur;  // the step whose K is copied next
-
-  auto advance = [&](Cursor& c) {
-    if (++c.tile < c.tiles) return;
+  auto next_rows = [&](Cursor& c) {  // to the next rows with tiles; none are behind the line's end
     c.tile = 0;
     if (++c.rb < p.row_blocks) return;
     c.rb = 0;
@@ -239,65 +236,69 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
     } while (c.tiles == 0);
   };
 
-  // The ring: unit 2 n is K of this warp's keys of step n, unit 2 n + 1 their V. A page id is
-  // fetched a step before its first use. Nothing is copied from the sequence's end on (whole
-  // boxes: the rest of its last page comes along), nor from pages outside the cache, whose
-  // blocks are marked in `left_out`, 4 steps' marks in turn.
+  // The ring: unit 2 n is K of this warp's keys of step n, unit 2 n + 1 their V. Lane l holds the
+  // planes (page, head) of the l-th of up to 32 steps from `ahead` on, fetched at once a step
+  // before the first of them; -1: behind the sequence's end, not copied (whole boxes: the rest
+  // of its last page comes along); -2: a page outside the cache, not copied, its block marked in
+  // `left_out` (4 steps' marks in turn).
   const uint32_t ring = smem_u32(smem) + warp * (kU * C::kUnit);
   const uint32_t scales = smem_u32(smem) + C::kScaleOff + warp * (C::kScaleSteps * 2 * kBlocks * 4);
   const int box = min(p.page, kKeys);
+  const int row_at = (warp * kKeys) & (p.page - 1);  // in its page: a tile is whole pages
+  const float* scale_of = p.scale[lane & 1];          // lane 2 i + kv copies the scale of block i
+  Cursor ahead = cur;
+  int held = 0, held_at = 0, held_plane[kBlocks];  // steps in the lanes, the next one to copy
+  int plane_at[kBlocks] = {-1, -1};                // of the step copied last
   uint32_t left_out = 0;
-  int page_next[kBlocks];                      // of `ahead`
-  int plane_at[kBlocks], row_at, boxes = 0;    // of the step whose V is copied next
-  auto fetch_pages = [&]() {
+  auto fetch_pages = [&](int left) {  // of the next steps, `left` before the run's end
+    held = min(min(ahead.tiles - ahead.tile, left), 32);
+    held_at = 0;
+    const int32_t* row = p.table + ahead.b * p.table_stride;
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) {
-      const int key = ahead.tile * C::kTile + warp * kKeys + i * 16;
-      page_next[i] = key < ahead.length
-                         ? p.table[ahead.b * p.table_stride + (key >> p.page_shift)] : 0;
+      const int key = (ahead.tile + lane) * C::kTile + warp * kKeys + i * 16;
+      held_plane[i] = -1;
+      if (lane < held && key < ahead.length) {
+        const int id = row[key >> p.page_shift];
+        const bool good = static_cast<unsigned>(id) < static_cast<unsigned>(p.num_pages);
+        held_plane[i] = good ? id * p.Hkv + ahead.h : -2;
+        if (!good && p.status) atomicOr(p.status, TA_DEVSTAT_BAD_PAGE);
+      }
     }
+    ahead.tile += held;
   };
   int issue_slot = 0;
   auto copy_unit = [&](const CUtensorMap* map) {
     if (lane == 0) {
       uint64_t* bar = full + issue_slot;
       const uint32_t dst = ring + issue_slot * C::kUnit;
-      mbar_arrive_expect_tx(bar, boxes * box * (C::kPlanes * C::kCols));
+      const bool first = plane_at[0] >= 0, second = box < kKeys && plane_at[1] >= 0;
+      mbar_arrive_expect_tx(bar, (first + second) * box * (C::kPlanes * C::kCols));
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i)
-        if (plane_at[i] >= 0 && (i * 16) % box == 0)
+        if (i == 0 ? first : second)
 #pragma unroll
           for (int c = 0; c < C::kPlanes; ++c)
-            tma_load_3d(dst + c * C::kPlane + i * 16 * C::kCols, map, bar, c * 128,
-                        (row_at + i * 16) & (p.page - 1), plane_at[i]);
+            tma_load_3d(dst + c * C::kPlane + i * 16 * C::kCols, map, bar, c * 128, row_at, plane_at[i]);
     }
     issue_slot = issue_slot + 1 == kU ? 0 : issue_slot + 1;
   };
-  auto copy_k = [&](int n) {  // step n, at `ahead`; then `ahead` moves on
+  auto copy_k = [&](int n) {
     if (n < steps) {
-      const int key0 = ahead.tile * C::kTile + warp * kKeys;
-      const uint32_t marks = (n & 3) * kBlocks;
-      left_out &= ~(((1u << kBlocks) - 1) << marks);
-      row_at = key0 & (p.page - 1);
-      boxes = 0;
+      const int slot4 = n & 3;
+      left_out &= ~(((1u << kBlocks) - 1) << (slot4 * kBlocks));
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
-        plane_at[i] = -1;
-        if (key0 + i * 16 >= ahead.length) continue;
-        if (static_cast<unsigned>(page_next[i]) >= static_cast<unsigned>(p.num_pages)) {
-          left_out |= 1u << (marks + i);
-          if (lane == 0 && p.status) atomicOr(p.status, TA_DEVSTAT_BAD_PAGE);
-          continue;
-        }
-        plane_at[i] = page_next[i] * p.Hkv + ahead.h;
-        if ((i * 16) % box == 0) ++boxes;
-        if (lane < 2)
-          cp_async4(scales + (((n & 3) * 2 + lane) * kBlocks + i) * 4, p.scale[lane] + plane_at[i]);
+        plane_at[i] = __shfl_sync(0xffffffffu, held_plane[i], held_at);
+        if (plane_at[i] == -2) left_out |= 1u << (slot4 * kBlocks + i);
       }
+      const int mine = lane < 2 ? plane_at[0] : plane_at[1];
+      if (lane < 2 * kBlocks && mine >= 0)
+        cp_async4(scales + ((slot4 * 2 + (lane & 1)) * kBlocks + (lane >> 1)) * 4, scale_of + mine);
       copy_unit(&map_k);
-      if (n + 1 < steps) {
-        advance(ahead);
-        fetch_pages();
+      if (++held_at == held && n + 1 < steps) {
+        if (ahead.tile == ahead.tiles) next_rows(ahead);
+        fetch_pages(steps - n - 1);
       }
     }
     cp_commit();
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
   auto copy_v = [&](int n) {
     if (n < steps) copy_unit(&map_v);
   };
-  fetch_pages();
+  fetch_pages(steps);
 #pragma unroll
   for (int u = 0; u < kU - 1; ++u) {
     if (u % 2 == 0) copy_k(u / 2);
@@ -339,12 +340,6 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
   bool fresh = true;
   int begin_tile = cur.tile;
   for (int step = 0; step < steps; ++step) {
-    wait_unit();
-    if (kU % 2 == 1) copy_k(step + kU / 2);  // unit 2 step + kU - 1
-    else copy_v(step + kU / 2 - 1);
-    cp_wait<(kU - 1) / 2>();
-    __syncwarp();
-
     if (fresh) {  // rows of a new (sequence, head): queries, limits, empty sums
       fresh = false;
       begin_tile = cur.tile;
@@ -414,6 +409,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
       safe = __reduce_min_sync(0xffffffffu, least);
       if constexpr (C::kQShared) __syncthreads();
     }
+    wait_unit();
+    if (kU % 2 == 1) copy_k(step + kU / 2);  // unit 2 step + kU - 1
+    else copy_v(step + kU / 2 - 1);
+    cp_wait<(kU - 1) / 2>();
+    __syncwarp();
 
     const int key0 = cur.tile * C::kTile + warp * kKeys;
     const bool any = key0 < cur.length;
@@ -611,6 +611,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
     const bool seq_end = cur.tile + 1 == cur.tiles;
     if (seq_end || step + 1 == steps) {
       const bool whole = seq_end && begin_tile == 0;
+      if (begin_tile == 0 && threadIdx.x == 0) {  // the runs with parts of these rows
+        const int64_t last = w0 + step - cur.tile + cur.tiles - 1;
+        p.spans[(static_cast<int64_t>(cur.b) * p.Hkv + cur.h) * p.row_blocks + cur.rb] =
+            make_int2(blockIdx.x, whole ? blockIdx.x : static_cast<int>(run_of(last, total, parts)));
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -701,7 +706,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
       fresh = true;
     }
     next_unit();
-    advance(cur);
+    if (seq_end) next_rows(cur);
+    else ++cur.tile;
   }
   if (*abort_flag) {  // a copy was late: every issued one must land before the block ends
     volatile int no_abort = 0;
@@ -716,77 +722,77 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
 // of sequences without keys. One block: kWarps rows, a warp each, or with `spread` one row
 // whose runs the warps divide (few rows, many runs).
 template <int NJ, int NT>
-__global__ void __launch_bounds__(kThreads) merge_kernel(const AttendParams p, int parts_max,
-                                                         int spread) {
+__global__ void __launch_bounds__(kThreads) merge_kernel(const AttendParams p, int parts, int spread) {
   using C = Cfg<NJ, NT>;
   constexpr int kVec = NJ <= 2 ? 1 : 2;  // float4 a lane: 32 lanes cover the head dim
-  __shared__ int64_t s_scan[kWarps];
   __shared__ float s_o[kWarps][NJ * 64];
   __shared__ float s_ml[kWarps][2];
-  __shared__ int64_t s_at;
-  __shared__ int s_tiles;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows = p.group * p.T;
   const int per = spread ? 1 : kWarps;
   const int row_groups = (rows + per - 1) / per;
-  const int rg = blockIdx.x % row_groups;
-  const int h = (blockIdx.x / row_groups) % p.Hkv;
-  const int b = blockIdx.x / row_groups / p.Hkv;
-  const int hrs = p.Hkv * p.row_blocks;
-  const Scan sc = scan_items<kWarps>(p.B, s_scan, [&](int i) {
-    return static_cast<int64_t>(tiles_of(extent_of(p, i), C::kTile)) * hrs;
-  });
-  {
-    int64_t at = sc.mine;
-    for (int i = sc.i0; i < sc.i1; ++i) {
-      const int n = tiles_of(extent_of(p, i), C::kTile);
-      if (i == b) {
-        s_at = at;
-        s_tiles = n;
-      }
-      at += static_cast<int64_t>(n) * hrs;
-    }
-  }
-  __syncthreads();
-  const int tiles = s_tiles;
+  const int bh = blockIdx.x / row_groups;
+  const int rg = blockIdx.x - bh * row_groups;
+  const int b = bh / p.Hkv, h = bh - b * p.Hkv;
   const int row = spread ? rg : rg * kWarps + warp;
   const int rb = row / C::kRows, r = row - rb * C::kRows;
-  const int64_t parts = min(static_cast<int64_t>(parts_max), sc.total);
-  int64_t i0 = 0, i1 = 0, first = 0;
-  if (tiles > 0) {
-    first = s_at + static_cast<int64_t>(h * p.row_blocks + rb) * tiles;
-    i0 = run_of(first, sc.total, parts);
-    i1 = run_of(first + tiles - 1, sc.total, parts);
+  const int tiles = tiles_of(extent_of(p, b), C::kTile);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int i0 = 0, i1 = 0;
+  if (row < rows) {
+    const int2 span = p.spans[static_cast<int64_t>(bh) * p.row_blocks + rb];  // unset without tiles
+    i0 = max(span.x, 0);  // in range even if the lengths changed after the runs were cut
+    i1 = min(span.y, parts - 1);
   }
   const bool mine = row < rows && !(tiles > 0 && i0 == i1);  // else that run wrote the row
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (spread && !mine) return;  // one row a block: all its threads alike
   float m = -INFINITY, l = 0.f;
   float4 a[kVec];
 #pragma unroll
   for (int v = 0; v < kVec; ++v) a[v] = make_float4(0.f, 0.f, 0.f, 0.f);
   if (mine && tiles > 0) {
-    const int64_t step = spread ? kWarps : 1;
-#pragma unroll 4
-    for (int64_t i = i0 + (spread ? warp : 0); i <= i1; i += step) {
-      // a run that begins at or before `first` has this head's first tile: its second slot
-      const int second = run_begin(i, sc.total, parts) <= first ? 1 : 0;
-      const int64_t at = (i * 2 + second) * C::kRows + r;
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-      const float mn = fmaxf(m, ml.x);
+    const int step = spread ? kWarps : 1;
+    constexpr int kAtOnce = 4;  // parts whose loads are in flight together
+    for (int i = i0 + (spread ? warp : 0); i <= i1; i += kAtOnce * step) {
+      float2 ml[kAtOnce];
+      float4 x[kAtOnce][kVec];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int run = i + k * step;
+        ml[k] = make_float2(-INFINITY, 0.f);  // no part: a sum and outputs of 0
+        // the run with this head's first tile left its part in its second slot
+        const int64_t at = (static_cast<int64_t>(run) * 2 + (run == i0 ? 1 : 0)) * C::kRows + r;
+        if (run <= i1) ml[k] = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) {
+          const int d = (v * 32 + lane) * 4;
+          x[k][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (run <= i1 && d < p.D) x[k][v] = *reinterpret_cast<const float4*>(p.part_o + at * C::kDim + d);
+        }
+      }
+      float mn = m;
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) mn = fmaxf(mn, ml[k].x);
       // without a maximum: sums of 0 or NaN and outputs of 0, kept as they are
       const float fa = m == -INFINITY ? 1.f : exp2f(m - mn);
-      const float fb = ml.x == -INFINITY ? 1.f : exp2f(ml.x - mn);
-      l = l * fa + ml.y * fb;
+      l *= fa;
 #pragma unroll
       for (int v = 0; v < kVec; ++v) {
-        const int d = (v * 32 + lane) * 4;
-        if (d < p.D) {
-          const float4 x = *reinterpret_cast<const float4*>(p.part_o + at * C::kDim + d);
-          a[v].x = a[v].x * fa + x.x * fb;
-          a[v].y = a[v].y * fa + x.y * fb;
-          a[v].z = a[v].z * fa + x.z * fb;
-          a[v].w = a[v].w * fa + x.w * fb;
+        a[v].x *= fa;
+        a[v].y *= fa;
+        a[v].z *= fa;
+        a[v].w *= fa;
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const float fb = ml[k].x == -INFINITY ? 1.f : exp2f(ml[k].x - mn);
+        l = fmaf(ml[k].y, fb, l);
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) {
+          a[v].x = fmaf(x[k][v].x, fb, a[v].x);
+          a[v].y = fmaf(x[k][v].y, fb, a[v].y);
+          a[v].z = fmaf(x[k][v].z, fb, a[v].z);
+          a[v].w = fmaf(x[k][v].w, fb, a[v].w);
         }
       }
       m = mn;
@@ -866,6 +872,7 @@ cudaError_t launch(AttendParams p, const CUtensorMap& map_k, const CUtensorMap& 
   const int parts = static_cast<int>(most < resident ? most : resident);
   const int64_t part_rows = resident * 2 * C::kRows;
   p.part_ml = p.part_o + part_rows * C::kDim;
+  p.spans = reinterpret_cast<int2*>(p.part_ml + part_rows * 2);
   kern<<<parts, kThreads, C::kBytes, stream>>>(map_k, map_v, p);
   if ((err = cudaGetLastError()) != cudaSuccess) return err;
 
@@ -917,10 +924,13 @@ auto with_config(int rows, int D, F f) {
 
 }  // namespace
 
-size_t attend_workspace_bytes(int, int Hq, int Hkv, int T, int D, int sm_count) {
-  return with_config((Hq / Hkv) * T, D, [&](auto shape) {
+size_t attend_workspace_bytes(int B, int Hq, int Hkv, int T, int D, int sm_count) {
+  const int rows = (Hq / Hkv) * T;
+  return with_config(rows, D, [&](auto shape) {
     using C = typename decltype(shape)::Config;
-    return static_cast<size_t>(C::kBlocksPerSm) * sm_count * 2 * C::kRows * (C::kDim + 2) * sizeof(float);
+    const size_t row_blocks = (rows + C::kRows - 1) / C::kRows;
+    return static_cast<size_t>(C::kBlocksPerSm) * sm_count * 2 * C::kRows * (C::kDim + 2) * sizeof(float) +
+           static_cast<size_t>(B) * Hkv * row_blocks * sizeof(int2);
   });
 }
 
