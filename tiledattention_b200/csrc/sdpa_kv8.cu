@@ -156,10 +156,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 __device__ __forceinline__ int tiles_of(const SeqExtent& e, int tile) {
   return e.count > 0 ? (e.length + tile - 1) / tile : 0;
 }
+// On the line, rows of one (sequence, head) take a unit for each tile, behind kBefore units for their
+// queries and their merge, which cost a block about the time of a tile.
+constexpr int kBefore = 1;
+__device__ __forceinline__ int units_of(int tiles) { return tiles > 0 ? tiles + kBefore : 0; }
 
-// A place on the line of tiles.
+// A place on the line.
 struct Cursor {
   int b, h, rb, tile, tiles, length;
+  int left;  // units to the run's end, this tile's included: none without a tile
 };
 
 template <int NJ, int NT>
@@ -190,18 +195,17 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
   const Scan sc = scan_items<kWarps>(p.B, s_scan, [&](int b) {
     const SeqExtent e = extent_of(p, b);
     report_extent(p, e);
-    return static_cast<int64_t>(tiles_of(e, C::kTile)) * hrs;
+    return static_cast<int64_t>(units_of(tiles_of(e, C::kTile))) * hrs;
   });
   const int64_t total = sc.total;
   const int64_t parts = min(static_cast<int64_t>(gridDim.x), total);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x >= parts) return;
-  const int64_t w0 = run_begin(blockIdx.x, total, parts);
-  const int steps = static_cast<int>(run_begin(blockIdx.x + 1, total, parts) - w0);
+  const int64_t w0 = run_begin(blockIdx.x, total, parts), w1 = run_begin(blockIdx.x + 1, total, parts);
   {
     int64_t at = sc.mine;
     for (int b = sc.i0; b < sc.i1; ++b) {
-      const int64_t n = static_cast<int64_t>(tiles_of(extent_of(p, b), C::kTile)) * hrs;
+      const int64_t n = static_cast<int64_t>(units_of(tiles_of(extent_of(p, b), C::kTile))) * hrs;
       if (at <= w0 && w0 < at + n) {
         s_start[0] = b;
         s_start[1] = static_cast<int>(w0 - at);  // < 2^31: checked by the launcher
@@ -217,12 +221,17 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
     const SeqExtent e = extent_of(p, cur.b);
     cur.length = e.length;
     cur.tiles = tiles_of(e, C::kTile);
-    const int hr = s_start[1] / cur.tiles;
-    cur.tile = s_start[1] - hr * cur.tiles;
+    const int hr = s_start[1] / units_of(cur.tiles);
+    const int at = s_start[1] - hr * units_of(cur.tiles);
+    cur.tile = max(0, at - kBefore);
     cur.h = hr / p.row_blocks;
     cur.rb = hr - cur.h * p.row_blocks;
+    cur.left = static_cast<int>(w1 - w0) - max(0, kBefore - at);
   }
-  auto next_rows = [&](Cursor& c) {  // to the next rows with tiles; none are behind the line's end
+  if (cur.left <= 0) return;  // a run without a tile
+  auto next_rows = [&](Cursor& c) {  // from a tile's end to the next rows with tiles, if any is left
+    if (c.left <= 0) return;
+    c.left -= kBefore;
     c.tile = 0;
     if (++c.rb < p.row_blocks) return;
     c.rb = 0;
@@ -250,8 +259,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
   int held = 0, held_at = 0, held_plane[kBlocks];  // steps in the lanes, the next one to copy
   int plane_at[kBlocks] = {-1, -1};                // of the step copied last
   uint32_t left_out = 0;
-  auto fetch_pages = [&](int left) {  // of the next steps, `left` before the run's end
-    held = min(min(ahead.tiles - ahead.tile, left), 32);
+  auto fetch_pages = [&]() {  // of the next steps: none at the run's end
+    held = max(0, min(min(ahead.tiles - ahead.tile, ahead.left), 32));
     held_at = 0;
     const int32_t* row = p.table + ahead.b * p.table_stride;
 #pragma unroll
@@ -266,6 +275,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
       }
     }
     ahead.tile += held;
+    ahead.left -= held;
   };
   int issue_slot = 0;
   auto copy_unit = [&](const CUtensorMap* map) {
@@ -283,8 +293,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
     }
     issue_slot = issue_slot + 1 == kU ? 0 : issue_slot + 1;
   };
+  bool copied_k = false;  // the copies of V follow those of K
   auto copy_k = [&](int n) {
-    if (n < steps) {
+    copied_k = held_at < held;
+    if (copied_k) {
       const int slot4 = n & 3;
       left_out &= ~(((1u << kBlocks) - 1) << (slot4 * kBlocks));
 #pragma unroll
@@ -296,22 +308,17 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
       if (lane < 2 * kBlocks && mine >= 0)
         cp_async4(scales + ((slot4 * 2 + (lane & 1)) * kBlocks + (lane >> 1)) * 4, scale_of + mine);
       copy_unit(&map_k);
-      if (++held_at == held && n + 1 < steps) {
+      if (++held_at == held) {
         if (ahead.tile == ahead.tiles) next_rows(ahead);
-        fetch_pages(steps - n - 1);
+        fetch_pages();
       }
     }
     cp_commit();
   };
-  auto copy_v = [&](int n) {
-    if (n < steps) copy_unit(&map_v);
+  auto copy_v = [&]() {
+    if (copied_k) copy_unit(&map_v);
   };
-  fetch_pages(steps);
-#pragma unroll
-  for (int u = 0; u < kU - 1; ++u) {
-    if (u % 2 == 0) copy_k(u / 2);
-    else copy_v(u / 2);
-  }
+  fetch_pages();
 
   int slot = 0;
   uint32_t parity = 0;
@@ -338,9 +345,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
   uint4* s_q = reinterpret_cast<uint4*>(smem + C::kQOff);
   int safe = 0;  // keys that every row with any keys sees
   bool fresh = true;
+  int steps = 0;
   int begin_tile = cur.tile;
-  for (int step = 0; step < steps; ++step) {
-    if (fresh) {  // rows of a new (sequence, head): queries, limits, empty sums
+  // Unit u + kU - 1 is copied when unit u is waited for, so kU / 2 steps without work come first.
+  for (int step = -(kU / 2);; ++step) {
+    if (step >= 0 && fresh) {  // rows of a new (sequence, head): queries, limits, empty sums
       fresh = false;
       begin_tile = cur.tile;
       const SeqExtent e = extent_of(p, cur.b);
@@ -409,9 +418,14 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
       safe = __reduce_min_sync(0xffffffffu, least);
       if constexpr (C::kQShared) __syncthreads();
     }
-    wait_unit();
+    if (step >= 0) wait_unit();
     if (kU % 2 == 1) copy_k(step + kU / 2);  // unit 2 step + kU - 1
-    else copy_v(step + kU / 2 - 1);
+    else copy_v();
+    if (step < 0) {
+      if (kU % 2 == 1) copy_v();
+      else copy_k(step + kU / 2);
+      continue;
+    }
     cp_wait<(kU - 1) / 2>();
     __syncwarp();
 
@@ -545,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
     }
 
     wait_unit();
-    if (kU % 2 == 1) copy_v(step + kU / 2);  // unit 2 step + 1 + kU - 1
+    if (kU % 2 == 1) copy_v();  // unit 2 step + 1 + kU - 1
     else copy_k(step + kU / 2);
     if (any) {
       const uint32_t vb = ring + slot * C::kUnit;
@@ -609,10 +623,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
 
     // ---- the end of this (sequence, head) or of the run: merge the warps
     const bool seq_end = cur.tile + 1 == cur.tiles;
-    if (seq_end || step + 1 == steps) {
+    if (seq_end || cur.left == 1) {
       const bool whole = seq_end && begin_tile == 0;
       if (begin_tile == 0 && threadIdx.x == 0) {  // the runs with parts of these rows
-        const int64_t last = w0 + step - cur.tile + cur.tiles - 1;
+        const int64_t last = w1 - cur.left - cur.tile + cur.tiles - 1;
         p.spans[(static_cast<int64_t>(cur.b) * p.Hkv + cur.h) * p.row_blocks + cur.rb] =
             make_int2(blockIdx.x, whole ? blockIdx.x : static_cast<int>(run_of(last, total, parts)));
       }
@@ -706,8 +720,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
       fresh = true;
     }
     next_unit();
+    --cur.left;
     if (seq_end) next_rows(cur);
     else ++cur.tile;
+    ++steps;
+    if (cur.left <= 0) break;
   }
   if (*abort_flag) {  // a copy was late: every issued one must land before the block ends
     volatile int no_abort = 0;
@@ -863,9 +880,9 @@ cudaError_t launch(AttendParams p, const CUtensorMap& map_k, const CUtensorMap& 
   }
   const int rows = p.group * p.T;
   p.row_blocks = (rows + C::kRows - 1) / C::kRows;
-  // Most tiles that the lengths can ask for; more blocks than that would have none.
+  // Most units that the lengths can ask for; more blocks than that would have none.
   const int64_t seq_tiles = (static_cast<int64_t>(p.width) * p.page + C::kTile - 1) / C::kTile;
-  const int64_t per_seq = seq_tiles * p.Hkv * p.row_blocks;
+  const int64_t per_seq = (seq_tiles + kBefore) * p.Hkv * p.row_blocks;
   if (per_seq > 0x7fffffffll) return cudaErrorInvalidValue;
   const int64_t most = per_seq * p.B;
   const int64_t resident = static_cast<int64_t>(C::kBlocksPerSm) * sm_count;
