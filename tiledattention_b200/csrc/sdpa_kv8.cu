@@ -157,8 +157,10 @@ __device__ __forceinline__ int tiles_of(const SeqExtent& e, int tile) {
   return e.count > 0 ? (e.length + tile - 1) / tile : 0;
 }
 // On the line, rows of one (sequence, head) take a unit for each tile, behind kBefore units for their
-// queries and their merge, which cost a block about the time of a tile.
-constexpr int kBefore = 1;
+// queries and their merge. Without these units a run over many short sequences ends last (32
+// sequences of up to 4096: 45.8 us); with 1, 2, 3 it is 37.1, 35.0, 34.9 us, and 5 tokens of 8
+// sequences at head dim 256 take 39.3, 36.9, 36.9 us.
+constexpr int kBefore = 2;
 __device__ __forceinline__ int units_of(int tiles) { return tiles > 0 ? tiles + kBefore : 0; }
 
 // A place on the line.
@@ -189,6 +191,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
     fence_mbar_init();
     if (warp == 0) *abort_flag = 0;
   }
+  // Launched before the kernel before it has ended (programmatic launch: 2 us of 35 saved in a row of
+  // calls): nothing that it may write is read above this line. The merge kernel does not let the
+  // next call in before its own end: blocks that came while it ran made a call of 64 sequences
+  // of 16384 take 430 us for 350.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // This block's run of the line, and the sequence it begins in.
   const int hrs = p.Hkv * p.row_blocks;
@@ -890,22 +897,24 @@ cudaError_t launch(AttendParams p, const CUtensorMap& map_k, const CUtensorMap& 
   const int64_t part_rows = resident * 2 * C::kRows;
   p.part_ml = p.part_o + part_rows * C::kDim;
   p.spans = reinterpret_cast<int2*>(p.part_ml + part_rows * 2);
-  kern<<<parts, kThreads, C::kBytes, stream>>>(map_k, map_v, p);
-  if ((err = cudaGetLastError()) != cudaSuccess) return err;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kBytes;
+  cfg.stream = stream;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  if ((err = cudaLaunchKernelEx(&cfg, kern, map_k, map_v, p)) != cudaSuccess) return err;
 
   const int64_t few = static_cast<int64_t>(p.B) * p.Hkv * rows;
   const int spread = few <= 2ll * sm_count ? 1 : 0;
   const int64_t blocks = spread ? few : static_cast<int64_t>(p.B) * p.Hkv * ((rows + kWarps - 1) / kWarps);
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-  cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, merge_kernel<NJ, NT>, p, parts, spread);
 }
 
