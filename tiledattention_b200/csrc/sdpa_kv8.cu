@@ -62,10 +62,12 @@ struct Cfg {
   static constexpr int kPlane = kKeys * kCols;
   static constexpr int kUnit = kPlanes * kPlane;   // K or V bytes of a warp's step
   // Blocks a SM, as the registers allow (the output takes 16 NJ NT of them, q 8 NJ NT where it
-  // is not shared), and the ring's units, as shared memory then allows.
+  // is not shared), and the ring's units, as shared memory then allows. One block more costs
+  // spills and time: 16 sequences of 8192, 8 heads, head dim 128, 16 rows 91 us with 3 blocks,
+  // 64 with 2; head dim 64, 32 rows 101 and 68.
   static constexpr bool kQShared = NJ * NT > 6;
-  static constexpr int kBlocksPerSm = NJ <= 2 ? (NJ * NT <= 2 ? 4 : NJ * NT <= 4 ? 3 : 2) : 2;
-  static constexpr int kUnits = NJ == 1 ? 6 : NJ == 2 ? (kBlocksPerSm == 4 ? 3 : kBlocksPerSm == 3 ? 4 : 5) : 3;
+  static constexpr int kBlocksPerSm = NJ * NT == 1 ? 4 : NJ * NT == 2 ? 3 : 2;
+  static constexpr int kUnits = NJ == 1 ? 6 : NJ == 2 ? (NT == 1 ? 4 : NT == 2 ? 6 : 5) : 3;
   static constexpr int kScaleSteps = 4;  // steps whose scales are kept: more than units ahead / 2
   // merge: a unit holds kRows x kMergeCols floats
   static constexpr int kMergeCols = kUnit / (kRows * 4) < kDim ? kUnit / (kRows * 4) : kDim;
@@ -77,7 +79,8 @@ struct Cfg {
   static constexpr int kMlOff = kScaleOff + kScaleBytes;
   static constexpr int kBarOff = kMlOff + 2 * kWarps * kRows * 4;
   static constexpr int kScanOff = kBarOff + kWarps * kUnits * 8;
-  static constexpr int kBytes = kScanOff + 64 + 1024;  // slack: units are 1024-byte aligned
+  static constexpr int kRowsOff = kScanOff + 64;
+  static constexpr int kBytes = kRowsOff + (kQShared ? 2 * kWarps * kRows * 4 : 0) + 1024;  // slack: units are 1024-byte aligned
 };
 constexpr uint64_t kTimeoutNs = 1000000000ull;  // 1 s per wait for a copy
 
@@ -346,8 +349,21 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
 
   // Of 8-row tile nt a thread holds rows 2t and 2t + 1 of scores and output, row g of q.
   float o[NJ * 4][NT][4];  // 16 dims: (g, 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1)
-  float ref[NT][2], l_run[NT][2], mul[NT][2];
-  int lim[NT][2];
+  float ref[NT][2], l_run[NT][2];
+  // A row's factor of the scores and its limit: in registers, or where q is shared in shared memory
+  // (a copy for each warp).
+  float mul[C::kQShared ? 1 : NT][2];
+  int lim[C::kQShared ? 1 : NT][2];
+  float* s_mul = reinterpret_cast<float*>(smem + C::kRowsOff) + warp * C::kRows;
+  int* s_lim = reinterpret_cast<int*>(smem + C::kRowsOff) + (kWarps + warp) * C::kRows;
+  auto factors = [&](int nt) {
+    if constexpr (C::kQShared) return *reinterpret_cast<const float2*>(s_mul + nt * 8 + 2 * t);
+    else return make_float2(mul[nt][0], mul[nt][1]);
+  };
+  auto limit_of = [&](int nt, int r) {
+    if constexpr (C::kQShared) return s_lim[nt * 8 + 2 * t + r];
+    else return lim[nt][r];
+  };
   uint32_t qf[C::kQShared ? 1 : NT][NJ * 4][2];  // chunk, pair of dims
   uint4* s_q = reinterpret_cast<uint4*>(smem + C::kQOff);
   int safe = 0;  // keys that every row with any keys sees
@@ -414,10 +430,18 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
             qf[nt][c][1] = f[c][1];
           }
         }
+        if constexpr (C::kQShared) {
+          if (t == 0) {
+            s_mul[nt * 8 + g] = factor;
+            s_lim[nt * 8 + g] = limit;
+          }
+        }
 #pragma unroll
-        for (int r2 = 0; r2 < 2; ++r2) {  // from row g's lanes to those of columns 2t, 2t + 1
-          lim[nt][r2] = __shfl_sync(0xffffffffu, limit, (2 * t + r2) * 4);
-          mul[nt][r2] = __shfl_sync(0xffffffffu, factor, (2 * t + r2) * 4);
+        for (int r2 = 0; r2 < 2; ++r2) {
+          if constexpr (!C::kQShared) {  // from row g's lanes to those of columns 2t, 2t + 1
+            lim[nt][r2] = __shfl_sync(0xffffffffu, limit, (2 * t + r2) * 4);
+            mul[nt][r2] = __shfl_sync(0xffffffffu, factor, (2 * t + r2) * 4);
+          }
           ref[nt][r2] = -INFINITY;
           l_run[nt][r2] = 0.f;
         }
@@ -475,35 +499,34 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
 
     uint32_t pf[kBlocks][NT][2];  // weights as the second product's B: set 0, set 1
     if (any) {
-      // t = score * c + e: the scales of the block's page
-      float c[kBlocks][NT][2], e[kBlocks], back[kBlocks];
+      // t = score * c + ev in the scores' place, by the scales of the block's page
+      float back[kBlocks];
       const uint32_t marks = left_out >> ((step & 3) * kBlocks) & ((1u << kBlocks) - 1);
+      const bool masked = key0 + kKeys > safe || marks;  // some row's limit, or pages to leave out
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
         const uint32_t at = scales + ((step & 3) * 2 * kBlocks + i) * 4;
         const float ks = lds32(at);
         const int ev = stored_exponent(__float_as_uint(lds32(at + kBlocks * 4)));
+        const float e = static_cast<float>(ev);
         back[i] = pow2f(-ev);
-        e[i] = static_cast<float>(ev);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          c[i][nt][0] = mul[nt][0] * ks;
-          c[i][nt][1] = mul[nt][1] * ks;
+          const float2 f = factors(nt);
+          const float c0 = f.x * ks, c1 = f.y * ks;
+          s[i][nt][0] = fmaf(s[i][nt][0], c0, e);
+          s[i][nt][1] = fmaf(s[i][nt][1], c1, e);
+          s[i][nt][2] = fmaf(s[i][nt][2], c0, e);
+          s[i][nt][3] = fmaf(s[i][nt][3], c1, e);
         }
-      }
-      if (key0 + kKeys > safe || marks) {  // some row's limit, or pages to leave out
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
+        if (masked) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               const int key = marks >> i & 1 ? 0x7fffffff : key0 + i * 16 + key_of_column(g, x >> 1);
-              s[i][nt][x] = key < lim[nt][x & 1] ? fmaf(s[i][nt][x], c[i][nt][x & 1], e[i]) : -INFINITY;
+              if (key >= limit_of(nt, x & 1)) s[i][nt][x] = -INFINITY;
             }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) c[i][nt][0] = c[i][nt][1] = 1.f;
-          e[i] = 0.f;
         }
       }
       float cand[NT][2];
@@ -514,8 +537,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
         for (int r = 0; r < 2; ++r) {
           float m = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < kBlocks; ++i)
-            m = fmaxf(m, fmaf(fmaxf(s[i][nt][r], s[i][nt][2 + r]), c[i][nt][r], e[i]));
+          for (int i = 0; i < kBlocks; ++i) m = fmaxf(m, fmaxf(s[i][nt][r], s[i][nt][2 + r]));
           cand[nt][r] = m;
           grow |= m > ref[nt][r] + kGrowth;
         }
@@ -553,10 +575,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) {
           const float(&x)[4] = s[i][nt];
-          const float w0 = ex2_approx(fmaf(x[0], c[i][nt][0], e[i] - r0));
-          const float w1 = ex2_approx(fmaf(x[1], c[i][nt][1], e[i] - r1));
-          const float w2 = ex2_approx(fmaf(x[2], c[i][nt][0], e[i] - r0));
-          const float w3 = ex2_approx(fmaf(x[3], c[i][nt][1], e[i] - r1));
+          const float w0 = ex2_approx(x[0] - r0);
+          const float w1 = ex2_approx(x[1] - r1);
+          const float w2 = ex2_approx(x[2] - r0);
+          const float w3 = ex2_approx(x[3] - r1);
           l_run[nt][0] = fmaf(w0 + w2, back[i], l_run[nt][0]);
           l_run[nt][1] = fmaf(w1 + w3, back[i], l_run[nt][1]);
           pf[i][nt][0] = transpose8(pack_f16(w0, w1));
@@ -597,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
                   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
-                      if (key0 + i * 16 + key < lim[nt][r])
+                      if (key0 + i * 16 + key < limit_of(nt, r))
                         o[m][nt][2 * hi + r] = __int_as_float(0x7fffffff);
                 }
             __syncwarp();
@@ -641,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          if (lim[nt][r] == 0) {  // a row without keys: its unmasked scores were of no row
+          if (limit_of(nt, r) == 0) {  // a row without keys: its unmasked scores were of no row
             ref[nt][r] = -INFINITY;
             l_run[nt][r] = 0.f;
           }
