@@ -26,7 +26,7 @@ SOURCES = ["capi.cu", "sdpa_fwd_sm100.cu", "sdpa_fwd_sm100_shared_kv.cu", "lse_c
            "rotary.cu", "kv8_append.cu", "sdpa_kv8.cu",
            "sdpa_kv8_chunk.cu", "capi_serving.cu"]
 HEADERS = ["sm100_ptx.cuh", "sdpa_common.cuh", "sdpa_fwd_sm100.h", "lse_combine.h", "capi_internal.h",
-           "rotary.h", "kv8.h", "kv8_device.cuh"]
+           "rotary.h", "kv8.h", "kv8_device.cuh", "overlapped_launch.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # One-call host launcher (CPython extension over libtorch; no device code): see
 # csrc/fast_launch.cpp.

@@ -14,6 +14,7 @@
 #include <stdint.h>
 
 #include "kv8.h"
+#include "overlapped_launch.cuh"
 #include "tiledattention_b200.h"
 
 namespace ta {
@@ -94,6 +95,7 @@ __device__ __forceinline__ float pow2f(int e) {
 
 template <bool BF16>
 __global__ void __launch_bounds__(128) append_kernel(const AppendParams p, int slots) {
+  wait_for_stream();
   const int b = blockIdx.x / slots;
   const int h = blockIdx.y;
   const int kind = blockIdx.z;
@@ -194,9 +196,7 @@ cudaError_t launch_append(const AppendParams& p, cudaStream_t stream) {
   const int64_t blocks = static_cast<int64_t>(p.B) * slots;
   if (blocks > 0x7fffffffll || p.Hkv > 65535) return cudaErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(blocks), p.Hkv, 2);
-  if (p.bf16) append_kernel<true><<<grid, 128, 0, stream>>>(p, slots);
-  else append_kernel<false><<<grid, 128, 0, stream>>>(p, slots);
-  return cudaGetLastError();
+  return launch_overlapped(p.bf16 ? append_kernel<true> : append_kernel<false>, grid, 128, 0, stream, p, slots);
 }
 
 }  // namespace kv8

@@ -8,6 +8,7 @@
 #include <stdint.h>
 
 #include "kv8.h"
+#include "overlapped_launch.cuh"
 #include "sm100_ptx.cuh"
 #include "tiledattention_b200.h"
 

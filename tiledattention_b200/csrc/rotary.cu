@@ -16,6 +16,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "overlapped_launch.cuh"
 #include "rotary.h"
 
 namespace ta {
@@ -112,6 +113,7 @@ template <bool BF16, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads)
     rotary_vector_kernel(const RotaryParams p, int n_slots, int heads_per_thread) {
   constexpr int kAhead = 4;
+  wait_for_stream();
   const Place at = place_of(p, n_slots);
   if (!at.ok) return;
   const int heads = p.t[0].heads + p.t[1].heads;
@@ -176,6 +178,7 @@ __global__ void __launch_bounds__(kThreads)
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads)
     rotary_scalar_kernel(const RotaryParams p, int n_slots, int heads_per_thread) {
+  wait_for_stream();
   const Place at = place_of(p, n_slots);
   if (!at.ok) return;
   const int b = at.b, s = at.s;
@@ -222,19 +225,13 @@ cudaError_t launch_rotary(const RotaryParams& p, bool vector, int sm_count, cuda
   while (hpt > 1 && blocks * ((heads + hpt - 1) / hpt) < want) hpt /= 2;
   while ((heads + hpt - 1) / hpt > 65535) hpt *= 2;
   const dim3 grid(static_cast<unsigned>(blocks), (heads + hpt - 1) / hpt);
-  if (vector) {
-    if (p.interleaved) {
-      if (p.bf16) rotary_vector_kernel<true, true><<<grid, kThreads, 0, stream>>>(p, n_slots, hpt);
-      else rotary_vector_kernel<false, true><<<grid, kThreads, 0, stream>>>(p, n_slots, hpt);
-    } else {
-      if (p.bf16) rotary_vector_kernel<true, false><<<grid, kThreads, 0, stream>>>(p, n_slots, hpt);
-      else rotary_vector_kernel<false, false><<<grid, kThreads, 0, stream>>>(p, n_slots, hpt);
-    }
-  } else {
-    if (p.bf16) rotary_scalar_kernel<true><<<grid, kThreads, 0, stream>>>(p, n_slots, hpt);
-    else rotary_scalar_kernel<false><<<grid, kThreads, 0, stream>>>(p, n_slots, hpt);
-  }
-  return cudaGetLastError();
+  const auto launch = [&](auto kernel) {
+    return launch_overlapped(kernel, grid, kThreads, 0, stream, p, n_slots, hpt);
+  };
+  if (!vector) return p.bf16 ? launch(rotary_scalar_kernel<true>) : launch(rotary_scalar_kernel<false>);
+  if (p.interleaved)
+    return p.bf16 ? launch(rotary_vector_kernel<true, true>) : launch(rotary_vector_kernel<false, true>);
+  return p.bf16 ? launch(rotary_vector_kernel<true, false>) : launch(rotary_vector_kernel<false, false>);
 }
 
 }  // namespace ta

@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
   // calls): nothing that it may write is read above this line. The merge kernel does not let the
   // next call in before its own end: blocks that came while it ran made a call of 64 sequences
   // of 16384 take 430 us for 350.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_stream();
 
   // This block's run of the line, and the sequence it begins in.
   const int hrs = p.Hkv * p.row_blocks;
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
   });
   const int64_t total = sc.total;
   const int64_t parts = min(static_cast<int64_t>(gridDim.x), total);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_next_kernel_in();
   if (blockIdx.x >= parts) return;
   const int64_t w0 = run_begin(blockIdx.x, total, parts), w1 = run_begin(blockIdx.x + 1, total, parts);
   {
@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const AttendParams p, i
   const int row = spread ? rg : rg * kWarps + warp;
   const int rb = row / C::kRows, r = row - rb * C::kRows;
   const int tiles = tiles_of(extent_of(p, b), C::kTile);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_stream();
   int i0 = 0, i1 = 0;
   if (row < rows) {
     const int2 span = p.spans[static_cast<int64_t>(bh) * p.row_blocks + rb];  // unset without tiles
@@ -919,25 +919,16 @@ cudaError_t launch(AttendParams p, const CUtensorMap& map_k, const CUtensorMap& 
   const int64_t part_rows = resident * 2 * C::kRows;
   p.part_ml = p.part_o + part_rows * C::kDim;
   p.spans = reinterpret_cast<int2*>(p.part_ml + part_rows * 2);
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(parts));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::kBytes;
-  cfg.stream = stream;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  if ((err = cudaLaunchKernelEx(&cfg, kern, map_k, map_v, p)) != cudaSuccess) return err;
+  err = launch_overlapped(kern, dim3(static_cast<unsigned>(parts)), kThreads, C::kBytes, stream, map_k,
+                          map_v, p);
+  if (err != cudaSuccess) return err;
 
   const int64_t few = static_cast<int64_t>(p.B) * p.Hkv * rows;
   const int spread = few <= 2ll * sm_count ? 1 : 0;
   const int64_t blocks = spread ? few : static_cast<int64_t>(p.B) * p.Hkv * ((rows + kWarps - 1) / kWarps);
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, merge_kernel<NJ, NT>, p, parts, spread);
+  return launch_overlapped(merge_kernel<NJ, NT>, dim3(static_cast<unsigned>(blocks)), kThreads, 0, stream,
+                           p, parts, spread);
 }
 
 // One configuration, as an argument.

@@ -245,6 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
   Barriers* bars = reinterpret_cast<Barriers*>(smem + C::kBarOff);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  wait_for_stream();
 
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
   };
   const Scan sc = scan_items<kWarps>(p.B * p.row_blocks, start->scan, item_work);  // has a barrier
   tc_fence_after();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_next_kernel_in();
   const uint32_t tmem = bars->tmem_base;
   const int64_t parts = min(static_cast<int64_t>(gridDim.x), sc.total);
   const bool has_run = blockIdx.x < parts;
@@ -917,7 +918,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttendParams p) {
   constexpr int kVec = D / 32;
   constexpr int kStride = D + 8;  // of a row of the 16-bit tile, values
   __shared__ __align__(16) uint16_t tile[32 * kStride];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_stream();
   const Cut cut = p.cuts[blockIdx.x];
   if (cut.first < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1011,19 +1012,10 @@ cudaError_t launch(AttendParams p, int sm_count, cudaStream_t stream) {
   const int64_t part_rows = static_cast<int64_t>(sm_count) * 2 * C::kRows;
   p.part_ml = p.part_o + part_rows * D;
   p.cuts = reinterpret_cast<Cut*>(p.part_ml + part_rows * 2);
-  kern<<<parts, kThreads, C::kBytes, stream>>>(p);
-  if ((err = cudaGetLastError()) != cudaSuccess) return err;
-  cudaLaunchConfig_t cfg{};
+  err = launch_overlapped(kern, dim3(parts), kThreads, C::kBytes, stream, p);
+  if (err != cudaSuccess) return err;
   const int merged = static_cast<int>(rows < C::kRows ? rows : C::kRows);
-  cfg.gridDim = dim3(parts, (merged + 31) / 32);
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, merge_kernel<D>, p);
+  return launch_overlapped(merge_kernel<D>, dim3(parts, (merged + 31) / 32), 256, 0, stream, p);
 }
 
 }  // namespace
