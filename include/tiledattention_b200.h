@@ -234,8 +234,8 @@ int ta_kv8_append(const void* k, const void* v, const int64_t* k_strides, const 
 
 /*
  * ta_sdpa_kv8 — o = softmax(scale q K^T + mask) V of T query rows per sequence over the cached
- * tokens [0, lengths[b]) of sequence b, for Hq = G * Hkv query heads (head h reads cache head
- * h / G). counts[b] (null: T) of the T rows are real; they are the sequence's last tokens, so
+ * tokens [0, lengths[b]) of sequence b, for Hq = G * Hkv query heads, G <= 256 and G * T < 2^24
+ * (head h reads cache head h / G). counts[b] (null: T) of the T rows are real; they are the sequence's last tokens, so
  * with causal = 1 row t sees keys [0, lengths[b] - counts[b] + t]; with causal = 0 all
  * lengths[b]. Rows without a key, and rows from counts[b] on, give o = 0 and lse = -inf.
  *   q, o        device, `dtype`, [B,Hq,T,D] with element strides (multiples of 16 bytes)

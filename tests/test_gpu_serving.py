@@ -636,3 +636,131 @@ def test_decoding_loop_over_the_operators():
     # exactly: the last step is attention over what the cache now holds
     want, _, tol, _ = plain.attend64(qr[:, :, -1:], *cache, table, [total] * B)
     _within(got[:, :, -1:], want, tol)
+
+
+@pytest.mark.parametrize("Hq,Hkv,T,D", [(8, 2, 1, 128), (20, 2, 2, 256), (6, 2, 5, 64), (8, 1, 4, 128),
+                                        (4, 2, 40, 128), (2, 1, 70, 64)])
+def test_lines_of_short_and_long_sequences(Hq, Hkv, T, D):
+    """Sequences without keys, of one token and of many in one batch: runs that hold many whole
+    sequences beside runs of a part of one."""
+    B = 48
+    lengths = [(0, 1, T, 17, 300, 64)[b % 6] for b in range(B)]
+    lengths[7], lengths[20], lengths[B - 1] = 5000, 2049, 0
+    counts = [min(T, n) if b % 5 else max(0, min(T, n) - 1) for b, n in enumerate(lengths)]
+    _attend_case(B, Hq, Hkv, T, D, 32, lengths, counts, BF16, seed=T)
+    _attend_case(B, Hq, Hkv, T, D, 32, [0] * B, [0] * B, BF16, seed=T)
+
+
+@pytest.mark.parametrize("D,T", [(128, 32), (128, 33), (192, 48), (192, 49), (256, 48), (256, 49)])
+def test_border_of_the_two_kernels(D, T):
+    _attend_case(3, 2, 2, T, D, 64, [T, 700, 129 + T], None, FP16, seed=T)
+
+
+@pytest.mark.parametrize("Hq,Hkv,T,D", [(8, 2, 1, 128), (8, 2, 8, 128), (4, 2, 60, 128), (4, 1, 30, 256)])
+def test_calls_at_once_and_graphs(Hq, Hkv, T, D):
+    """The same bits from calls in a row, on two streams at once, and from two captured graphs
+    replayed in turn with lengths, table and queries that have changed since."""
+    import tiledattention_b200 as ta
+
+    B, page = 5, 16
+    cache = ta.KVCache8(*plain.make_cache(B * 70 + 2, Hkv, page, D, 1, DEV))
+    table = _table(B, 70, B * 70 + 2, 2)
+    lengths = _ints([1100, T, 77 + T, 640, 1001])
+    q = _randn(B, Hq, T, D, seed=3)
+    want = ta.sdpa_kv_cache(q, cache, table, lengths)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = [ta.sdpa_kv_cache(q, cache, table, lengths) for _ in range(20)]
+    got += [ta.sdpa_kv_cache(q, cache, table, lengths) for _ in range(20)]
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(x, want) for x in got)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = ta.sdpa_kv_cache(q, cache, table, lengths, return_lse=True)
+        graphs.append((g, out))
+    for n in ([T, 1100, 900, T + 1, 20 + T], [T] * 5, [1120] * 5):
+        lengths.copy_(_ints(n))
+        q.copy_(_randn(B, Hq, T, D, seed=sum(n)))
+        table.copy_(table.roll(1, 0))
+        for g, out in graphs * 2:
+            out[0].fill_(7), out[1].fill_(7)
+            g.replay()
+            fresh = ta.sdpa_kv_cache(q, cache, table, lengths, return_lse=True)
+            assert torch.equal(out[0], fresh[0]) and torch.equal(out[1], fresh[1])
+    ta.check_device_status(DEV)
+
+
+def test_each_call_sees_what_the_one_before_wrote():
+    """Rotation, write and attention in a row over one set of buffers, eagerly and in a graph,
+    against the same calls with the device idle between them."""
+    import tiledattention_b200 as ta
+
+    B, Hq, Hkv, D, page, steps = 4, 8, 2, 128, 16, 24
+    freq, mag = ta.rotary_frequencies(D, device=DEV)
+    q, k, v = (_randn(B, h, 1, D, seed=i) for i, h in enumerate((Hq, Hkv, Hkv)))
+    table = _table(B, 4, B * 4, 1)
+
+    def step(cache, at, x, idle):
+        pos = at.view(B, 1)
+        qr, kr = ta.rotary(x, k, pos, freq, magnitude=mag)
+        idle()
+        ta.kv_cache_append(kr, v, cache, table, at)
+        idle()
+        at += 1
+        idle()
+        out = ta.sdpa_kv_cache(qr, cache, table, at)
+        idle()
+        x.copy_(out)  # the next query
+        idle()
+
+    def run(idle):
+        cache, at, x = ta.kv_cache_alloc(B * 4, Hkv, page, D, device=DEV), _ints([0, 3, 15, 30]), q.clone()
+        for _ in range(steps):
+            step(cache, at, x, idle)
+        return x, cache
+
+    want, want_cache = run(torch.cuda.synchronize)
+    got, cache = run(lambda: None)
+    same = lambda a, b: all(torch.equal(s.view(torch.uint8), t.view(torch.uint8)) for s, t in zip(a, b))
+    assert torch.equal(got, want) and same(cache, want_cache)
+    cache, at, x = ta.kv_cache_alloc(B * 4, Hkv, page, D, device=DEV), _ints([0, 3, 15, 30]), q.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for _ in range(4):
+            step(cache, at, x, lambda: None)
+    for _ in range(steps // 4):
+        g.replay()
+    assert torch.equal(x, want) and same(cache, want_cache)
+    ta.check_device_status(DEV)
+
+
+def test_heads_beyond_a_group_are_refused():
+    import tiledattention_b200 as ta
+
+    cache = ta.KVCache8(*plain.make_cache(2, 1, 16, 64, 1, DEV))
+    with pytest.raises(ta.InvalidShapeError, match="256 query heads"):
+        ta.sdpa_kv_cache(_randn(1, 257, 1, 64), cache, _ints([[0, 1]]), _ints([20]))
+    _attend_case(1, 256, 1, 1, 64, 16, [20], None, BF16)
+
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_short_workspaces_are_refused(T):
+    from tiledattention_b200 import _native, _runtime
+
+    lib = _runtime.get_native_library()
+    cache = plain.make_cache(2, 2, 16, 64, 1, DEV)
+    q, table, lengths = _randn(1, 4, T, 64), _ints([[0, 1]]), _ints([20])
+    out = torch.full_like(q, 7)
+    need = lib.ta_sdpa_kv8_workspace(1, 4, 2, T, 64)
+    work = torch.empty(need + 16, dtype=torch.uint8, device=DEV)
+    for at, size in ((0, need - 1), (0, 0), (0, -1), (8, need)):
+        rc = lib.ta_sdpa_kv8(
+            q.data_ptr(), _native.strides4(q.stride()), out.data_ptr(), _native.strides4(out.stride()), None,
+            *(t.data_ptr() for t in cache), 2, 16, table.data_ptr(), 2, 2, lengths.data_ptr(), None, 1, 4, 2,
+            T, 64, 1, 1, 0.1, work.data_ptr() + at, size, None, torch.cuda.current_stream().cuda_stream)
+        assert rc == _native.TA_ERR_INVALID_ARGUMENT, (at, size)
+    torch.cuda.synchronize()
+    assert (out == 7).all()

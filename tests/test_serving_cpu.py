@@ -285,3 +285,9 @@ def test_launcher_declines_host_tensors(lib):
     assert fast.sdpa_kv8(q, *_cache(), _ints(0)[None], _ints(0), None, True, -1.0, False) is None
     assert fast.sdpa_kv8(*[None] * 11) is None
     assert fast.launches() == before
+
+
+def test_attend_groups_and_workspace(lib):
+    assert _attend(lib, Hq=257 * 2) == _native.TA_ERR_INVALID_ARGUMENT
+    assert b"256 query heads" in lib.ta_last_error()
+    assert _attend(lib, Hq=64, T=1 << 19) == _native.TA_ERR_INVALID_ARGUMENT  # 2^24 rows

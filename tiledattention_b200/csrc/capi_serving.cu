@@ -229,7 +229,7 @@ int ta_sdpa_kv8(const void* q, const int64_t* q_strides, void* o, const int64_t*
                 void* workspace, int64_t workspace_bytes, unsigned int* dev_status, void* stream) {
   TaNvtxRange nvtx_range("ta_sdpa_kv8");
   ta_capi_clear_error();
-  if (!q || !o || !q_strides || !o_strides || !lengths || !workspace)
+  if (!q || !o || !q_strides || !o_strides || !lengths)
     return ta_capi_fail(TA_ERR_INVALID_ARGUMENT, "null pointer argument");
   int rc = check_cache(k_pages, v_pages, k_scale, v_scale, num_pages, page, table, table_stride,
                        table_width, B, Hkv, T, D);
@@ -240,6 +240,7 @@ int ta_sdpa_kv8(const void* q, const int64_t* q_strides, void* o, const int64_t*
     return ta_capi_fail(TA_ERR_INVALID_ARGUMENT, "at most 256 query heads per cache head");
   if (static_cast<int64_t>(Hq / Hkv) * T >= (1 << 24))
     return ta_capi_fail(TA_ERR_INVALID_ARGUMENT, "too many query rows per cache head");
+  if (!workspace) return ta_capi_fail(TA_ERR_INVALID_ARGUMENT, "null workspace");
   if (!is_16bit(dtype)) return ta_capi_fail(TA_ERR_UNSUPPORTED_DTYPE, "q: fp16 or bf16");
   if (!(scale > 0.f) || !std::isfinite(scale))
     return ta_capi_fail(TA_ERR_INVALID_ARGUMENT, "scale must be a positive finite number");

@@ -209,7 +209,8 @@ def sdpa_kv_cache(q, cache: KVCache8, page_table, lengths, *, counts=None, causa
     """Attention of new tokens over an 8-bit cache: softmax(scale q K^T + mask) V.
 
     q:          [B, Hq, T, D] CUDA tensor, float16 or bfloat16; Hq a multiple of the cache's
-                heads (query head h reads cache head h // (Hq / Hkv)).
+                heads, at most 256 times them (query head h reads cache head
+                h // (Hq / Hkv)).
     cache:      KVCache8 whose pages hold the tokens, the new ones among them.
     page_table: int32 [B, width], as in kv_cache_append.
     lengths:    int32 [B]: tokens of each sequence in the cache; 0 for an unused row.
