@@ -11,10 +11,16 @@ from tiledattention_b200 import (  # noqa: F401
     DTypeNotSupportedError,
     InvalidShapeError,
     KernelError,
+    KVCache8,
     TiledAttentionError,
     UnsupportedPlatformError,
     __version__,
     check_device_status,
+    kv_cache_alloc,
+    kv_cache_append,
+    rotary,
+    rotary_frequencies,
+    sdpa_kv_cache,
     sdpa_partial,
     sdpa_split_kv,
     sdpa_with_lse,
