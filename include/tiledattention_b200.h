@@ -198,7 +198,8 @@ int ta_sdpa_fwd_split_noalloc(const void* q, const void* k, const void* v, void*
  *                 strides position_strides (0 for a shared row)
  *   inv_freq      device double [rotary_dim / 2], radians per position
  * Bases and strides that are multiples of 16 bytes, with D a multiple of 8 and rotary_dim of
- * 16 (interleaved: 8), take 16-byte accesses; everything else runs element by element.
+ * 16 (interleaved: 8), take 16-byte accesses; half and a quarter of these, 8- and 4-byte ones;
+ * everything else, and head dims beyond 256 accesses, runs element by element.
  */
 int ta_rotary(const void* q, void* q_out, const int64_t* q_strides, const int64_t* q_out_strides,
               int Hq, const void* k, void* k_out, const int64_t* k_strides,

@@ -764,3 +764,34 @@ def test_short_workspaces_are_refused(T):
         assert rc == _native.TA_ERR_INVALID_ARGUMENT, (at, size)
     torch.cuda.synchronize()
     assert (out == 7).all()
+
+
+@pytest.mark.parametrize("B,H,Hk,S,D,R,inter,dtype", [
+    (1, 2, 1, 3, 2304, 2304, True, BF16),    # more slots of 16 bytes than a block has threads
+    (1, 2, 1, 3, 2304, 32, False, FP16),
+    (9, 6, 3, 220, 80, 40, False, BF16),     # halves of 20: 8-byte accesses
+    (2, 3, 2, 33, 84, 84, True, FP16),
+    (2, 3, 2, 33, 70, 36, False, BF16),      # halves of 18: 4-byte accesses
+    (3, 2, 1, 50, 38, 22, True, FP16),
+    (3, 2, 1, 50, 38, 22, False, FP16),      # halves of 11: value by value
+])
+def test_rotary_widths_of_access(B, H, Hk, S, D, R, inter, dtype):
+    test_rotary_matches_64_bits(B, H, Hk, S, D, R, inter, dtype)
+
+
+def test_rotary_alignment_of_views():
+    """Rows at 2, 4 and 8 bytes, of head dims that are whole vectors: the same bits as aligned ones."""
+    import tiledattention_b200 as ta
+
+    freq, mag = ta.rotary_frequencies(64, device=DEV)
+    pos = torch.arange(30, device=DEV)
+    x = _randn(2, 3, 30, 64, seed=4)
+    for inter in (False, True):
+        want = ta.rotary(x, x, pos, freq, magnitude=mag, interleaved=inter)
+        for pad in (1, 2, 4, 6):
+            wide = torch.zeros(2, 3, 30, 64 + 2 * pad, dtype=BF16, device=DEV)
+            view = wide[..., pad:pad + 64]
+            view.copy_(x)
+            for pair in ((view, x), (x, view), (view, view)):
+                got = ta.rotary(*pair, pos, freq, magnitude=mag, interleaved=inter)
+                assert all(torch.equal(a, b) for a, b in zip(got, want))

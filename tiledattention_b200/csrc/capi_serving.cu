@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 
@@ -34,10 +35,17 @@ bool is_16bit(int dtype) { return dtype == TA_DTYPE_F16 || dtype == TA_DTYPE_BF1
 
 bool aligned(const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-// 16-byte rows of 16-bit values: base and outer strides of dims with more than one entry.
+// Bytes, a power of two up to 16, that divide the base and the outer strides (of dims with more than
+// one entry) of 16-bit values.
+int rows_alignment(const void* p, const int64_t* st, int64_t n0, int64_t n1, int64_t n2) {
+  uint64_t bits = reinterpret_cast<uintptr_t>(p) | 16;
+  const int64_t n[3] = {n0, n1, n2};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] != 1) bits |= static_cast<uint64_t>(st[i]) * 2;
+  return static_cast<int>(bits & (~bits + 1));
+}
 bool rows_aligned(const void* p, const int64_t* st, int64_t n0, int64_t n1, int64_t n2) {
-  return aligned(p, 16) && (n0 == 1 || st[0] % 8 == 0) && (n1 == 1 || st[1] % 8 == 0) &&
-         (n2 == 1 || st[2] % 8 == 0);
+  return rows_alignment(p, st, n0, n1, n2) == 16;
 }
 
 int launched(cudaError_t err, const char* what) {
@@ -142,12 +150,13 @@ int ta_rotary(const void* q, void* q_out, const int64_t* q_strides, const int64_
   ta::RotaryParams p{};
   p.t[0] = {q, q_out, q_strides[0], q_strides[1], q_strides[2],
             q_out_strides[0], q_out_strides[1], q_out_strides[2], Hq};
-  bool vector = rows_aligned(q, q_strides, B, Hq, S) && rows_aligned(q_out, q_out_strides, B, Hq, S);
+  int alignment = std::min(rows_alignment(q, q_strides, B, Hq, S),
+                           rows_alignment(q_out, q_out_strides, B, Hq, S));
   if (k) {
     p.t[1] = {k, k_out, k_strides[0], k_strides[1], k_strides[2],
               k_out_strides[0], k_out_strides[1], k_out_strides[2], Hk};
-    vector = vector && rows_aligned(k, k_strides, B, Hk, S) &&
-             rows_aligned(k_out, k_out_strides, B, Hk, S);
+    alignment = std::min({alignment, rows_alignment(k, k_strides, B, Hk, S),
+                          rows_alignment(k_out, k_out_strides, B, Hk, S)});
   }
   p.positions = positions;
   p.pos_sb = position_strides[0];
@@ -162,8 +171,7 @@ int ta_rotary(const void* q, void* q_out, const int64_t* q_strides, const int64_
   p.inverse = inverse != 0;
   p.bf16 = dtype == TA_DTYPE_BF16;
   p.magnitude = magnitude;
-  vector = vector && D % 8 == 0 && rotary_dim % (p.interleaved ? 8 : 16) == 0;
-  return launched(ta::launch_rotary(p, vector, sm_count(), static_cast<cudaStream_t>(stream)),
+  return launched(ta::launch_rotary(p, alignment, sm_count(), static_cast<cudaStream_t>(stream)),
                   "rotary launch failed");
 }
 

@@ -26,6 +26,7 @@ struct RotaryParams {
   float magnitude;
 };
 
-cudaError_t launch_rotary(const RotaryParams& p, bool vector, int sm_count, cudaStream_t stream);
+// alignment: bytes (a power of two up to 16) that divide all bases and outer strides.
+cudaError_t launch_rotary(const RotaryParams& p, int alignment, int sm_count, cudaStream_t stream);
 
 }  // namespace ta
