@@ -10,7 +10,8 @@
 // number, which at position 2^20 leaves an error near 2^-33 turns where a float product would
 // leave 2^-4 radians. The fraction goes to sincospif in float. That costs about 50
 // instructions a pair, so a thread computes its pairs' cos and sin once and applies them to
-// several heads (they depend on the position only).
+// several heads (they depend on the position only). Measured: 8 x 4096 tokens, 32 + 32 heads of 128:
+// 161 us, 6.66 TB/s, a copy's rate; 32 single tokens, 32 + 8 heads: 2.3 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

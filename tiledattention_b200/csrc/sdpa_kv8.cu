@@ -30,9 +30,13 @@
 //
 // What bounds the loop next to HBM is instruction issue (2 conversions for 4 codes, 1 MMA for
 // 256 codes and 8 rows), so everything a step does not need is kept out of it: masks are applied only
-// where a step reaches a row's limit, the scales ride in the multiply-add before exp2, and the
-// reference of a row's weights moves (and is agreed on between lanes) only when a score passes it
-// by 2^15.
+// where a step reaches a row's limit, a page's scales take one multiply-add a score, page ids are fetched
+// for up to 32 steps at once, and the reference of a row's weights moves (and is agreed on between
+// lanes) only when a score passes it by 2^15.
+//
+// Measured: 64 sequences of 16384, 64 heads over 8, head dim 128: 350 us, 6.1 TB/s (copying
+// alone, without any arithmetic: 335). 32 sequences of up to 4096, 32 heads over 8: 33 us,
+// 4.0 TB/s (5 us of it the merge kernel, 5 until the first keys are there). One of 777: 8 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
