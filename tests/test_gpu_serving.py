@@ -795,3 +795,28 @@ def test_rotary_alignment_of_views():
             for pair in ((view, x), (x, view), (view, view)):
                 got = ta.rotary(*pair, pos, freq, magnitude=mag, interleaved=inter)
                 assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("fast", [True, False])
+def test_rotary_gradient_of_one_output(fast, monkeypatch):
+    """Where only one of the outputs is used, the other input's gradient is none or zero, and only
+    one rotation runs backward."""
+    import tiledattention_b200 as ta
+
+    if not fast:
+        monkeypatch.setenv("TILEDATTN_SYNC_MODE", "post")  # the Python path
+    freq, mag = ta.rotary_frequencies(64, device=DEV)
+    pos = torch.arange(9, device=DEV)
+    for used in (0, 1):
+        q, k = (_randn(2, 3, 9, 64, seed=i).requires_grad_() for i in (1, 2))
+        out = ta.rotary(q, k, pos, freq, magnitude=mag)
+        g = _randn(2, 3, 9, 64, seed=5)
+        out[used].backward(g)
+        want = ta.rotary(g, None, pos, freq, magnitude=mag, inverse=True)[0]
+        assert torch.equal((q, k)[used].grad, want)
+        other = (q, k)[1 - used].grad
+        assert other is None or not other.any()
+        # a gradient that is the broadcast of one number
+        q2 = q.detach().requires_grad_()
+        ta.rotary(q2, None, pos, freq)[0].sum().backward()
+        assert torch.equal(q2.grad, ta.rotary(torch.ones_like(q2), None, pos, freq, inverse=True)[0])

@@ -294,6 +294,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
                               {interleaved, magnitude, inverse}, qo, ko),
                 "rotary: ", g_last_error ? g_last_error() : "", " (launch)");
     ctx->save_for_backward({pos, freq});
+    ctx->set_materialize_grads(false);  // of an unused output: undefined, not zeros to be turned
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["magnitude"] = magnitude;
     ctx->saved_data["inverse"] = inverse;

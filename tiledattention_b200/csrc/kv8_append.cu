@@ -109,7 +109,8 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendParams p, int s
     if (start < 0 || count < 0) return;
     count = min(min(count, static_cast<int64_t>(p.T)), capacity - start);
   }
-  const int64_t slot = start / p.page + blockIdx.x % slots;
+  // (page is a power of two: a 64-bit division would cost as much as converting the page)
+  const int64_t slot = (p.starts[b] >> (__ffs(p.page) - 1)) + (blockIdx.x - b * slots);
   const SlotSpan span = slot_span(start, count, slot, p.page);
   if (span.row1 <= span.row0) return;
 

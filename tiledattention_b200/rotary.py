@@ -165,6 +165,7 @@ def _autograd_function():
         @staticmethod
         def forward(ctx, q, k, positions, inv_freq, interleaved, magnitude, inverse):
             ctx.save_for_backward(positions, inv_freq)
+            ctx.set_materialize_grads(False)
             ctx.how = (interleaved, magnitude, inverse)
             out_q, out_k = run_rotary(q, k, positions, inv_freq, interleaved, magnitude, inverse)
             return out_q if k is None else (out_q, out_k)
