@@ -8,7 +8,8 @@
 // share every 128-key tile; rows are (token, head of the group), so all heads of a group share
 // the keys too. Roles:
 //   warps 0-3, 4-7  softmax and epilogue of row tile 0, 1 (thread = row); they also bring the
-//                   rows of q into shared memory as fp16 times a power of two
+//                   rows of q into shared memory as fp16 times a power of two (at head dim 256
+//                   warps 4-7 are converters of V, and warps 8-11 of K)
 //   warps 8-11      converters: codes from the pages straight into registers (up to a tile
 //                   ahead), fp16 (exact) into the 128-byte-swizzled tiles that tcgen05 reads, a
 //                   unit being one tile's K or V
@@ -527,22 +528,25 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         }
       }
     }
-  } else if (warp >= 8) {
+  } else if (warp >= (C::kTiles == 2 ? 8 : 4)) {
     // ------------------------------------------------------------ converters
     regs_dec<kConvertRegs>();
     if (has_run) {
       constexpr int kRowsPerPass = 128 / C::kChunks;  // of 128 threads, 16 codes each
-      // Passes in flight: those of a tile (K and V), at head dim 256 of a unit.
-      constexpr bool kWholeTile = C::kChunks <= 8;
-      constexpr int kHeld = kWholeTile ? 2 * C::kChunks : C::kChunks;
-      const int tid = threadIdx.x - 256;
+      // The passes of a tile are in flight, of K and V, or where the second row tile's warps convert too
+      // of one of them: those warps V, the others K. (Warps 8-11 alone, a unit in flight: 2 x 1024
+      // tokens at the end of 8192, 32 heads over 8, head dim 256: 1102 us, so 921.)
+      constexpr int kKinds = C::kTiles == 2 ? 2 : 1;
+      static_assert(kKinds == 2 || C::kStages == 2, "a stage for K and one for V");
+      const int first_kind = warp < 8 ? 1 : 0;
+      constexpr int kHeld = kKinds * C::kChunks;
       // Lanes: 4 chunks of one 128-byte row of the tile and the next key's, so that 8
       // lanes' 16-byte stores meet 8 different banks.
       const int c = (lane & 3) | (C::kChunks == 4 ? 0 : (lane >> 3 & (C::kChunks / 4 - 1)) << 2);
       const int row_in_warp = C::kChunks == 4 ? lane >> 2
                               : C::kChunks == 8 ? ((lane >> 2) & 1) | (lane >> 4 << 1)
                                                 : (lane >> 2) & 1;
-      const int row0 = (warp - 8) * (kRowsPerPass / 4) + row_in_warp;
+      const int row0 = (warp & 3) * (kRowsPerPass / 4) + row_in_warp;
       const bool real = c * 16 < p.D;
       const uint32_t store = smem_u32(kv_smem) + (c >> 2) * (kTileKeys * 128);  // 64 dims: 128 bytes a key
       // The thread's two 16-byte pieces of a row, swizzled; a pass's rows are 8 k apart or more.
@@ -552,10 +556,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       constexpr int kPlaces = kRowsPerPass >= 16 ? C::kChunks : C::kChunks / 2;
       const uint32_t places = smem_u32(place) + (kRowsPerPass > 16 ? row0 >> 4 : 0) * 8;
       const int in_block = row0 & 15;
-      const uint8_t* const mine[2] = {p.pages[0] + in_block * p.D + c * 16,
+      const uint8_t* const mine[2] = {p.pages[first_kind] + in_block * p.D + c * 16,
                                       p.pages[1] + in_block * p.D + c * 16};
       bool ok = true;
-      int st = 0, phase = 0;  // of the next unit
+      int st = first_kind, phase = 0;  // of the next unit
 
       int64_t at[kPlaces];  // of the tile whose codes are loaded next
       auto read_places = [&](int slot) {
@@ -565,13 +569,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
                        : "=l"(at[i])
                        : "r"(places + (slot * kGroups + i * (kRowsPerPass > 16 ? kRowsPerPass / 16 : 1)) * 8));
       };
-      // Codes of pass i of a unit (kind 0 K, 1 V) of that tile. Rows without a key read as zeros.
-      auto fetch = [&](int i, int kind) {
+      // Codes of pass i of the u-th unit here of that tile. Rows without a key read as zeros.
+      auto fetch = [&](int i, int u) {
         const int64_t where = at[kRowsPerPass >= 16 ? i : i / 2];
         const int row = in_block + (kRowsPerPass < 16 ? (i & 1) * kRowsPerPass : 0);
         uint4 v = make_uint4(0, 0, 0, 0);
         if (real && row < static_cast<int>(where & 31))
-          v = __ldg(reinterpret_cast<const uint4*>(mine[kind] + (where >> 5) + (row - in_block) * p.D));
+          v = __ldg(reinterpret_cast<const uint4*>(mine[u] + (where >> 5) + (row - in_block) * p.D));
         return v;
       };
       auto wait_meta = [&](int n) {
@@ -595,17 +599,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         ok = wait_meta(tile_no);  // the next tile's pages
         if (!ok) break;
         now = bars->tiles[tile_no % kMeta];
-        if (kWholeTile) read_places(tile_no % kMeta);
+        read_places(tile_no % kMeta);
 #pragma unroll
-        for (int kind = 0; kind < 2; ++kind) {
-          if (!kWholeTile && kind == 1) read_places(tile_no % kMeta);
+        for (int u = 0; u < kKinds; ++u) {
+          const int kind = kKinds == 2 ? u : first_kind;  // 0 K, 1 V
           ok = ok && mbar_wait_bounded(&bars->kv_empty[st], phase ^ 1, abort_flag, kTimeoutNs);
           if (!ok) break;
           const uint32_t dst = store + st * C::kTileBytes;
           uint32_t nans = 0;
 #pragma unroll
           for (int i = 0; i < C::kChunks; ++i) {
-            const uint4 v = held[kWholeTile ? kind * C::kChunks + i : i];
+            const uint4 v = held[u * C::kChunks + i];
             if (kind == 1) nans |= nan_bits(v.x) | nan_bits(v.y) | nan_bits(v.z) | nan_bits(v.w);
             uint32_t f[8];
             codes_to_f16(v.x, f[0], f[1]);
@@ -630,18 +634,19 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           }
           fence_proxy_async_shared();
           mbar_arrive(&bars->kv_full[st]);
-          // The registers' next loads: the next tile's, or at head dim 256 the next unit's. All in one
-          // burst: a load issued between the uses of others makes those uses wait for it too.
+          // The registers' next loads, the next tile's. All in one burst: a load issued between the uses
+          // of others makes those uses wait for it too.
 #pragma unroll
-          for (int i = 0; i < C::kChunks; ++i)
-            held[kWholeTile ? kind * C::kChunks + i : i] = fetch(i, kWholeTile ? kind : kind ^ 1);
-          if (++st == C::kStages) {
+          for (int i = 0; i < C::kChunks; ++i) held[u * C::kChunks + i] = fetch(i, u);
+          if (kKinds == 1) {
+            phase ^= 1;
+          } else if (++st == C::kStages) {
             st = 0;
             phase ^= 1;
           }
         }
       }
-      if (!ok && tid == 0 && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_LOAD, abort_flag);
+      if (!ok && threadIdx.x % 128 == 0 && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_LOAD, abort_flag);
     }
   } else {
     regs_inc<kSoftmaxRegs>();
