@@ -327,6 +327,9 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
   }
 };
 
+// A tensor that carries a forward-mode tangent: the Python path turns that too.
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+
 PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 7) Py_RETURN_NONE;
   const at::Tensor* q = tensor_arg(args[0]);
@@ -339,6 +342,7 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const RotaryHow how{args[4] == Py_True, PyFloat_AS_DOUBLE(args[5]), args[6] == Py_True};
   at::Tensor qo, ko;
   try {
+    if (has_tangent(*q) || (k && has_tangent(*k))) Py_RETURN_NONE;
     if (at::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad()))) {
       auto out = RotaryFunction::apply(*q, k ? std::optional<at::Tensor>(*k) : std::nullopt, *pos, *freq, how.interleaved,
                                        how.magnitude, how.inverse);

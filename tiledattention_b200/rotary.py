@@ -190,6 +190,23 @@ def _autograd_function():
     return Rotary
 
 
+def _forward_mode(torch_mod, q, k, positions, inv_freq, **how):
+    """(q, k) turned with their tangents, which a linear map takes to the tangents' own rotation;
+    None where neither carries one."""
+    fwad = torch_mod.autograd.forward_ad
+    if not torch_mod._C._is_fwd_grad_enabled():
+        return None
+    (q, dq), (k, dk) = (fwad.unpack_dual(t) if t is not None else (None, None) for t in (q, k))
+    if dq is None and dk is None:
+        return None
+    q, k = rotary(q, k, positions, inv_freq, **how)
+    if dq is not None:
+        dq, dk = rotary(dq, dk, positions, inv_freq, **how)
+    else:
+        dk = rotary(dk, None, positions, inv_freq, **how)[0]
+    return tuple(t if d is None else fwad.make_dual(t, d) for t, d in ((q, dq), (k, dk)))
+
+
 def rotary(q, k, positions, inv_freq, *, interleaved: bool = False, magnitude: float = 1.0,
            inverse: bool = False):
     """Rotary positions: (q, k) with every pair of dims turned by position * inv_freq.
@@ -204,7 +221,8 @@ def rotary(q, k, positions, inv_freq, *, interleaved: bool = False, magnitude: f
     inverse:     turn the other way (what the gradient does).
 
     Returns new contiguous tensors, computed asynchronously on the current torch stream;
-    differentiable in q and k.
+    differentiable in q and k, in reverse mode (twice too) and in forward mode. positions and
+    inv_freq are constants to it.
     """
     out = _fast_launch(q, k, positions, inv_freq, interleaved, magnitude, inverse)
     if out is not None:
@@ -218,6 +236,11 @@ def rotary(q, k, positions, inv_freq, *, interleaved: bool = False, magnitude: f
     torch_mod = _runtime.get_torch_module()
     _check(torch_mod, q, k, positions, inv_freq)
     magnitude = float(magnitude)
+    if torch_mod.autograd.forward_ad._current_level >= 0:
+        out = _forward_mode(torch_mod, q, k, positions, inv_freq, interleaved=interleaved,
+                            magnitude=magnitude, inverse=inverse)
+        if out is not None:
+            return out
     if torch_mod.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         out = _autograd_function().apply(q, k, positions, inv_freq, interleaved, magnitude, inverse)
         return (out, None) if k is None else out
