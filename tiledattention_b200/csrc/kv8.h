@@ -91,7 +91,7 @@ struct AttendParams {
   unsigned int* status;
   float* part_o;                  // partial outputs, maxima and sums (see sdpa_kv8.cu)
   float* part_ml;
-  int2* spans;                    // first and last run of a block of rows (see sdpa_kv8.cu)
+  int2* spans;                    // first and last run of a block of rows; (1, 0): none has keys of it
   Cut* cuts;
   int B, Hq, Hkv, T, D, page, page_shift, width, num_pages, bf16, causal;
   int group;                      // Hq / Hkv, at most kMaxGroup

@@ -209,7 +209,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
   const Scan sc = scan_items<kWarps>(p.B, s_scan, [&](int b) {
     const SeqExtent e = extent_of(p, b);
     report_extent(p, e);
-    return static_cast<int64_t>(units_of(tiles_of(e, C::kTile))) * hrs;
+    const int tiles = tiles_of(e, C::kTile);
+    if (tiles == 0 && b % gridDim.x == blockIdx.x)  // no run comes by: the merge kernel writes the rows
+      for (int i = 0; i < hrs; ++i) p.spans[static_cast<int64_t>(b) * hrs + i] = make_int2(1, 0);
+    return static_cast<int64_t>(units_of(tiles)) * hrs;
   });
   const int64_t total = sc.total;
   const int64_t parts = min(static_cast<int64_t>(gridDim.x), total);
@@ -769,7 +772,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
 }
 
 // Merges the partial results of (sequence, head)s that several runs share, and writes the rows
-// of sequences without keys. One block: kWarps rows, a warp each, or with `spread` one row
+// of sequences without keys: both by the attend kernel's records, and nothing of it is read before
+// that kernel has ended (lengths read earlier, while it runs, would save 0.4 us of 32). One block: kWarps rows, a warp each, or with `spread` one row
 // whose runs the warps divide (few rows, many runs).
 template <int NJ, int NT>
 __global__ void __launch_bounds__(kThreads) merge_kernel(const AttendParams p, int parts, int spread) {
@@ -786,21 +790,20 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const AttendParams p, i
   const int b = bh / p.Hkv, h = bh - b * p.Hkv;
   const int row = spread ? rg : rg * kWarps + warp;
   const int rb = row / C::kRows, r = row - rb * C::kRows;
-  const int tiles = tiles_of(extent_of(p, b), C::kTile);
   wait_for_stream();
   int i0 = 0, i1 = 0;
   if (row < rows) {
-    const int2 span = p.spans[static_cast<int64_t>(bh) * p.row_blocks + rb];  // unset without tiles
-    i0 = max(span.x, 0);  // in range even if the lengths changed after the runs were cut
+    const int2 span = p.spans[static_cast<int64_t>(bh) * p.row_blocks + rb];
+    i0 = max(span.x, 0);
     i1 = min(span.y, parts - 1);
   }
-  const bool mine = row < rows && !(tiles > 0 && i0 == i1);  // else that run wrote the row
+  const bool mine = i0 != i1;  // else one run wrote the row; i0 > i1: no run has a key of it
   if (spread && !mine) return;  // one row a block: all its threads alike
   float m = -INFINITY, l = 0.f;
   float4 a[kVec];
 #pragma unroll
   for (int v = 0; v < kVec; ++v) a[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (mine && tiles > 0) {
+  if (i0 < i1) {
     const int step = spread ? kWarps : 1;
     constexpr int kAtOnce = 4;  // parts whose loads are in flight together
     for (int i = i0 + (spread ? warp : 0); i <= i1; i += kAtOnce * step) {
