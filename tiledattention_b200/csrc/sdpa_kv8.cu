@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
 #pragma unroll
           for (int i = 0; i < kBlocks; ++i) m = fmaxf(m, fmaxf(s[i][nt][r], s[i][nt][2 + r]));
           cand[nt][r] = m;
-          grow |= m > ref[nt][r] + kGrowth;
+          grow |= m - ref[nt][r] > kGrowth;  // not m > ref + kGrowth, a sum that rounds up from 2^24 on
         }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
             a[r] = 1.f;
-            if (m > ref[nt][r] + kGrowth) {
+            if (m - ref[nt][r] > kGrowth) {
               const float to = m - kBelow;
               a[r] = ex2_approx(ref[nt][r] - to);  // 0 from -inf
               ref[nt][r] = to;
