@@ -37,6 +37,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
 #include <utility>
 
 #include "kv8_device.cuh"
@@ -57,6 +58,11 @@ static_assert(128 * (2 * kSoftmaxRegs + kConvertRegs + kSideRegs) == kThreads * 
               "register split must match the launch allocation");
 constexpr uint32_t kTmemCols = 512;
 constexpr float kBelow = 7.f, kGrowth = 15.f;  // see sdpa_kv8.cu
+// t - ref comes out of one multiply-add on the score and so is more exact than ref, which is a rounded t
+// less 7: a weight may pass 2^15 by 2^(3 * 2^-24 |ref|), which from |ref| = 2^22 on may pass fp16's 65504.
+// A block with a reference beyond kFar goes on in a second form of the loop that rounds t first, as the
+// kernel for few rows does. (A branch in the one loop: 2 x 1024 tokens at the end of 8192 374-416 us for 324.)
+constexpr float kFar = 1048576.f;
 constexpr uint64_t kTimeoutNs = 1000000000ull;  // 1 s per wait
 constexpr int kMeta = 8;                       // tiles whose places, pages and scales are kept
 constexpr int kGroups = kTileKeys / 16;        // blocks of 16 keys: one page each
@@ -196,6 +202,8 @@ template <int D>
 __device__ __forceinline__ bool has_two(const AttendParams& p, int rb) {
   return Cfg<D>::kTiles == 2 && p.group * p.T - rb * Cfg<D>::kRows > kTileRows;
 }
+
+__device__ __forceinline__ bool is_far(float ref) { return fabsf(ref) > kFar && ref != -INFINITY; }
 
 __device__ __forceinline__ void report(const AttendParams& p, uint32_t code, volatile int* abort_flag) {
   *abort_flag = 1;
@@ -737,103 +745,121 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         }
 
         float ref = -INFINITY, l_run = 0.f;
-        for (int j2 = 0; j2 < 2 * s.n; ++j2, ++seen) {
-          const int half = j2 & 1;
-          const int slot = tile_no % kMeta;
-          if (half == 0)
-            ok = mbar_wait_bounded(&bars->meta_full[slot], (tile_no / kMeta) & 1, abort_flag, kTimeoutNs);
-          ok = ok && mbar_wait_bounded(&bars->s_full[t][half], (seen >> 1) & 1, abort_flag, kTimeoutNs);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          uint32_t x[64];
-          tmem_ld64(t_s + half * kHalfKeys, *reinterpret_cast<uint32_t(*)[32]>(x),
-                    *reinterpret_cast<uint32_t(*)[32]>(x + 32));
-          tmem_wait_ld();
-          const int key0 = (s.t0 + (j2 >> 1)) * kTileKeys + half * kHalfKeys;
-          if (key0 + kHalfKeys > safe) {
-            const int visible = lim - key0;
+        // The block's halves from j2 on; the first that was not finished.
+        auto halves = [&](auto far_rows, int j2) {
+          constexpr bool kFarRows = decltype(far_rows)::value;
+          for (; j2 < 2 * s.n; ++j2, ++seen) {
+            const int half = j2 & 1;
+            const int slot = tile_no % kMeta;
+            if (half == 0)
+              ok = mbar_wait_bounded(&bars->meta_full[slot], (tile_no / kMeta) & 1, abort_flag, kTimeoutNs);
+            ok = ok && mbar_wait_bounded(&bars->s_full[t][half], (seen >> 1) & 1, abort_flag, kTimeoutNs);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return j2;
+            tc_fence_after();
+            uint32_t x[64];
+            tmem_ld64(t_s + half * kHalfKeys, *reinterpret_cast<uint32_t(*)[32]>(x),
+                      *reinterpret_cast<uint32_t(*)[32]>(x + 32));
+            tmem_wait_ld();
+            const int key0 = (s.t0 + (j2 >> 1)) * kTileKeys + half * kHalfKeys;
+            if (key0 + kHalfKeys > safe) {
+              const int visible = lim - key0;
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (i >= visible) x[i] = 0xff800000u;
-          }
-          const Meta* m = meta + slot * kGroups + half * (kGroups / 2);
-          // t = score * c + e, c held above zero so that a masked score stays -inf
-          float cand = -INFINITY;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            float a = fmaxf(__uint_as_float(x[16 * g]), __uint_as_float(x[16 * g + 1]));
-            float b = fmaxf(__uint_as_float(x[16 * g + 2]), __uint_as_float(x[16 * g + 3]));
-#pragma unroll
-            for (int i = 4; i < 16; i += 4) {
-              a = fmax3(a, __uint_as_float(x[16 * g + i]), __uint_as_float(x[16 * g + i + 1]));
-              b = fmax3(b, __uint_as_float(x[16 * g + i + 2]), __uint_as_float(x[16 * g + i + 3]));
+              for (int i = 0; i < 64; ++i)
+                if (i >= visible) x[i] = 0xff800000u;
             }
-            cand = fmaxf(cand, fmaf(fmaxf(a, b), fmaxf(mul * m[g].ks, 1e-37f), m[g].e));
-          }
-          const bool grow = cand > ref + kGrowth;
-          if (__any_sync(0xffffffffu, grow)) {
-            float alpha = 1.f;
-            if (grow) {
-              alpha = ex2_approx(ref - (cand - kBelow));  // 0 from -inf
-              ref = cand - kBelow;
-              l_run *= alpha;
+            const Meta* m = meta + slot * kGroups + half * (kGroups / 2);
+            // t = score * c + e, c held above zero so that a masked score stays -inf
+            float cand = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              float a = fmaxf(__uint_as_float(x[16 * g]), __uint_as_float(x[16 * g + 1]));
+              float b = fmaxf(__uint_as_float(x[16 * g + 2]), __uint_as_float(x[16 * g + 3]));
+#pragma unroll
+              for (int i = 4; i < 16; i += 4) {
+                a = fmax3(a, __uint_as_float(x[16 * g + i]), __uint_as_float(x[16 * g + i + 1]));
+                b = fmax3(b, __uint_as_float(x[16 * g + i + 2]), __uint_as_float(x[16 * g + i + 3]));
+              }
+              cand = fmaxf(cand, fmaf(fmaxf(a, b), fmaxf(mul * m[g].ks, 1e-37f), m[g].e));
             }
-            if (j2 > 0) {
-              // The product of the half before may still be adding to the output. Behind it come the
-              // scores of the half after this one, or in the last tile its own signal.
-              ok = j2 + 1 < 2 * s.n
-                       ? mbar_wait_bounded(&bars->s_full[t][half ^ 1], ((seen + 1) >> 1) & 1, abort_flag, kTimeoutNs)
-                       : mbar_wait_bounded(&bars->o_final[t][0], segs & 1, abort_flag, kTimeoutNs);
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-              tc_fence_after();
-              const uint64_t alpha2 = f2_pack(alpha, alpha);
+            const bool grow = cand - ref > kGrowth;  // not cand > ref + kGrowth, a sum that may round up
+            if (__any_sync(0xffffffffu, grow)) {
+              float alpha = 1.f;
+              if (grow) {
+                alpha = ex2_approx(ref - (cand - kBelow));  // 0 from -inf
+                ref = cand - kBelow;
+                l_run *= alpha;
+              }
+              if (j2 > 0) {
+                // The product of the half before may still be adding to the output. Behind it come the
+                // scores of the half after this one, or in the last tile its own signal.
+                ok = j2 + 1 < 2 * s.n
+                         ? mbar_wait_bounded(&bars->s_full[t][half ^ 1], ((seen + 1) >> 1) & 1, abort_flag, kTimeoutNs)
+                         : mbar_wait_bounded(&bars->o_final[t][0], segs & 1, abort_flag, kTimeoutNs);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return j2;
+                tc_fence_after();
+                const uint64_t alpha2 = f2_pack(alpha, alpha);
 #pragma unroll 1
-              for (int cc = 0; cc < D / 32; ++cc) {
-                uint32_t o[32];
-                tmem_ld32(t_o + cc * 32, o);
-                tmem_wait_ld();
+                for (int cc = 0; cc < D / 32; ++cc) {
+                  uint32_t o[32];
+                  tmem_ld32(t_o + cc * 32, o);
+                  tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                  float a0, a1;
-                  f2_unpack(f2_mul(f2_pack(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), alpha2),
-                            a0, a1);
-                  o[i] = __float_as_uint(a0);
-                  o[i + 1] = __float_as_uint(a1);
+                  for (int i = 0; i < 32; i += 2) {
+                    float a0, a1;
+                    f2_unpack(f2_mul(f2_pack(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), alpha2),
+                              a0, a1);
+                    o[i] = __float_as_uint(a0);
+                    o[i + 1] = __float_as_uint(a1);
+                  }
+                  tmem_st32(t_o + cc * 32, o);
                 }
-                tmem_st32(t_o + cc * 32, o);
+              }
+              if (!kFarRows && __any_sync(0xffffffffu, is_far(ref))) return j2;  // this half in the other form
+            }
+            if (kFarRows && is_far(ref)) {  // t - ref in the scores' place, as what gives it without ref
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const float cs = fmaxf(mul * m[g].ks, 1e-37f), inv = 1.f / cs;
+                const float e = m[g].e, finite_e = fmaxf(e, -1e3f);
+#pragma unroll
+                for (int i = 16 * g; i < 16 * g + 16; ++i)
+                  x[i] = __float_as_uint((fmaf(__uint_as_float(x[i]), cs, e) - ref - finite_e) * inv);
               }
             }
-          }
-          // The weights (16-bit, two a column) go over the first 32 of the half's columns.
-          const float r = ref == -INFINITY ? 0.f : ref;
-          uint32_t pk[32];
+            // The weights (16-bit, two a column) go over the first 32 of the half's columns.
+            const float r = ref == -INFINITY || (kFarRows && is_far(ref)) ? 0.f : ref;
+            uint32_t pk[32];
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float cs = fmaxf(mul * m[g].ks, 1e-37f), sh = m[g].e - r;
-            const uint64_t c2 = f2_pack(cs, cs), s2 = f2_pack(sh, sh);
-            uint64_t sum = f2_pack(0.f, 0.f);
+            for (int g = 0; g < 4; ++g) {
+              const float cs = fmaxf(mul * m[g].ks, 1e-37f), sh = m[g].e - r;
+              const uint64_t c2 = f2_pack(cs, cs), s2 = f2_pack(sh, sh);
+              uint64_t sum = f2_pack(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float a0, a1;
-              f2_unpack(f2_fma(f2_pack(__uint_as_float(x[16 * g + 2 * i]),
-                                       __uint_as_float(x[16 * g + 2 * i + 1])), c2, s2), a0, a1);
-              a0 = ex2_approx(a0);
-              a1 = ex2_approx(a1);
-              pk[g * 8 + i] = pack_f16(a0, a1);
-              sum = f2_add(sum, f2_pack(a0, a1));
+              for (int i = 0; i < 8; ++i) {
+                float a0, a1;
+                f2_unpack(f2_fma(f2_pack(__uint_as_float(x[16 * g + 2 * i]),
+                                         __uint_as_float(x[16 * g + 2 * i + 1])), c2, s2), a0, a1);
+                a0 = ex2_approx(a0);
+                a1 = ex2_approx(a1);
+                pk[g * 8 + i] = pack_f16(a0, a1);
+                sum = f2_add(sum, f2_pack(a0, a1));
+              }
+              float s0, s1;
+              f2_unpack(sum, s0, s1);
+              l_run = fmaf(s0 + s1, m[g].back, l_run);
             }
-            float s0, s1;
-            f2_unpack(sum, s0, s1);
-            l_run = fmaf(s0 + s1, m[g].back, l_run);
+            tmem_st32(t_s + half * kHalfKeys, pk);
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&bars->p_full[t][half]);
+            tile_no += half;
           }
-          tmem_st32(t_s + half * kHalfKeys, pk);
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(&bars->p_full[t][half]);
-          tile_no += half;
-        }
+          return j2;
+        };
+        const int far_from = halves(std::false_type(), 0);
+        if (ok && far_from < 2 * s.n) halves(std::true_type(), far_from);
         if (ok) {  // the last tile's products
           ok = mbar_wait_bounded(&bars->o_final[t][0], segs & 1, abort_flag, kTimeoutNs) &&
                mbar_wait_bounded(&bars->o_final[t][1], segs & 1, abort_flag, kTimeoutNs);
