@@ -212,7 +212,8 @@ int ta_rotary(const void* q, void* q_out, const int64_t* q_strides, const int64_
  * The paged 8-bit key/value cache (no reference counterpart): k_pages and v_pages are device
  * e4m3 codes [num_pages, Hkv, page, D], contiguous and 16-byte aligned, with page 16, 32, 64
  * or 128 and D a multiple of 16 up to 256; k_scale and v_scale are device float32
- * [num_pages, Hkv], powers of two 2^e, -50 <= e <= 50: a value is code * scale. Token i of
+ * [num_pages, Hkv], zero or from 2^-50 to 2^50: a value is code * scale. What ta_kv8_append writes has
+ * scales 2^e; a page filled elsewhere may have any other. Token i of
  * sequence b is row i % page of page table[b * table_stride + i / page] (device int32, width
  * table_width). Page ids outside [0, num_pages) set TA_DEVSTAT_BAD_PAGE and are neither written
  * nor attended to; starts, counts and lengths outside their range set TA_DEVSTAT_BAD_LENGTH and

@@ -2,9 +2,10 @@
 // (sdpa_kv8*.cu) share. Host-callable parts are checked on the CPU (tests/native/kv8_check.cu).
 //
 // Pages [P, Hkv, page, D] of e4m3, D a multiple of 16 up to 256, page 16, 32, 64 or 128; one
-// float32 scale 2^e, e in [kScaleExpMin, kScaleExpMax], for each (page, head). Powers of two
-// cost an e4m3 value nothing (its own exponent does the rest) and make every product with a
-// scale exact. The range of e keeps 2^(difference of two exponents) inside float32.
+// float32 scale for each (page, head). What is written here has scales 2^e, e in [kScaleExpMin,
+// kScaleExpMax]: powers of two cost an e4m3 value nothing (its own exponent does the rest) and make
+// every product with a scale exact. Caches made elsewhere may have any scale of that range. The range
+// keeps 2^(difference of two exponents) inside float32.
 #pragma once
 
 #include <cuda.h>
@@ -26,10 +27,16 @@ __host__ __device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
   return need < kScaleExpMin ? kScaleExpMin : (need > kScaleExpMax ? kScaleExpMax : need);
 }
 
-// Exponent of a stored scale (a power of two), held in range whatever the bits are.
+// Exponent of a stored scale, held in range whatever the bits are.
 __host__ __device__ __forceinline__ int stored_exponent(uint32_t scale_bits) {
   const int e = static_cast<int>((scale_bits >> 23) & 0xffu) - 127;
   return e < kScaleExpMin ? kScaleExpMin : (e > kScaleExpMax ? kScaleExpMax : e);
+}
+
+// A stored scale's bits with its exponent held in range and no sign: itself for every scale from
+// 2^kScaleExpMin up to below 2^(kScaleExpMax + 1).
+__host__ __device__ __forceinline__ uint32_t held_scale(uint32_t scale_bits) {
+  return static_cast<uint32_t>(stored_exponent(scale_bits) + 127) << 23 | (scale_bits & 0x7fffffu);
 }
 
 // A page id from the table, or -1 where the slot or the id is outside its range.

@@ -4,7 +4,8 @@
 // largest finite magnitude of the page's new tokens gives the least power of two s with
 // amax <= 448 s; a page that already holds tokens keeps max(its s, the needed one), and where
 // that grows its old codes are rounded again (exact outside e4m3's subnormals). Codes are
-// x / s rounded to nearest even; what is beyond +-448 s saturates, NaN stays NaN.
+// x / s rounded to nearest even; what is beyond +-448 s saturates, NaN stays NaN. A page filled
+// elsewhere may have an s between powers of two: codes then are x (1 / s) with 1 / s in float32.
 //
 // HBM-bound: 2 bytes read and 1 written a value. One block per (page, head, K or V): the page's
 // tokens are loaded once into registers (kHeld 16-byte vectors a thread: 64 x 128 values fit
@@ -56,7 +57,7 @@ __device__ __forceinline__ uint32_t f32_bits(uint32_t h) {
   return __float_as_uint(f);
 }
 
-// Two values of a packed word, times `mul` (a power of two), as two e4m3 codes.
+// Two values of a packed word, times `mul`, as two e4m3 codes.
 template <bool BF16>
 __device__ __forceinline__ uint32_t codes2(uint32_t w, float mul) {
   float lo, hi;
@@ -78,7 +79,7 @@ __device__ __forceinline__ uint2 codes8(const uint4& v, float mul) {
                     codes2<BF16>(v.z, mul) | (codes2<BF16>(v.w, mul) << 16));
 }
 
-// Four e4m3 codes times mul (a power of two <= 1), rounded again.
+// Four e4m3 codes times mul (<= 1), rounded again.
 __device__ __forceinline__ uint32_t recode4(uint32_t w, float mul) {
   uint32_t out = 0;
 #pragma unroll
@@ -90,8 +91,9 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float mul) {
   return out;
 }
 
-__device__ __forceinline__ float pow2f(int e) {
-  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+// Reciprocal of the power of two below a positive float32, from its bits.
+__device__ __forceinline__ float pow2_reciprocal(uint32_t bits) {
+  return __uint_as_float(0x7f000000u - (bits & 0x7f800000u));
 }
 
 template <bool BF16>
@@ -142,7 +144,7 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendParams p, int s
   uint8_t* out = p.pages[kind] +
                  ((static_cast<int64_t>(page) * p.Hkv + h) * p.page) * static_cast<int64_t>(p.D);
   float* scale = p.scale[kind] + static_cast<int64_t>(page) * p.Hkv + h;
-  const int before = span.row0 > 0 ? stored_exponent(__float_as_uint(*scale)) : kScaleExpMin;
+  const uint32_t before = span.row0 > 0 ? held_scale(__float_as_uint(*scale)) : 0u;
 #pragma unroll
   for (int k = 0; k < kHeld; ++k) m = max_magnitude(held[k], m);
   for (int i = threadIdx.x + kHeld * 128; i < n; i += 128) m = max_magnitude(load(i), m);
@@ -163,10 +165,10 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendParams p, int s
     m = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
   }
 
-  int e = scale_exponent(f32_bits<BF16>(m));
+  uint32_t s = static_cast<uint32_t>(scale_exponent(f32_bits<BF16>(m)) + 127) << 23;  // float32 bits, which order as values
   if (span.row0 > 0) {  // every thread has the old scale: a barrier lies between
-    if (e > before) {
-      const float mul = pow2f(before - e);
+    if (s > before) {
+      const float mul = __uint_as_float(before) * pow2_reciprocal(s);
       uint4* old = reinterpret_cast<uint4*>(out);
       for (int i = threadIdx.x; i < span.row0 * p.D / 16; i += 128) {
         uint4 w = old[i];
@@ -177,11 +179,12 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendParams p, int s
         old[i] = w;
       }
     } else {
-      e = before;
+      s = before;
     }
   }
-  if (threadIdx.x == 0) *scale = pow2f(e);
-  const float mul = pow2f(-e);
+  if (threadIdx.x == 0) *scale = __uint_as_float(s);
+  float mul = pow2_reciprocal(s);
+  if (s & 0x7fffffu) mul = __fdividef(1.f, __uint_as_float(s));
   uint2* dst = reinterpret_cast<uint2*>(out + span.row0 * p.D);  // rows are contiguous
 #pragma unroll
   for (int k = 0; k < kHeld; ++k) {

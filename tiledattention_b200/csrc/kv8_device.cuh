@@ -34,6 +34,22 @@ __device__ __forceinline__ float pow2f(int e) {
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
+// log2 and reciprocal of a value scale as it is stored, its exponent held in range: exact for powers
+// of two, which is what this library writes.
+struct ValueScale {
+  float e, back;
+};
+__device__ __forceinline__ ValueScale value_scale(uint32_t scale_bits) {
+  const int e = stored_exponent(scale_bits);
+  ValueScale r{static_cast<float>(e), pow2f(-e)};
+  if (scale_bits & 0x7fffffu) {
+    const float m = __uint_as_float(0x3f800000u | (scale_bits & 0x7fffffu));
+    r.e += __log2f(m);
+    r.back = __fdividef(r.back, m);
+  }
+  return r;
+}
+
 // Natural-log log-sum-exp of a row from its maximum (log2) and sum; -inf without a key.
 __device__ __forceinline__ float lse_of(float m, float l) {
   return l == 0.f ? -INFINITY : (fmaxf(m, -3.4e38f) + log2f(l)) * 0.69314718055994531f;

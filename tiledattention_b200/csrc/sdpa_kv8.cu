@@ -1,6 +1,6 @@
 // Attention of few query rows over the paged 8-bit cache (decoding, checking drafted tokens).
 //
-//   s_j = scale * (q . k_j) * 2^ek_j          k_j, v_j e4m3 codes, ek_j, ev_j the exponents of
+//   s_j = scale * (q . k_j) * 2^ek_j          k_j, v_j e4m3 codes, ek_j, ev_j the log2 of
 //   o   = sum_j 2^(t_j - m) v_j / sum_j 2^(t_j - m - ev_j)    their pages' scales,
 //   t_j = log2(e) s_j + ev_j                  m a running maximum of t
 //
@@ -514,9 +514,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
       for (int i = 0; i < kBlocks; ++i) {
         const uint32_t at = scales + ((step & 3) * 2 * kBlocks + i) * 4;
         const float ks = lds32(at);
-        const int ev = stored_exponent(__float_as_uint(lds32(at + kBlocks * 4)));
-        const float e = static_cast<float>(ev);
-        back[i] = pow2f(-ev);
+        const ValueScale vs = value_scale(__float_as_uint(lds32(at + kBlocks * 4)));
+        const float e = vs.e;
+        back[i] = vs.back;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float2 f = factors(nt);

@@ -85,7 +85,7 @@ struct Cfg {
 
 struct Meta {   // of 16 keys: their scales in softmax's terms
   float ks;     // scale of K
-  float e;      // exponent of V's scale; -inf where there is no key: such keys have no weight
+  float e;      // log2 of V's scale; -inf where there is no key: such keys have no weight
   float back;   // 2^-e
   int unused;
 };
@@ -492,8 +492,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           Meta m{1.f, -INFINITY, 0.f, 0};
           int64_t at = 0;
           if (a0.id >= 0) {
-            const int ev = stored_exponent(__float_as_uint(vs));
-            m = Meta{ks, static_cast<float>(ev), pow2f(-ev), 0};
+            const ValueScale v = value_scale(__float_as_uint(vs));
+            m = Meta{ks, v.e, v.back, 0};
             const int key = a0.tile.key0 + lane * 16;
             const int64_t row = (static_cast<int64_t>(a0.id) * p.Hkv + a0.h) * p.page + (key & (p.page - 1));
             at = row * p.D * 32 + min(16, a0.tile.length - key);

@@ -1,8 +1,8 @@
 """The paged 8-bit key/value cache and attention over it: what takes sdpa's place once a
 decoder generates tokens.
 
-A cache holds e4m3 codes in pages [P, Hkv, page, D] with one float32 power-of-two scale for
-each (page, head); a page table [B, width] says which page holds which tokens of a sequence.
+A cache holds e4m3 codes in pages [P, Hkv, page, D] with one float32 scale (a power of two where
+it is written here) for each (page, head); a page table [B, width] says which page holds which tokens of a sequence.
 kv_cache_append() writes new tokens (csrc/kv8_append.cu), sdpa_kv_cache() attends to the cached
 ones (csrc/sdpa_kv8.cu). The reference has no cache; argument checks, errors and launches
 follow sdpa's.
@@ -35,8 +35,9 @@ class KVCache8(NamedTuple):
     """Storage of an 8-bit cache (one layer's): torch tensors that the caller owns.
 
     k, v:             float8_e4m3fn [P, Hkv, page, D], contiguous.
-    k_scale, v_scale: float32 [P, Hkv], contiguous, powers of two from 2^-50 to 2^50; the values
-                      of a page are its codes times its scale.
+    k_scale, v_scale: float32 [P, Hkv], contiguous, zero or from 2^-50 to 2^50; the values of a
+                      page are its codes times its scale. kv_cache_append writes powers of two,
+                      pages filled elsewhere may have others.
     """
 
     k: Any
