@@ -119,6 +119,13 @@ def _rows(t):
         memory_format=_runtime.get_torch_module().contiguous_format)
 
 
+def _table_rows(t):
+    """The table itself where its rows are runs of ints side by side or apart, else a copy (of a
+    row expanded over the batch, too)."""
+    apart = t.shape[0] == 1 or t.stride(0) >= t.shape[1]
+    return t if t.stride(1) == 1 and apart else t.contiguous()
+
+
 def _device_of(torch_mod, t):
     same = t.device.index == torch_mod.cuda.current_device()
     return _NULL_CTX if same else torch_mod.cuda.device(t.device)
@@ -184,7 +191,7 @@ def run_kv_cache_append(k, v, cache, page_table, starts, counts):
     if k.numel() == 0:
         return
     k, v = _rows(k.detach()), _rows(v.detach())
-    page_table = page_table if page_table.stride(1) == 1 else page_table.contiguous()
+    page_table = _table_rows(page_table)
     starts = starts.contiguous()
     counts = counts.contiguous() if counts is not None else None
     batch, heads, tokens, dim = (int(x) for x in k.shape)
@@ -276,7 +283,7 @@ def run_sdpa_kv_cache(q, cache, page_table, lengths, counts, causal, scale, retu
     if out.numel() == 0:
         return (out, lse) if return_lse else out
     q = _rows(q.detach())
-    page_table = page_table if page_table.stride(1) == 1 else page_table.contiguous()
+    page_table = _table_rows(page_table)
     lengths = lengths.contiguous()
     counts = counts.contiguous() if counts is not None else None
     kv_heads = int(cache[0].shape[1])
