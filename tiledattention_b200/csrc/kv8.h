@@ -62,6 +62,11 @@ __host__ __device__ __forceinline__ SlotSpan slot_span(int64_t start, int64_t co
   return {static_cast<int>(lo - first), static_cast<int>(hi - first), lo - start};
 }
 
+// Pages that T > 0 tokens touch at most.
+__host__ __device__ __forceinline__ int64_t slots_for(int T, int page) {
+  return (static_cast<int64_t>(T) + page - 2) / page + 1;
+}
+
 struct AppendParams {
   const void* x[2];               // k, v: [B, Hkv, T, D], 16-bit
   int64_t sb[2], sh[2], ss[2];    // element strides (dim stride 1)
@@ -143,6 +148,11 @@ __host__ __device__ __forceinline__ SeqExtent checked_extent(int length, int cou
   return e;
 }
 
+// Tiles of `tile` keys that hold n, for every n >= 0: n + tile - 1 may pass 2^31.
+__host__ __device__ __forceinline__ int tiles_for(int n, int tile) {
+  return static_cast<int>((static_cast<uint32_t>(n) + static_cast<uint32_t>(tile) - 1u) / static_cast<uint32_t>(tile));
+}
+
 // Key tiles of rows [row0, row0 + n) of a sequence's `rows` rows (token, head of the group):
 // up to the last key that any of them sees.
 __host__ __device__ __forceinline__ int block_tiles(const SeqExtent& e, int rows, uint32_t recip, int row0,
@@ -152,7 +162,7 @@ __host__ __device__ __forceinline__ int block_tiles(const SeqExtent& e, int rows
   const int first = divide_by_group(row0, recip), last = divide_by_group(end - 1, recip);
   if (first >= e.count) return 0;
   const int lim = row_limit(e.length, e.count, last < e.count ? last : e.count - 1, causal);
-  return (lim + tile - 1) / tile;
+  return tiles_for(lim, tile);
 }
 
 // Work of the split kernel is a line of `total` tiles (sequence, then head and row block, then

@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendParams p, int s
 }  // namespace
 
 cudaError_t launch_append(const AppendParams& p, cudaStream_t stream) {
-  const int slots = (p.T + p.page - 2) / p.page + 1;  // pages that T tokens touch at most
+  const int slots = static_cast<int>(slots_for(p.T, p.page));
   const int64_t blocks = static_cast<int64_t>(p.B) * slots;
   if (blocks > 0x7fffffffll || p.Hkv > 65535) return cudaErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(blocks), p.Hkv, 2);

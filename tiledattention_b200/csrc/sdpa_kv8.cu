@@ -161,7 +161,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return r;
 }
 __device__ __forceinline__ int tiles_of(const SeqExtent& e, int tile) {
-  return e.count > 0 ? (e.length + tile - 1) / tile : 0;
+  return e.count > 0 ? tiles_for(e.length, tile) : 0;
 }
 // On the line, rows of one (sequence, head) take a unit for each tile, behind kBefore units for their
 // queries and their merge. Without these units a run over many short sequences ends last (32
@@ -282,9 +282,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
     const int32_t* row = p.table + ahead.b * p.table_stride;
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) {
-      const int key = (ahead.tile + lane) * C::kTile + warp * kKeys + i * 16;
+      const uint32_t key = static_cast<uint32_t>(ahead.tile + lane) * C::kTile + warp * kKeys + i * 16;
       held_plane[i] = -1;
-      if (lane < held && key < ahead.length) {
+      if (lane < held && key < static_cast<uint32_t>(ahead.length)) {
         const int id = row[key >> p.page_shift];
         const bool good = static_cast<unsigned>(id) < static_cast<unsigned>(p.num_pages);
         held_plane[i] = good ? id * p.Hkv + ahead.h : -2;
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
       // t = score * c + ev in the scores' place, by the scales of the block's page
       float back[kBlocks];
       const uint32_t marks = left_out >> ((step & 3) * kBlocks) & ((1u << kBlocks) - 1);
-      const bool masked = key0 + kKeys > safe || marks;  // some row's limit, or pages to leave out
+      const bool masked = key0 > safe - kKeys || marks;  // some row's limit, or pages to leave out
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
         const uint32_t at = scales + ((step & 3) * 2 * kBlocks + i) * 4;
@@ -603,12 +603,12 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
       // that were not copied, and keys that some row does not see (the rest of the last page,
       // later tokens of the same call).
       const uint32_t marks = left_out >> ((step & 3) * kBlocks) & ((1u << kBlocks) - 1);
-      if (key0 + kKeys > safe || marks) {
+      if (key0 > safe - kKeys || marks) {
 #pragma unroll 1
         for (int i = 0; i < kBlocks; ++i) {
           const bool copied = key0 + i * 16 < cur.length && !(marks >> i & 1);
           bool nan = !copied;
-          if (copied && key0 + i * 16 + 16 > safe)
+          if (copied && key0 + i * 16 > safe - 16)
             for (int x = lane; x < 64 * NJ; x += 32)
               nan |= any_nan(lds128(vb + chunk_at<C::kCols, C::kPlane>(i * 16 + x / (NJ * 4), x % (NJ * 4))));
           if (!__any_sync(0xffffffffu, nan)) continue;

@@ -466,8 +466,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
           if (!ok) return a;
           a.h = w.s.h;
           a.tile = Tile{(w.s.t0 + j) * kTileKeys, w.s.length, w.s.safe, seg - 1};
-          const int key = a.tile.key0 + lane * 16;
-          if (lane < kGroups && key < w.s.length) {
+          const uint32_t key = static_cast<uint32_t>(a.tile.key0) + lane * 16;
+          if (lane < kGroups && key < static_cast<uint32_t>(w.s.length)) {
             a.id = p.table[w.s.b * p.table_stride + (key >> p.page_shift)];
             if (static_cast<unsigned>(a.id) >= static_cast<unsigned>(p.num_pages)) a.id = -2;
           }
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       }
       for (int tile_no = 1; ok && now.length >= 0; ++tile_no) {
         const int key0 = now.key0;
-        const bool edge = key0 + kTileKeys > now.safe;  // values that some row does not see
+        const bool edge = key0 > now.safe - kTileKeys;  // values that some row does not see
         int* const nan_here = nan_key + now.seg % kSegs * D;
         int* const any_nan = &bars->any_nan[now.seg % kSegs];
         ok = wait_meta(tile_no);  // the next tile's pages
@@ -762,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
                       *reinterpret_cast<uint32_t(*)[32]>(x + 32));
             tmem_wait_ld();
             const int key0 = (s.t0 + (j2 >> 1)) * kTileKeys + half * kHalfKeys;
-            if (key0 + kHalfKeys > safe) {
+            if (key0 > safe - kHalfKeys) {
               const int visible = lim - key0;
 #pragma unroll
               for (int i = 0; i < 64; ++i)
