@@ -34,6 +34,13 @@ __device__ __forceinline__ float pow2f(int e) {
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
+// What takes a row of q whose largest magnitude is amax < 2^(ex + 15) into [2^14, 2^15). A row with an
+// infinity becomes NaN: so are all its softmax weights (its scores are infinities and NaN, but all of them may
+// be -inf, which alone would look like a row without keys).
+__device__ __forceinline__ float row_factor(float amax, int ex) {
+  return amax == INFINITY ? __int_as_float(0x7fffffff) : pow2f(-ex);
+}
+
 // log2 and reciprocal of a value scale as it is stored, its exponent held in range: exact for powers
 // of two, which is what this library writes.
 struct ValueScale {

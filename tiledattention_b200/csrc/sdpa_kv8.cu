@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
         // every bf16 or fp16 value of the row to 2^-39 of the largest. Held to exponents whose
         // factors are normal float32 values.
         const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 14, -126), 113);
-        const float up = pow2f(-ex), factor = p.scale_log2 * pow2f(ex);
+        const float up = row_factor(amax, ex), factor = p.scale_log2 * pow2f(ex);
         uint32_t f[NJ * 4][2];
 #pragma unroll
         for (int c = 0; c < NJ * 4; ++c) {

@@ -721,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             }
           }
           const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 14, -126), 113);
-          const float up = pow2f(-ex);
+          const float up = row_factor(amax, ex);
           mul = p.scale_log2 * pow2f(ex);
           uint8_t* dst = q_smem + t * C::kTileBytes + r_in_tile * 128;
 #pragma unroll 1
