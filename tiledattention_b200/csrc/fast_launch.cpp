@@ -37,6 +37,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
@@ -185,6 +186,9 @@ PyObject* launch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     Py_DECREF(po);
     Py_DECREF(pl);
     return tup;
+  } catch (python_error& e) {  // of Python code that torch called: its own, not ours to answer
+    e.restore();
+    return nullptr;
   } catch (const std::exception&) {
     // Any ATen error (e.g. out of memory on the output): leave it to the full path, which
     // raises it through torch's own error translation.
@@ -351,6 +355,9 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     } else if (!rotary_launch(*q, k, *pos, *freq, how, qo, ko)) {
       Py_RETURN_NONE;
     }
+  } catch (python_error& e) {  // of Python code that torch called: its own, not ours to answer
+    e.restore();
+    return nullptr;
   } catch (const std::exception&) {
     Py_RETURN_NONE;
   }
@@ -433,6 +440,9 @@ PyObject* kv8_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (rc != 0) Py_RETURN_NONE;
     ++g_launches;
     Py_RETURN_TRUE;
+  } catch (python_error& e) {  // of Python code that torch called: its own, not ours to answer
+    e.restore();
+    return nullptr;
   } catch (const std::exception&) {
     Py_RETURN_NONE;
   }
@@ -492,6 +502,9 @@ PyObject* sdpa_kv8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(o)));
     PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(lse)));
     return out;
+  } catch (python_error& e) {  // of Python code that torch called: its own, not ours to answer
+    e.restore();
+    return nullptr;
   } catch (const std::exception&) {
     Py_RETURN_NONE;
   }
