@@ -51,11 +51,7 @@ constexpr int kTileRows = 128, kTileKeys = 128;
 constexpr int kHalfKeys = kTileKeys / 2;  // keys of a score half
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-// Register split of the launch's 512 x 128 registers: softmax, converters, MMA and idle.
 constexpr int kLaunchRegs = 128;
-constexpr int kSoftmaxRegs = 160, kConvertRegs = 128, kSideRegs = 64;
-static_assert(128 * (2 * kSoftmaxRegs + kConvertRegs + kSideRegs) == kThreads * kLaunchRegs,
-              "register split must match the launch allocation");
 constexpr uint32_t kTmemCols = 512;
 constexpr float kBelow = 7.f, kGrowth = 15.f;  // see sdpa_kv8.cu
 // t - ref comes out of one multiply-add on the score and so is more exact than ref, which is a rounded t
@@ -72,6 +68,12 @@ template <int D>
 struct Cfg {
   static constexpr int kTiles = D == 256 ? 1 : 2;
   static constexpr int kRows = kTiles * kTileRows;
+  // Register split of the launch's 512 x 128 registers: softmax (a group of 128 threads a row tile),
+  // converters (the rest of warps 0-11), the others. With one row tile these have no spills (with two
+  // their walk over the line has): 2 x 1024 tokens at the end of 8192, head dim 256, 890 us; with 64 for them 980.
+  static constexpr int kSoftmaxRegs = 160, kConvertRegs = 128, kSideRegs = kTiles == 2 ? 64 : 96;
+  static_assert(128 * (kTiles * kSoftmaxRegs + (3 - kTiles) * kConvertRegs + kSideRegs) == kThreads * kLaunchRegs,
+                "register split must match the launch allocation");
   static constexpr int kTileBytes = kTileRows * D * 2;  // a q tile, or a K or V unit
   static constexpr int kStages = D == 64 ? 6 : D == 128 ? 4 : 2;
   static constexpr int kChunks = D / 16;                // 16-code chunks of a key
@@ -326,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
     }
 
   if (warp >= 12) {
-    regs_dec<kSideRegs>();
+    regs_dec<C::kSideRegs>();
     if (warp == 12 || (warp == 15 && C::kTiles == 2)) {
       // ------------------------------------------------------------ MMA issuers
       if (lane == 0 && has_run) {
@@ -538,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
     }
   } else if (warp >= (C::kTiles == 2 ? 8 : 4)) {
     // ------------------------------------------------------------ converters
-    regs_dec<kConvertRegs>();
+    regs_dec<C::kConvertRegs>();
     if (has_run) {
       constexpr int kRowsPerPass = 128 / C::kChunks;  // of 128 threads, 16 codes each
       // The passes of a tile are in flight, of K and V, or where the second row tile's warps convert too
@@ -657,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
       if (!ok && threadIdx.x % 128 == 0 && !*abort_flag) report(p, TA_DEVSTAT_TIMEOUT_LOAD, abort_flag);
     }
   } else {
-    regs_inc<kSoftmaxRegs>();
+    regs_inc<C::kSoftmaxRegs>();
     // ------------------------------------------------------------ softmax + epilogue
     const int t = warp >> 2;  // row tile of this warpgroup
     if (t < C::kTiles && has_run) {
