@@ -114,8 +114,8 @@ namespace kv8 {
 // Many rows fill the chunk kernel's tiles of 128; few rows are served by the other kernel, whose time
 // grows with each 32 rows (16 above head dim 128) while the chunk kernel's stays. Measured, few-row
 // kernel and chunk kernel, 16 sequences of 8192, 8 cache heads: head dim 128, 32 rows
-// 106 and 176 us, 40 rows 183 and 175; head dim 256, 48 rows 278 and 285 us, 64 rows 377 and 285.
-// A single short sequence loses by it (2048 tokens, head dim 128, 40 rows: 23 and 28 us).
+// 108 and 173 us, 40 rows 184 and 174; head dim 256, 48 rows 272 and 274 us, 64 rows 382 and 275.
+// A single short sequence loses by it (2048 tokens, 2 cache heads, head dim 128, 40 rows: 20 and 25 us).
 bool uses_chunk(int rows, int D) { return rows > (D > 128 ? 48 : 32); }
 }  // namespace kv8
 }  // namespace ta

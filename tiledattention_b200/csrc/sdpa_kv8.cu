@@ -34,9 +34,9 @@
 // for up to 32 steps at once, and the reference of a row's weights moves (and is agreed on between
 // lanes) only when a score passes it by 2^15.
 //
-// Measured: 64 sequences of 16384, 64 heads over 8, head dim 128: 350 us, 6.1 TB/s (copying
-// alone, without any arithmetic: 335). 32 sequences of up to 4096, 32 heads over 8: 33 us,
-// 4.0 TB/s (5 us of it the merge kernel, 5 until the first keys are there). One of 777: 8 us.
+// Measured: 64 sequences of 16384, 64 heads over 8, head dim 128: 347 us, 6.2 TB/s (copying
+// alone, without any arithmetic: 335). 32 sequences of up to 4096, 32 heads over 8: 32 us,
+// 4.1 TB/s (5 us of it the merge kernel, 5 until the first keys are there). One of 777: 8 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -68,7 +68,8 @@ struct Cfg {
   // Blocks a SM, as the registers allow (the output takes 16 NJ NT of them, q 8 NJ NT where it
   // is not shared), and the ring's units, as shared memory then allows. One block more costs
   // spills and time: 16 sequences of 8192, 8 heads, head dim 128, 16 rows 91 us with 3 blocks,
-  // 64 with 2; head dim 64, 32 rows 101 and 68.
+  // 66 with 2; head dim 64, 32 rows 101 and 69. <2, 4> and <4, 2> spill with 2 blocks too (338 and 54
+  // bytes of stores at 255 registers).
   static constexpr bool kQShared = NJ * NT > 6;
   static constexpr int kBlocksPerSm = NJ * NT == 1 ? 4 : NJ * NT == 2 ? 3 : 2;
   static constexpr int kUnits = NJ == 1 ? 6 : NJ == 2 ? (NT == 1 ? 4 : NT == 2 ? 6 : 5) : 3;
@@ -773,8 +774,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<NJ, NT>::kBlocksPerSm))
 
 // Merges the partial results of (sequence, head)s that several runs share, and writes the rows
 // of sequences without keys: both by the attend kernel's records, and nothing of it is read before
-// that kernel has ended (lengths read earlier, while it runs, would save 0.4 us of 32). One block: kWarps rows, a warp each, or with `spread` one row
-// whose runs the warps divide (few rows, many runs).
+// that kernel has ended (lengths read earlier, while it runs, would save 0.4 us of 32). One block: kWarps
+// rows, a warp each, or with `spread` one row whose runs the warps divide (few rows, many runs).
 template <int NJ, int NT>
 __global__ void __launch_bounds__(kThreads) merge_kernel(const AttendParams p, int parts, int spread) {
   using C = Cfg<NJ, NT>;

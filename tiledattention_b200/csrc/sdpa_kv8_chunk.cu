@@ -27,9 +27,10 @@
 // CTA: causal blocks of different length and uneven sequences fill the GPU evenly. A block that is
 // cut leaves partial results, merged by a second kernel that starts before this one ends.
 //
-// Measured: 2 x 1024 tokens of 32 heads (8 in the cache) at the end of 8192, head dim 128: 326 us,
-// 792 TFLOP/s of those that the masks leave. A tile takes some 5000 clocks, of which the MMAs are
-// 2 x 634 and softmax's own instructions most of the rest; a block's start and end take some
+// Measured: 2 x 1024 tokens of 32 heads (8 in the cache) at the end of 8192, head dim 128: 319 us,
+// 808 TFLOP/s of those that the masks leave. A tile takes some 5000 clocks, of which the MMAs are
+// 2 x 634; most stalls are on scores from tensor memory and on fixed latencies, and the walk over the
+// line spills (some 580 bytes of loads, with two row tiles). A block's start and end take some
 // 18000 (its rows of q, the first scores, the last weights, the output).
 //
 // Every wait is bounded: on expiry the kernel records TA_DEVSTAT_* bits, drains its MMAs, frees

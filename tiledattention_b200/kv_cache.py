@@ -149,7 +149,8 @@ def kv_cache_append(k, v, cache: KVCache8, page_table, starts, *, counts=None) -
 
     Runs asynchronously on the current torch stream. Page ids outside the cache are skipped, and
     starts and counts outside their range held in range: both are reported by
-    check_device_status(). Pages that two sequences write in one call have no defined content.
+    check_device_status(). Pages that two sequences, or two slots of one, write in one call have no
+    defined content.
     """
     fast = _native._fast
     if fast is not None and _runtime._runtime_ready and _async_mode() and type(cache) is KVCache8:

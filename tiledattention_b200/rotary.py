@@ -34,7 +34,10 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str =
               leaves the fastest.
     "yarn"    pairs that turn at least `fast` times over the original context keep their speed,
               those that turn at most `slow` times are divided by factor, a linear ramp in
-              turns between; magnitude 0.1 ln(factor) + 1.
+              turns between, as the method's paper has it; magnitude 0.1 ln(factor) + 1. Many
+              published checkpoints were made with a ramp linear in the pair's index, whose
+              frequencies between differ (up to some 2 times): pass rotary() such a model's own
+              inv_freq.
     "bands"   as "yarn" with magnitude 1.
     """
     torch_mod = _runtime.get_torch_module()
