@@ -64,6 +64,12 @@ def _check(dev):
         with torch.no_grad():  # says nothing about forward mode
             out = ta.rotary(fwad.make_dual(q, dq), None, pos, freq, **how)[0]
         assert torch.equal(_tangent(out), turned_q)
+        zero = fwad.make_dual(q, torch._efficientzerotensor(q.shape, dtype=q.dtype, device=dev))
+        for other in (k, fwad.make_dual(k, dk)):
+            oq, ok = ta.rotary(zero, other, pos, freq, **how)
+            assert _tangent(oq) is None or not _tangent(oq).any()
+            assert torch.equal(fwad.unpack_dual(oq).primal, want_q)
+            assert other is k or torch.equal(_tangent(ok), turned_k)
         out = ta.rotary(q, k, pos, freq, **how)  # a level, but no tangent
         assert _tangent(out[0]) is None and torch.equal(out[0], want_q)
         # both modes: the gradient of the turned tangent, and of the value

@@ -200,8 +200,11 @@ def _forward_mode(torch_mod, q, k, positions, inv_freq, **how):
     if not torch_mod._C._is_fwd_grad_enabled():
         return None
     (q, dq), (k, dk) = (fwad.unpack_dual(t) if t is not None else (None, None) for t in (q, k))
+    dual = dq is not None or dk is not None
+    # torch's tangents of zero may have no memory to read; a zero turns into a zero, which is none
+    dq, dk = (None if d is None or d._is_zerotensor() else d for d in (dq, dk))
     if dq is None and dk is None:
-        return None
+        return rotary(q, k, positions, inv_freq, **how) if dual else None
     q, k = rotary(q, k, positions, inv_freq, **how)
     if dq is not None:
         dq, dk = rotary(dq, dk, positions, inv_freq, **how)
